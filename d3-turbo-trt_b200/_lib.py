@@ -7,6 +7,7 @@ CUDA stream of the tensor's device.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -41,6 +42,21 @@ class CopySegment(ctypes.Structure):
         ("dst_row_stride", ctypes.c_int64),
     ]
 
+
+class Kv4CacheStruct(ctypes.Structure):
+    """``d3b_kv4_cache``: a pool of 4-bit key/value pages."""
+
+    _fields_ = [
+        ("pool", ctypes.c_void_p),
+        ("layers", ctypes.c_int64),
+        ("pages", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("page_tokens", ctypes.c_int),
+    ]
+
+
+_CACHE = ctypes.POINTER(Kv4CacheStruct)
 
 SIGNATURES: list[tuple[str, Any, list[Any]]] = [
     ("d3b_version", _I, []),
@@ -87,6 +103,21 @@ SIGNATURES: list[tuple[str, Any, list[Any]]] = [
     ),
     ("d3b_gated_delta_workspace_size", _SZ, [_I, _I, _I]),
     ("d3b_gated_delta_state_workspace_size", _SZ, [_I, _I, _I, _I, _I]),
+    ("d3b_kv4_page_bytes", _I64, [_I, _I, _I]),
+    ("d3b_kv4_append", _I, [_CACHE, _I64, _VP, _I64P, _VP, _I64P, _VP, _I64, _I, _VP]),
+    ("d3b_kv4_read", _I, [_CACHE, _I64, _VP, _I64, _I64, _VP, _VP, _I, _VP]),
+    ("d3b_kv4_move_pages", _I, [_CACHE, _VP, _VP, _I64, _VP, _I64, _VP]),
+    ("d3b_kv4_decode_workspace_size", _SZ, [_CACHE, _I, _I, _I, _I64]),
+    (
+        "d3b_kv4_decode",
+        _I,
+        [_CACHE, _I64, _VP, _I64P, _VP, _I64, _I64, _VP, _I, _I, _I, _I, _I, _F, _VP, _I64P, _VP, _SZ, _VP],
+    ),
+    (
+        "d3b_qk_norm_mrope",
+        _I,
+        [_VP, _I64P, _I, _VP, _I64P, _I, _VP, _VP, _VP, _I64P, _VP, _VP, _I, _I, _VP, _VP, _I, _I, _I, _I, _F, _VP],
+    ),
     ("d3b_copy_segments", _I, [ctypes.POINTER(CopySegment), _I, _VP]),
     ("d3b_arena_create", _I, [_U64, _U64, ctypes.POINTER(ctypes.c_void_p)]),
     ("d3b_arena_alloc", _I, [_VP, _U64, _U64P]),
@@ -135,6 +166,20 @@ def stream_of(t: torch.Tensor) -> ctypes.c_void_p:
 
 def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
+
+
+def on_device(device: torch.device) -> Any:
+    """Context with ``device`` as the current one (nothing is switched where it is already)."""
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def rows16(t: torch.Tensor) -> torch.Tensor:
+    """``t`` where its last dimension is contiguous and every row starts on 16 bytes (16-bit types), else a copy."""
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in t.stride()[:-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def i64_array(values) -> Any:

@@ -1,0 +1,301 @@
+"""Key/value cache in 4 bits, in pages, and the attention that reads it (sm_100a).
+
+``Kv4Cache`` is a pool of pages for every layer; a page holds ``page_tokens`` tokens' keys and
+values of all kv heads. A row is kept as e2m1 codes with one e4m3 scale for 16 channels and one
+power of two: 4.56 bits a value at head_dim 128, against 16 in a snapshot (the layout is written
+down in ``include/d3b200.h``). What a row reads back as is exactly representable in bf16 and, up to
+its largest magnitude, in fp16.
+
+* ``cache.append(layer, k, v, slots)`` quantises rows into slots (page * page_tokens + place);
+* ``cache.read(layer, table, tokens)`` gives a sequence's rows back in 16 bits;
+* ``cache.copy_pages(src, dst)`` / ``cache.move_pages(src, dst, tables)`` copy pages of every
+  layer, the latter rewriting page tables in the same launch;
+* ``decode_attention(q, cache, layer, table, lengths, scale=...)`` attends with the newest tokens
+  of many sequences, each over its own pages;
+* ``question_attention(q, cache, layer, table, state_len, k_q, v_q, lengths, scale=...)`` is
+  ``prefix_bidir_attention`` over a state that lies in the cache.
+
+Page numbers, slots and lengths given as device tensors are not read on the host: the kernels leave
+out what does not fit the pool or the table and set the device error word (``SITE_BAD_SLOT``,
+``SITE_BAD_PAGE``, ``SITE_BAD_LENGTH``, ``SITE_BAD_MOVE``; ``_lib.device_error()`` reads it).
+A row that held a NaN or an infinity reads back as NaN.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Sequence
+
+import torch
+
+from .. import _lib
+from .prefix_bidir import _launch as _prefix_bidir, block_offsets
+
+HEAD_DIMS = (64, 128, 256)
+PAGE_TOKENS = (16, 32, 64, 128, 256)
+SITE_BAD_SLOT, SITE_BAD_PAGE, SITE_BAD_LENGTH, SITE_BAD_MOVE = 2101, 2102, 2103, 2104
+
+_TYPES = (torch.float16, torch.bfloat16)
+
+
+def page_bytes(kv_heads: int, head_dim: int, page_tokens: int) -> int:
+    """Bytes of one page of one layer."""
+    _check_shape(kv_heads, head_dim, page_tokens)
+    return kv_heads * (page_tokens // 16) * (18 * head_dim + 32)
+
+
+def _check_shape(kv_heads: int, head_dim: int, page_tokens: int) -> None:
+    if head_dim not in HEAD_DIMS:
+        raise RuntimeError(f"unsupported head_dim {head_dim}")
+    if page_tokens not in PAGE_TOKENS:
+        raise RuntimeError(f"page_tokens must be one of {PAGE_TOKENS}, got {page_tokens}")
+    if not 0 < kv_heads <= 65535:
+        raise RuntimeError(f"kv_heads must lie in [1, 65535], got {kv_heads}")
+
+
+def _index(t: torch.Tensor, dtype: torch.dtype, device: torch.device, what: str) -> None:
+    if t.dtype != dtype or t.device != device:
+        raise RuntimeError(f"{what} must be {dtype} on {device}, got {t.dtype} on {t.device}")
+
+
+class Kv4Cache:
+    """``pool`` [layers, pages, page_bytes] uint8, allocated here or, with ``over``, the caller's."""
+
+    def __init__(self, layers: int, pages: int, *, kv_heads: int, head_dim: int, page_tokens: int = 64,
+                 device: torch.device | str | int | None = None):
+        if layers < 0 or pages < 0:
+            raise RuntimeError("layers and pages must not be negative")
+        size = page_bytes(kv_heads, head_dim, page_tokens)
+        dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        if dev.type != "cuda":
+            raise RuntimeError("the 4-bit cache needs CUDA")
+        self._adopt(torch.empty(layers, pages, size, dtype=torch.uint8, device=dev), kv_heads, head_dim, page_tokens)
+
+    @classmethod
+    def over(cls, pool: torch.Tensor, *, kv_heads: int, head_dim: int, page_tokens: int = 64) -> "Kv4Cache":
+        """A cache over an existing uint8 buffer [layers, pages, page_bytes] (contiguous, not copied)."""
+        size = page_bytes(kv_heads, head_dim, page_tokens)
+        if not pool.is_cuda:
+            raise RuntimeError("the 4-bit cache needs CUDA")
+        if pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[2] != size:
+            raise RuntimeError(f"pool must be uint8 [layers, pages, {size}], got {pool.dtype} {tuple(pool.shape)}")
+        if not pool.is_contiguous() or pool.data_ptr() % 16:
+            raise RuntimeError("pool must be contiguous and 16-byte aligned")
+        cache = cls.__new__(cls)
+        cache._adopt(pool, kv_heads, head_dim, page_tokens)
+        return cache
+
+    def _adopt(self, pool: torch.Tensor, kv_heads: int, head_dim: int, page_tokens: int) -> None:
+        self.pool, self.kv_heads, self.head_dim, self.page_tokens = pool, kv_heads, head_dim, page_tokens
+        self.layers, self.pages = pool.shape[0], pool.shape[1]
+        self.device = pool.device
+        self._c = _lib.Kv4CacheStruct(pool.data_ptr(), self.layers, self.pages, kv_heads, head_dim, page_tokens)
+        self._ref = ctypes.byref(self._c)
+
+    @property
+    def nbytes(self) -> int:
+        return self.pool.numel()
+
+    def _check_layer(self, layer: int) -> None:
+        if not 0 <= layer < self.layers:
+            raise RuntimeError(f"layer {layer} of {self.layers}")
+
+    def slots(self, pages: Sequence[int] | torch.Tensor, start: int, count: int) -> torch.Tensor:
+        """int64 slots of tokens ``start`` .. ``start + count`` of the sequence whose pages these are."""
+        table = torch.as_tensor(pages, dtype=torch.int64, device=self.device)
+        if start < 0 or count < 0 or start + count > table.numel() * self.page_tokens:
+            raise RuntimeError(f"tokens {start} .. {start + count} of {table.numel()} pages")
+        at = torch.arange(start, start + count, device=self.device)
+        return table[at // self.page_tokens] * self.page_tokens + at % self.page_tokens
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        """Quantise rows k, v [n, kv_heads, head_dim] (fp16 or bf16, any token and head strides) into ``slots``.
+
+        ``slots`` [n] int64 on the device; a negative slot leaves its row out. Slots must differ: one
+        that is named twice holds a mixture of the rows."""
+        self._check_layer(layer)
+        shape = (slots.numel(), self.kv_heads, self.head_dim)
+        if slots.dim() != 1 or tuple(k.shape) != shape or tuple(v.shape) != shape:
+            raise RuntimeError(f"k and v must be [n, {self.kv_heads}, {self.head_dim}] and slots [n], got "
+                               f"{tuple(k.shape)}, {tuple(v.shape)}, {tuple(slots.shape)}")
+        if k.dtype not in _TYPES or v.dtype != k.dtype or k.device != self.device or v.device != self.device:
+            raise RuntimeError(f"k and v must be fp16 or bf16 on {self.device}, got {k.dtype} on {k.device} and "
+                               f"{v.dtype} on {v.device}")
+        _index(slots, torch.int64, self.device, "slots")
+        if shape[0] == 0:
+            return
+        k, v, slots = _lib.rows16(k), _lib.rows16(v), slots.contiguous()
+        with _lib.on_device(self.device):
+            status = _lib.lib().d3b_kv4_append(
+                self._ref, layer, k.data_ptr(), _lib.i64_array(k.stride()[:2]), v.data_ptr(),
+                _lib.i64_array(v.stride()[:2]), slots.data_ptr(), shape[0], _lib.dtype_code(k.dtype), _lib.stream_of(k))
+        _lib.check(status, "d3b_kv4_append")
+
+    def read(self, layer: int, table: torch.Tensor, tokens: int, *, dtype: torch.dtype = torch.bfloat16,
+             ) -> tuple[torch.Tensor, torch.Tensor]:
+        """(k, v) [kv_heads, tokens, head_dim] of the first ``tokens`` tokens of pages ``table`` [n] int32."""
+        self._check_layer(layer)
+        if dtype not in _TYPES:
+            raise RuntimeError(f"read gives fp16 or bf16, not {dtype}")
+        self._check_table(table, tokens)
+        both = torch.empty(2, self.kv_heads, tokens, self.head_dim, dtype=dtype, device=self.device)
+        k, v = both.unbind(0)
+        if tokens:
+            table = table.contiguous()
+            with _lib.on_device(self.device):
+                status = _lib.lib().d3b_kv4_read(self._ref, layer, table.data_ptr(), table.numel(), tokens, k.data_ptr(),
+                                                 v.data_ptr(), _lib.dtype_code(dtype), _lib.stream_of(both))
+            _lib.check(status, "d3b_kv4_read")
+        return k, v
+
+    def _check_table(self, table: torch.Tensor, tokens: int) -> None:
+        _index(table, torch.int32, self.device, "table")
+        if table.dim() != 1 or not 0 <= tokens <= table.numel() * self.page_tokens:
+            raise RuntimeError(f"{tokens} tokens in a table of shape {tuple(table.shape)} and pages of {self.page_tokens}")
+
+    def copy_pages(self, src: torch.Tensor | Sequence[int], dst: torch.Tensor | Sequence[int]) -> None:
+        """Copy page ``src[i]`` to page ``dst[i]`` in every layer. No destination may be a source or
+        stand twice (checked for lists; for device tensors that is the caller's part)."""
+        self._move(src, dst, None)
+
+    def move_pages(self, src: torch.Tensor | Sequence[int], dst: torch.Tensor | Sequence[int],
+                   tables: torch.Tensor) -> None:
+        """``copy_pages``, and every entry of ``tables`` (int32, contiguous) that is some ``src[i]``
+        becomes ``dst[i]``, in one launch. ``src`` must be ascending (the kernel records a list that
+        is not, or a destination among the sources, in the device error word)."""
+        _index(tables, torch.int32, self.device, "tables")
+        if not tables.is_contiguous():
+            raise RuntimeError("tables must be contiguous")
+        self._move(src, dst, tables)
+
+    def _move(self, src, dst, tables) -> None:
+        if not isinstance(src, torch.Tensor) and not isinstance(dst, torch.Tensor):
+            src, dst = [int(p) for p in src], [int(p) for p in dst]
+            if len(set(src) | set(dst)) < len(set(src)) + len(dst):
+                raise RuntimeError("a destination is a source or stands twice")
+            if tables is not None and any(a >= b for a, b in zip(src, src[1:])):
+                raise RuntimeError("src must be ascending")
+            if any(not 0 <= p < self.pages for p in src + dst):
+                raise RuntimeError(f"pages must lie in [0, {self.pages})")
+            both = torch.tensor([src, dst], dtype=torch.int32).to(self.device)
+            src, dst = both[0], both[1]
+        else:
+            src, dst = (t if isinstance(t, torch.Tensor) else torch.tensor(list(t), dtype=torch.int32, device=self.device)
+                        for t in (src, dst))
+        _index(src, torch.int32, self.device, "src")
+        _index(dst, torch.int32, self.device, "dst")
+        n = src.numel()
+        if src.dim() != 1 or dst.shape != src.shape or n > self.pages:
+            raise RuntimeError(f"src and dst must be [n] with n <= {self.pages}, got {tuple(src.shape)}, {tuple(dst.shape)}")
+        if n == 0:
+            return
+        src, dst = src.contiguous(), dst.contiguous()
+        with _lib.on_device(self.device):
+            status = _lib.lib().d3b_kv4_move_pages(self._ref, src.data_ptr(), dst.data_ptr(), n, _lib.ptr(tables),
+                                                   0 if tables is None else tables.numel(), _lib.stream_of(src))
+        _lib.check(status, "d3b_kv4_move_pages")
+
+
+def _check_query(q: torch.Tensor, cache: Kv4Cache, layer: int) -> None:
+    if not q.is_cuda or q.device != cache.device:
+        raise RuntimeError(f"q is on {q.device}, the cache on {cache.device}")
+    if q.dtype not in _TYPES:
+        raise RuntimeError("the 4-bit cache's attention needs fp16 or bf16 queries")
+    cache._check_layer(layer)
+    if q.shape[-1] != cache.head_dim:
+        raise RuntimeError(f"q has head_dim {q.shape[-1]}, the cache {cache.head_dim}")
+    if q.shape[1] == 0 or q.shape[1] % cache.kv_heads:
+        raise RuntimeError("heads must be divisible by kv heads")
+
+
+def _check_out(out: torch.Tensor, q: torch.Tensor) -> None:
+    if (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(-1) != 1
+            or out.data_ptr() % 16 or any(s % 8 for s in out.stride()[:-1])):
+        raise RuntimeError("out must be like q, with a contiguous last dimension and 16-byte aligned rows")
+
+
+def decode_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torch.Tensor, lengths: torch.Tensor, *,
+                     scale: float, causal: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the newest tokens of B sequences over their cached keys and values.
+
+    q [B, H, L, D] (any strides, D contiguous) or [B, H, D] for one token each; ``table`` [B, width]
+    int32 page numbers (entries behind a sequence's last page are not read); ``lengths`` [B] int32
+    tokens in the cache, the L newest among them already appended. Every token sees all ``lengths[b]``
+    tokens, or with ``causal`` those up to itself. Rows without a key are zero. Returns a tensor like q.
+    """
+    single = q.dim() == 3
+    if single:
+        q = q.unsqueeze(2)
+        out = None if out is None else out.unsqueeze(2)
+    if q.dim() != 4:
+        raise RuntimeError(f"q must be [B, H, L, D] or [B, H, D], got {tuple(q.shape)}")
+    _check_query(q, cache, layer)
+    rows, heads, width, _ = q.shape
+    device = cache.device
+    _index(table, torch.int32, device, "table")
+    _index(lengths, torch.int32, device, "lengths")
+    if table.dim() != 2 or table.shape[0] != rows or tuple(lengths.shape) != (rows,):
+        raise RuntimeError(f"table must be [{rows}, width] and lengths [{rows}], got {tuple(table.shape)}, "
+                           f"{tuple(lengths.shape)}")
+    q = _lib.rows16(q)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    else:
+        _check_out(out, q)
+    if rows and width:
+        if table.shape[1] and (table.stride(1) != 1 or table.stride(0) < 0):
+            table = table.contiguous()
+        lengths = lengths.contiguous()
+        lib = _lib.lib()
+        with _lib.on_device(device):
+            need = lib.d3b_kv4_decode_workspace_size(cache._ref, rows, heads, width, table.shape[1])
+            # from the caching allocator at every call: calls on other streams and captured graphs
+            # get their own, and it is ordered with the stream like any tensor
+            work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+            status = lib.d3b_kv4_decode(
+                cache._ref, layer, q.data_ptr(), _lib.i64_array(q.stride()[:3]), table.data_ptr(), table.stride(0),
+                table.shape[1], lengths.data_ptr(), rows, heads, width, int(causal), _lib.dtype_code(q.dtype), float(scale),
+                out.data_ptr(), _lib.i64_array(out.stride()[:3]), _lib.ptr(work), need, _lib.stream_of(q))
+        _lib.check(status, "d3b_kv4_decode")
+    return out.squeeze(2) if single else out
+
+
+def question_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torch.Tensor, state_len: int,
+                       k_q: torch.Tensor, v_q: torch.Tensor, lengths: Sequence[int] | torch.Tensor, *, scale: float,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """Bidirectional question attention over a state in the cache: ``prefix_bidir_attention`` whose
+    state keys and values are the first ``state_len`` tokens of pages ``table`` [n] int32.
+
+    q [B, H, L, D], k_q/v_q [B, H_kv, L, D], ``lengths`` as there. Returns [B, H, L, D], zero rows
+    for padding.
+    """
+    if q.dim() != 4:
+        raise RuntimeError(f"q must be [B, H, L, D], got {tuple(q.shape)}")
+    _check_query(q, cache, layer)
+    rows, heads, width, dim = q.shape
+    cache._check_table(table, state_len)
+    if k_q.dtype != q.dtype or v_q.dtype != q.dtype or k_q.device != q.device or v_q.device != q.device:
+        raise RuntimeError("q, k and v must share a dtype and a device")
+    if tuple(k_q.shape) != (rows, cache.kv_heads, width, dim) or v_q.shape != k_q.shape:
+        raise RuntimeError(f"k_q/v_q must be [B, H_kv, L, D] = {(rows, cache.kv_heads, width, dim)}")
+    if isinstance(lengths, torch.Tensor):
+        if lengths.numel() != rows:
+            raise RuntimeError(f"{lengths.numel()} lengths for {rows} question blocks")
+    else:
+        lengths = [int(n) for n in lengths]
+        if len(lengths) != rows or any(not 0 <= n <= width for n in lengths):
+            raise RuntimeError(f"lengths must be {rows} values in [0, {width}]")
+    if out is None:
+        out = torch.empty((rows, heads, width, dim), dtype=q.dtype, device=q.device)
+    else:
+        _check_out(out, q)
+    if rows == 0 or width == 0:
+        return out
+    with _lib.on_device(cache.device):
+        lens = block_offsets(lengths, q.device)
+        k, v = cache.read(layer, table, state_len, dtype=q.dtype)
+        k_q, v_q = _lib.rows16(k_q), _lib.rows16(v_q)
+        if k_q.stride() != v_q.stride():
+            k_q, v_q = (x.clone(memory_format=torch.contiguous_format) for x in (k_q, v_q))
+        _prefix_bidir(_lib.rows16(q), k, v, k_q, v_q, lens, scale, out)
+    return out

@@ -15,12 +15,17 @@ the bf16 normed / gated rows never travel through HBM:
   reference/d3_kernels.py:502-525 (``attn_out * sigmoid(gate)``, core.py:297).
 * ``sigmoid_gate_quant(attn_out, gate, mode)`` -> ``(q, scale)``: the gated rows
   quantised for o_proj.
+* ``qk_norm_rope`` / ``qk_norm_mrope``: the per-head norm of queries and keys with the partial
+  rotary embedding (core.py:233-237); the latter takes the positions themselves, on several axes,
+  and queries and keys in one launch.
 
 bf16 tensors on the GPU only; rows of up to 6144 elements (a multiple of 8),
-16-byte aligned. A ``RuntimeError`` names any other case; there is no fallback.
+16-byte aligned (``qk_norm_mrope``: fp16 too, head_dim 64, 128 or 256). A ``RuntimeError`` names any other case; there is no fallback.
 """
 
 from __future__ import annotations
+
+from typing import Sequence
 
 import torch
 
@@ -233,6 +238,90 @@ def qk_norm_rope(x: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor, sin: 
         _lib.stream_of(x))
     _lib.check(st, "d3b_qk_norm_rope")
     return out
+
+
+def rotary_axes(sections: Sequence[int], *, interleaved: bool = True) -> tuple[int, ...]:
+    """The position axis of every rotary frequency, for ``qk_norm_mrope``.
+
+    ``sections`` gives each axis' number of frequencies (their sum is half the rotary dimensions),
+    time first. Interleaved (the Qwen3.5 text model's order): axis a > 0 takes frequencies a, a + n,
+    a + 2n, ... (n axes) until its share is spent and axis 0 the others; else axis after axis.
+    """
+    sections = [int(s) for s in sections]
+    half, n = sum(sections), len(sections)
+    if not sections or min(sections) < 0:
+        raise ValueError(f"sections must be non-negative counts, got {sections}")
+    if not interleaved:
+        return tuple(a for a, s in enumerate(sections) for _ in range(s))
+    axes = [0] * half
+    for a in range(1, n):
+        taken = range(a, a + n * sections[a], n)
+        if sections[a] and taken[-1] >= half:
+            raise ValueError(f"sections {sections} do not interleave over {half} frequencies")
+        for i in taken:
+            axes[i] = a
+    return tuple(axes)
+
+
+_ROPE_TYPES = (torch.bfloat16, torch.float16)
+
+
+def qk_norm_mrope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                  positions: torch.Tensor, inv_freq: torch.Tensor, axes: Sequence[int],
+                  eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """q_norm and k_norm (Qwen3_5RMSNorm per head), then a rotary embedding over several position
+    axes (time, height, width), one launch for queries and keys.
+
+    q [rows, T, heads, D], k [rows, T, kv_heads, D] bf16 or fp16, D in {64, 128, 256} (any row, token
+    and head strides, last dim contiguous); weights [D] raw, the kernel applies 1 + w; positions
+    [axes, rows, T] int64; inv_freq [half] fp32, 2 * half <= D and half a multiple of 8; ``axes``
+    the axis of each frequency (``rotary_axes``). Text has equal positions on every axis.
+
+    Returns both as [rows, T, heads, D] token-major tensors. Computed in fp32 (angles in fp64) and
+    rounded once, where ``qk_norm_rope`` rounds after each of the reference's bf16 operations.
+    """
+    for x, what in ((q, "q"), (k, "k")):
+        if not x.is_cuda or x.dtype not in _ROPE_TYPES:
+            raise RuntimeError(f"qk_norm_mrope needs bf16 or fp16 CUDA tensors, got {what} {x.dtype} on {x.device}")
+        if x.dim() != 4 or (x.stride(-1) != 1 and x.shape[-1] != 1):
+            raise RuntimeError(f"qk_norm_mrope: {what} must be [rows, T, heads, D] with a contiguous last dim, got "
+                               f"{tuple(x.shape)} strides {x.stride()}")
+    rows, T, heads, D = q.shape
+    kv_heads = k.shape[2]
+    if k.dtype != q.dtype or k.device != q.device or k.shape[0] != rows or k.shape[1] != T or k.shape[3] != D:
+        raise RuntimeError(f"qk_norm_mrope: q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} do not match")
+    if D not in (64, 128, 256):
+        raise RuntimeError(f"unsupported head_dim {D}")
+    half = len(axes)
+    if half % 8 or 2 * half > D or inv_freq.dim() != 1 or inv_freq.numel() != half:
+        raise RuntimeError(f"qk_norm_mrope: {half} axes and {tuple(inv_freq.shape)} frequencies for head_dim {D}")
+    if inv_freq.dtype != torch.float32 or positions.dtype != torch.int64:
+        raise RuntimeError(f"qk_norm_mrope: inv_freq must be float32 and positions int64, got {inv_freq.dtype}, "
+                           f"{positions.dtype}")
+    if positions.dim() != 3 or positions.shape[1] != rows or positions.shape[2] != T or not 1 <= positions.shape[0] <= 8:
+        raise RuntimeError(f"qk_norm_mrope: positions must be [axes, {rows}, {T}], got {tuple(positions.shape)}")
+    if half and not 0 <= min(axes) <= max(axes) < positions.shape[0]:
+        raise RuntimeError(f"qk_norm_mrope: axes must lie in [0, {positions.shape[0]})")
+    device = q.device
+    if positions.device != device or inv_freq.device != device:
+        raise RuntimeError(f"qk_norm_mrope: positions and inv_freq must be on {device}")
+    if q_weight.numel() != D or k_weight.numel() != D:
+        raise RuntimeError(f"qk_norm_mrope: weights must have {D} values, got {q_weight.numel()} and {k_weight.numel()}")
+    q, k = _lib.rows16(q), _lib.rows16(k)
+    wq = _lib.rows16(q_weight.to(device=device, dtype=q.dtype))
+    wk = _lib.rows16(k_weight.to(device=device, dtype=q.dtype))
+    inv_freq = inv_freq.contiguous()
+    q_out = torch.empty(rows, T, heads, D, dtype=q.dtype, device=device)
+    k_out = torch.empty(rows, T, kv_heads, D, dtype=q.dtype, device=device)
+    if rows and T and heads + kv_heads:
+        with _lib.on_device(device):
+            st = _lib.lib().d3b_qk_norm_mrope(
+                q.data_ptr(), _lib.i64_array(q.stride()[:3]), heads, k.data_ptr(), _lib.i64_array(k.stride()[:3]), kv_heads,
+                wq.data_ptr(), wk.data_ptr(), positions.data_ptr(), _lib.i64_array(positions.stride()), inv_freq.data_ptr(),
+                bytes(axes), positions.shape[0], half, q_out.data_ptr(), k_out.data_ptr(), rows, T, D,
+                _lib.dtype_code(q.dtype), float(eps), _lib.stream_of(q))
+        _lib.check(st, "d3b_qk_norm_mrope")
+    return q_out, k_out
 
 
 def gdn_gates(a: torch.Tensor, b: torch.Tensor, neg_exp_a: torch.Tensor, dt_bias: torch.Tensor):

@@ -411,6 +411,104 @@ D3B_API int d3b_arena_free(void* arena, uint64_t offset);
 D3B_API int d3b_arena_stats(void* arena, uint64_t* stats);
 D3B_API void d3b_arena_destroy(void* arena);
 
+/*
+ * 4-bit key/value cache in pages: a state's K and V rows quantised into the pages of a pool,
+ * and the attention that reads them there. It has no counterpart in the reference, which keeps
+ * a snapshot's K/V in 16 bits (d3trt/model/core.py:28-40).
+ *
+ * pool [layers][pages][d3b_kv4_page_bytes()] bytes, 16-byte aligned. A page holds, for each kv
+ * head, page_tokens / 16 granules of 16 tokens (18 * head_dim + 32 bytes each):
+ *   K codes [16][D/2] (two e2m1 codes a byte, the even channel low), K scales [16][D/16] (e4m3),
+ *   K exponents [16] (one byte a row), V codes [16][D/2], V scales [D/16][16], V exponents [16];
+ *   value = code * scale * 2^(exponent - 127); exponent 255: the row held a NaN or an infinity
+ *   and every value of it reads as NaN.
+ * head_dim in {64, 128, 256}; page_tokens in {16, 32, 64, 128, 256} (else D3B_EUNSUPPORTED).
+ * Page p of a table holds tokens p * page_tokens ... of its sequence; slot s of a pool is token
+ * s % page_tokens of page s / page_tokens. Page numbers, slots and lengths live on the device:
+ * the kernels check each against the pool and the table, leave a bad one out and set the
+ * device error word (2101 slot, 2102 page, 2103 length, 2104 page list).
+ */
+typedef struct d3b_kv4_cache {
+  void* pool;
+  int64_t layers, pages;
+  int kv_heads, head_dim, page_tokens;
+} d3b_kv4_cache;
+
+/* Bytes of a page of one layer; 0 where the shape is not supported. */
+D3B_API int64_t d3b_kv4_page_bytes(int kv_heads, int head_dim, int page_tokens);
+
+/*
+ * Quantise n rows of K and V into the cache.
+ *   k, v [n, kv_heads, head_dim] dtype (f16 or bf16), strides {token, head} in elements
+ *     (multiples of 8; rows 16-byte aligned), head_dim contiguous
+ *   slots [n] int64 on the device; a negative slot leaves its row out. No two rows may name
+ *     the same slot: what that slot then holds is a mixture of the two.
+ * Per row: e = the least integer (>= -64) with max|x| <= 2688 * 2^e; per 16 channels
+ * scale = e4m3(max|x| * 2^-e / 6); code = e2m1(x * 2^-e / scale), both to nearest even.
+ */
+D3B_API int d3b_kv4_append(const d3b_kv4_cache* cache, int64_t layer, const void* k, const int64_t* k_strides,
+                           const void* v, const int64_t* v_strides, const int64_t* slots, int64_t n, int dtype,
+                           d3b_stream_t stream);
+
+/*
+ * The first `tokens` rows of a sequence: k, v [kv_heads, tokens, head_dim] contiguous, dtype f16
+ * or bf16 (exact; a magnitude above the type's largest becomes the largest).
+ *   table [n_pages] int32 on the device, n_pages * page_tokens >= tokens. Rows of a page number
+ *   outside the pool read as zeros.
+ */
+D3B_API int d3b_kv4_read(const d3b_kv4_cache* cache, int64_t layer, const int32_t* table, int64_t n_pages,
+                         int64_t tokens, void* k, void* v, int dtype, d3b_stream_t stream);
+
+/*
+ * Copy pages src[i] -> dst[i] in every layer, i < n, and rewrite page tables: each of the
+ * `entries` int32 values at `tables` that equals some src[i] becomes dst[i] (tables may be NULL
+ * with entries = 0). src and dst [n] int32 on the device. No destination may be a source or
+ * stand twice. With tables, src must be ascending.
+ */
+D3B_API int d3b_kv4_move_pages(const d3b_kv4_cache* cache, const int32_t* src, const int32_t* dst, int64_t n,
+                               int32_t* tables, int64_t entries, d3b_stream_t stream);
+
+/*
+ * Attention of the newest tokens of B sequences over their cached keys and values:
+ *   out[b,h,i] = softmax_j(scale * q[b,h,i] . key_j) . value_j over j < n(b, i), where n(b, i) =
+ *   lengths[b], or with causal lengths[b] - (L - 1 - i): token i is number lengths[b] - L + i of
+ *   its sequence and sees itself and what stands before it. Rows with no key are zero.
+ *   q, out [B, H, L, D] dtype f16 or bf16, strides {b, h, l} in elements (multiples of 8; rows
+ *     16-byte aligned); kv head of head h: h / (H / kv_heads)
+ *   table [B, width] int32, row stride table_stride; lengths [B] int32, both on the device.
+ *     Entries behind a sequence's last page are not read. A page number outside the pool leaves
+ *     its tokens out; a length outside [0, width * page_tokens] is clamped.
+ *   workspace: d3b_kv4_decode_workspace_size() bytes, 16-byte aligned (need not be zeroed;
+ *     launches that may overlap need one each). NULL where that is 0.
+ * Q, K and V enter the products exactly, in fp16 (queries under a power of two a row); softmax
+ * weights are rounded to fp16; sums are fp32.
+ */
+D3B_API size_t d3b_kv4_decode_workspace_size(const d3b_kv4_cache* cache, int B, int H, int L, int64_t width);
+D3B_API int d3b_kv4_decode(const d3b_kv4_cache* cache, int64_t layer, const void* q, const int64_t* q_strides,
+                           const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lengths, int B,
+                           int H, int L, int causal, int dtype, float scale, void* out, const int64_t* out_strides,
+                           void* workspace, size_t workspace_bytes, d3b_stream_t stream);
+
+/*
+ * Per-head RMSNorm of queries and keys, then a rotary embedding whose frequencies take their
+ * positions from several axes (time, height, width), one launch for both.
+ *   q [rows, T, q_heads, D], k [rows, T, k_heads, D] dtype f16 or bf16, strides {row, token,
+ *     head} in elements (multiples of 8; 16-byte aligned), D contiguous
+ *   y = x * rsqrt(mean(x^2) + eps) * (1 + weight), weights [D] of the same dtype
+ *   angle_i = positions[axis[i]] * inv_freq[i], i < half;
+ *   out_i = y_i cos - y_(i+half) sin, out_(i+half) = y_(i+half) cos + y_i sin, the rest y;
+ *   fp32 throughout (angles fp64), rounded once
+ *   positions [axes, rows, T] int64, strides {axis, row, token}; inv_freq [half] f32, both on
+ *     the device; axis [half] host bytes below `axes` (at most 8)
+ *   q_out, k_out [rows, T, heads, D] contiguous
+ * D in {64, 128, 256}; half a multiple of 8, 2 * half <= D. q_heads or k_heads may be 0.
+ */
+D3B_API int d3b_qk_norm_mrope(const void* q, const int64_t* q_strides, int q_heads, const void* k,
+                              const int64_t* k_strides, int k_heads, const void* q_weight, const void* k_weight,
+                              const int64_t* positions, const int64_t* pos_strides, const float* inv_freq,
+                              const uint8_t* axis, int axes, int half, void* q_out, void* k_out, int rows, int T,
+                              int head_dim, int dtype, float eps, d3b_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
