@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import threading
 from pathlib import Path
 from typing import Any
@@ -168,11 +169,23 @@ def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 
 
+_NO_SWITCH = contextlib.nullcontext()
+
+
 def on_device(device: torch.device) -> Any:
     """Context with ``device`` as the current one (nothing is switched where it is already)."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return _NO_SWITCH if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+# Raw handle of a device's current stream, without building a Stream object (0.1 us against 2.4).
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+@functools.lru_cache(maxsize=4096)
+def strides(values: tuple[int, ...], n: int) -> Any:
+    """The first ``n`` strides as a C array; kept by value, read only."""
+    return (ctypes.c_int64 * n)(*values[:n])
 
 
 def rows16(t: torch.Tensor) -> torch.Tensor:

@@ -578,8 +578,13 @@ size_t plan_bytes(const Plan& p, int D) {
 template <int D, int NT, bool BF>
 int launch(const DecodeArgs& a, const Plan& p, int B, cudaStream_t s) {
   constexpr int smem = Shape<D, NT>::kSmem;
-  if (cudaFuncSetAttribute(decode_kernel<D, NT, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return D3B_ECUDA;
+  static bool ready[64];  // by device; setting it twice is harmless
+  const int dev = d3b_host::current_device();
+  if (smem > 48 * 1024 && (dev < 0 || dev >= 64 || !ready[dev])) {
+    if (cudaFuncSetAttribute(decode_kernel<D, NT, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      return D3B_ECUDA;
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
   decode_kernel<D, NT, BF><<<(unsigned)(p.units * p.splits), kThreads, smem, s>>>(a);
   if (int rc = d3b_host::check_launch()) return rc;
   if (p.splits > 1) {

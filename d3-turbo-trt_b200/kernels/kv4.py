@@ -24,6 +24,7 @@ A row that held a NaN or an infinity reads back as NaN.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Sequence
 
 import torch
@@ -35,9 +36,10 @@ HEAD_DIMS = (64, 128, 256)
 PAGE_TOKENS = (16, 32, 64, 128, 256)
 SITE_BAD_SLOT, SITE_BAD_PAGE, SITE_BAD_LENGTH, SITE_BAD_MOVE = 2101, 2102, 2103, 2104
 
-_TYPES = (torch.float16, torch.bfloat16)
+_TYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
+@functools.lru_cache(maxsize=256)
 def page_bytes(kv_heads: int, head_dim: int, page_tokens: int) -> int:
     """Bytes of one page of one layer."""
     _check_shape(kv_heads, head_dim, page_tokens)
@@ -114,22 +116,24 @@ class Kv4Cache:
         ``slots`` [n] int64 on the device; a negative slot leaves its row out. Slots must differ: one
         that is named twice holds a mixture of the rows."""
         self._check_layer(layer)
-        shape = (slots.numel(), self.kv_heads, self.head_dim)
-        if slots.dim() != 1 or tuple(k.shape) != shape or tuple(v.shape) != shape:
+        n, device, dtype = slots.numel(), self.device, k.dtype
+        shape = (n, self.kv_heads, self.head_dim)
+        if slots.dim() != 1 or k.shape != shape or v.shape != shape:
             raise RuntimeError(f"k and v must be [n, {self.kv_heads}, {self.head_dim}] and slots [n], got "
                                f"{tuple(k.shape)}, {tuple(v.shape)}, {tuple(slots.shape)}")
-        if k.dtype not in _TYPES or v.dtype != k.dtype or k.device != self.device or v.device != self.device:
-            raise RuntimeError(f"k and v must be fp16 or bf16 on {self.device}, got {k.dtype} on {k.device} and "
+        if dtype not in _TYPES or v.dtype != dtype or k.device != device or v.device != device:
+            raise RuntimeError(f"k and v must be fp16 or bf16 on {device}, got {dtype} on {k.device} and "
                                f"{v.dtype} on {v.device}")
-        _index(slots, torch.int64, self.device, "slots")
-        if shape[0] == 0:
+        _index(slots, torch.int64, device, "slots")
+        if n == 0:
             return
         k, v, slots = _lib.rows16(k), _lib.rows16(v), slots.contiguous()
-        with _lib.on_device(self.device):
+        with _lib.on_device(device):
             status = _lib.lib().d3b_kv4_append(
-                self._ref, layer, k.data_ptr(), _lib.i64_array(k.stride()[:2]), v.data_ptr(),
-                _lib.i64_array(v.stride()[:2]), slots.data_ptr(), shape[0], _lib.dtype_code(k.dtype), _lib.stream_of(k))
-        _lib.check(status, "d3b_kv4_append")
+                self._ref, layer, k.data_ptr(), _lib.strides(k.stride(), 2), v.data_ptr(), _lib.strides(v.stride(), 2),
+                slots.data_ptr(), n, _TYPES[dtype], _lib.raw_stream(device.index))
+        if status:
+            _lib.check(status, "d3b_kv4_append")
 
     def read(self, layer: int, table: torch.Tensor, tokens: int, *, dtype: torch.dtype = torch.bfloat16,
              ) -> tuple[torch.Tensor, torch.Tensor]:
@@ -138,14 +142,14 @@ class Kv4Cache:
         if dtype not in _TYPES:
             raise RuntimeError(f"read gives fp16 or bf16, not {dtype}")
         self._check_table(table, tokens)
-        both = torch.empty(2, self.kv_heads, tokens, self.head_dim, dtype=dtype, device=self.device)
-        k, v = both.unbind(0)
+        k, v = torch.empty((2, self.kv_heads, tokens, self.head_dim), dtype=dtype, device=self.device).unbind(0)
         if tokens:
             table = table.contiguous()
             with _lib.on_device(self.device):
                 status = _lib.lib().d3b_kv4_read(self._ref, layer, table.data_ptr(), table.numel(), tokens, k.data_ptr(),
-                                                 v.data_ptr(), _lib.dtype_code(dtype), _lib.stream_of(both))
-            _lib.check(status, "d3b_kv4_read")
+                                                 v.data_ptr(), _TYPES[dtype], _lib.raw_stream(self.device.index))
+            if status:
+                _lib.check(status, "d3b_kv4_read")
         return k, v
 
     def _check_table(self, table: torch.Tensor, tokens: int) -> None:
@@ -191,9 +195,11 @@ class Kv4Cache:
             return
         src, dst = src.contiguous(), dst.contiguous()
         with _lib.on_device(self.device):
-            status = _lib.lib().d3b_kv4_move_pages(self._ref, src.data_ptr(), dst.data_ptr(), n, _lib.ptr(tables),
-                                                   0 if tables is None else tables.numel(), _lib.stream_of(src))
-        _lib.check(status, "d3b_kv4_move_pages")
+            status = _lib.lib().d3b_kv4_move_pages(
+                self._ref, src.data_ptr(), dst.data_ptr(), n, None if tables is None else tables.data_ptr(),
+                0 if tables is None else tables.numel(), _lib.raw_stream(self.device.index))
+        if status:
+            _lib.check(status, "d3b_kv4_move_pages")
 
 
 def _check_query(q: torch.Tensor, cache: Kv4Cache, layer: int) -> None:
@@ -239,7 +245,7 @@ def decode_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torch.
                            f"{tuple(lengths.shape)}")
     q = _lib.rows16(q)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        out = q.new_empty(q.shape)
     else:
         _check_out(out, q)
     if rows and width:
@@ -251,12 +257,13 @@ def decode_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torch.
             need = lib.d3b_kv4_decode_workspace_size(cache._ref, rows, heads, width, table.shape[1])
             # from the caching allocator at every call: calls on other streams and captured graphs
             # get their own, and it is ordered with the stream like any tensor
-            work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+            work = cache.pool.new_empty(need) if need else None
             status = lib.d3b_kv4_decode(
-                cache._ref, layer, q.data_ptr(), _lib.i64_array(q.stride()[:3]), table.data_ptr(), table.stride(0),
-                table.shape[1], lengths.data_ptr(), rows, heads, width, int(causal), _lib.dtype_code(q.dtype), float(scale),
-                out.data_ptr(), _lib.i64_array(out.stride()[:3]), _lib.ptr(work), need, _lib.stream_of(q))
-        _lib.check(status, "d3b_kv4_decode")
+                cache._ref, layer, q.data_ptr(), _lib.strides(q.stride(), 3), table.data_ptr(), table.stride(0),
+                table.shape[1], lengths.data_ptr(), rows, heads, width, causal, _TYPES[q.dtype], scale, out.data_ptr(),
+                _lib.strides(out.stride(), 3), work.data_ptr() if need else None, need, _lib.raw_stream(device.index))
+        if status:
+            _lib.check(status, "d3b_kv4_decode")
     return out.squeeze(2) if single else out
 
 
@@ -286,7 +293,7 @@ def question_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torc
         if len(lengths) != rows or any(not 0 <= n <= width for n in lengths):
             raise RuntimeError(f"lengths must be {rows} values in [0, {width}]")
     if out is None:
-        out = torch.empty((rows, heads, width, dim), dtype=q.dtype, device=q.device)
+        out = q.new_empty((rows, heads, width, dim))
     else:
         _check_out(out, q)
     if rows == 0 or width == 0:

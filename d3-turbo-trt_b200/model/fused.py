@@ -263,7 +263,7 @@ def rotary_axes(sections: Sequence[int], *, interleaved: bool = True) -> tuple[i
     return tuple(axes)
 
 
-_ROPE_TYPES = (torch.bfloat16, torch.float16)
+_ROPE_TYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
 def qk_norm_mrope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
@@ -280,12 +280,46 @@ def qk_norm_mrope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_we
     Returns both as [rows, T, heads, D] token-major tensors. Computed in fp32 (angles in fp64) and
     rounded once, where ``qk_norm_rope`` rounds after each of the reference's bf16 operations.
     """
+    # the checks go by shapes, strides and types alone: once for each set of them
+    key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device, q_weight.shape, q_weight.dtype,
+           k_weight.shape, k_weight.dtype, positions.shape, positions.dtype, positions.device, inv_freq.shape,
+           inv_freq.stride(), inv_freq.dtype, inv_freq.device, tuple(axes))
+    plan = _ROPE_PLANS.get(key)
+    if plan is None:
+        plan = _plan_mrope(q, k, q_weight, k_weight, positions, inv_freq, key[-1])
+        if len(_ROPE_PLANS) >= 1024:
+            _ROPE_PLANS.clear()
+        _ROPE_PLANS[key] = plan
+    q_shape, k_shape, axis, fn = plan
+    device, dtype = q.device, q.dtype
+    if q_weight.dtype != dtype or q_weight.device != device:
+        q_weight = q_weight.to(device=device, dtype=dtype)
+    if k_weight.dtype != dtype or k_weight.device != device:
+        k_weight = k_weight.to(device=device, dtype=dtype)
+    q, k, q_weight, k_weight = (_lib.rows16(x) for x in (q, k, q_weight, k_weight))
+    q_out, k_out = q.new_empty(q_shape), q.new_empty(k_shape)
+    if q_out.numel() + k_out.numel():
+        with _lib.on_device(device):
+            st = fn(q.data_ptr(), _lib.strides(q.stride(), 3), q_shape[2], k.data_ptr(), _lib.strides(k.stride(), 3),
+                    k_shape[2], q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(),
+                    _lib.strides(positions.stride(), 3), inv_freq.data_ptr(), axis, positions.shape[0], len(axis),
+                    q_out.data_ptr(), k_out.data_ptr(), q_shape[0], q_shape[1], q_shape[3], _ROPE_TYPES[dtype], eps,
+                    _lib.raw_stream(device.index))
+        if st:
+            _lib.check(st, "d3b_qk_norm_mrope")
+    return q_out, k_out
+
+
+_ROPE_PLANS: dict = {}
+
+
+def _plan_mrope(q, k, q_weight, k_weight, positions, inv_freq, axes):
+    """The checks of ``qk_norm_mrope`` and what its launch needs of the shapes."""
     for x, what in ((q, "q"), (k, "k")):
         if not x.is_cuda or x.dtype not in _ROPE_TYPES:
             raise RuntimeError(f"qk_norm_mrope needs bf16 or fp16 CUDA tensors, got {what} {x.dtype} on {x.device}")
-        if x.dim() != 4 or (x.stride(-1) != 1 and x.shape[-1] != 1):
-            raise RuntimeError(f"qk_norm_mrope: {what} must be [rows, T, heads, D] with a contiguous last dim, got "
-                               f"{tuple(x.shape)} strides {x.stride()}")
+        if x.dim() != 4:
+            raise RuntimeError(f"qk_norm_mrope: {what} must be [rows, T, heads, D], got {tuple(x.shape)}")
     rows, T, heads, D = q.shape
     kv_heads = k.shape[2]
     if k.dtype != q.dtype or k.device != q.device or k.shape[0] != rows or k.shape[1] != T or k.shape[3] != D:
@@ -295,33 +329,18 @@ def qk_norm_mrope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_we
     half = len(axes)
     if half % 8 or 2 * half > D or inv_freq.dim() != 1 or inv_freq.numel() != half:
         raise RuntimeError(f"qk_norm_mrope: {half} axes and {tuple(inv_freq.shape)} frequencies for head_dim {D}")
-    if inv_freq.dtype != torch.float32 or positions.dtype != torch.int64:
-        raise RuntimeError(f"qk_norm_mrope: inv_freq must be float32 and positions int64, got {inv_freq.dtype}, "
-                           f"{positions.dtype}")
+    if inv_freq.dtype != torch.float32 or (half > 1 and inv_freq.stride(0) != 1) or positions.dtype != torch.int64:
+        raise RuntimeError(f"qk_norm_mrope: inv_freq must be contiguous float32 and positions int64, got "
+                           f"{inv_freq.dtype}, {positions.dtype}")
     if positions.dim() != 3 or positions.shape[1] != rows or positions.shape[2] != T or not 1 <= positions.shape[0] <= 8:
         raise RuntimeError(f"qk_norm_mrope: positions must be [axes, {rows}, {T}], got {tuple(positions.shape)}")
     if half and not 0 <= min(axes) <= max(axes) < positions.shape[0]:
         raise RuntimeError(f"qk_norm_mrope: axes must lie in [0, {positions.shape[0]})")
-    device = q.device
-    if positions.device != device or inv_freq.device != device:
-        raise RuntimeError(f"qk_norm_mrope: positions and inv_freq must be on {device}")
-    if q_weight.numel() != D or k_weight.numel() != D:
-        raise RuntimeError(f"qk_norm_mrope: weights must have {D} values, got {q_weight.numel()} and {k_weight.numel()}")
-    q, k = _lib.rows16(q), _lib.rows16(k)
-    wq = _lib.rows16(q_weight.to(device=device, dtype=q.dtype))
-    wk = _lib.rows16(k_weight.to(device=device, dtype=q.dtype))
-    inv_freq = inv_freq.contiguous()
-    q_out = torch.empty(rows, T, heads, D, dtype=q.dtype, device=device)
-    k_out = torch.empty(rows, T, kv_heads, D, dtype=q.dtype, device=device)
-    if rows and T and heads + kv_heads:
-        with _lib.on_device(device):
-            st = _lib.lib().d3b_qk_norm_mrope(
-                q.data_ptr(), _lib.i64_array(q.stride()[:3]), heads, k.data_ptr(), _lib.i64_array(k.stride()[:3]), kv_heads,
-                wq.data_ptr(), wk.data_ptr(), positions.data_ptr(), _lib.i64_array(positions.stride()), inv_freq.data_ptr(),
-                bytes(axes), positions.shape[0], half, q_out.data_ptr(), k_out.data_ptr(), rows, T, D,
-                _lib.dtype_code(q.dtype), float(eps), _lib.stream_of(q))
-        _lib.check(st, "d3b_qk_norm_mrope")
-    return q_out, k_out
+    if positions.device != q.device or inv_freq.device != q.device:
+        raise RuntimeError(f"qk_norm_mrope: positions and inv_freq must be on {q.device}")
+    if q_weight.numel() != D or k_weight.numel() != D or q_weight.dim() != 1 or k_weight.dim() != 1:
+        raise RuntimeError(f"qk_norm_mrope: weights must be [{D}], got {tuple(q_weight.shape)} and {tuple(k_weight.shape)}")
+    return (rows, T, heads, D), (rows, T, kv_heads, D), bytes(axes), _lib.lib().d3b_qk_norm_mrope
 
 
 def gdn_gates(a: torch.Tensor, b: torch.Tensor, neg_exp_a: torch.Tensor, dt_bias: torch.Tensor):
