@@ -42,22 +42,31 @@ __device__ __forceinline__ uint32_t to_e2m1x8(const float (&x)[8]) {
   return r;
 }
 
-// a row is (token, head, K or V), K and V of a head next to each other
+// Rounded to 17 significant bits (half up). A quotient x / s is formed as x * (1 / s), which is off by
+// 2^-22 of it; x has at most 11 significant bits and s 4, so a quotient that is not a border of two
+// codes (at most 3 bits; for the scales' borders, 5 bits times 6) is 2^-12 of itself away from it, and
+// one that is a border becomes exactly that border here. The conversions below then round as the
+// quotient itself would.
+__device__ __forceinline__ float round17(float x) {
+  return __uint_as_float((__float_as_uint(x) + 0x40u) & 0xFFFFFF80u);
+}
+
+// grid: (groups of tokens, kv head, K or V); a row of D values is D/8 lanes
 template <int D, bool BF>
 __global__ void __launch_bounds__(kThreads) append_kernel(uint8_t* __restrict__ pool, int64_t page_bytes, int64_t pages,
-                                                          int heads, int page_shift, const uint16_t* __restrict__ k,
-                                                          int64_t sk_t, int64_t sk_h, const uint16_t* __restrict__ v,
-                                                          int64_t sv_t, int64_t sv_h,
-                                                          const int64_t* __restrict__ slots, int64_t rows, int* err) {
+                                                          int page_shift, const uint16_t* __restrict__ k, int64_t sk_t,
+                                                          int64_t sk_h, const uint16_t* __restrict__ v, int64_t sv_t,
+                                                          int64_t sv_h, const int64_t* __restrict__ slots, int64_t n,
+                                                          int* err) {
   constexpr int kLanes = D / 8;
   const int sub = threadIdx.x % kLanes;
-  int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / kLanes;
-  bool live = row < rows;  // every lane stays for the shuffles
-  row = live ? row : 0;
-  const bool is_v = row & 1;
-  const int64_t th = row >> 1;
-  const int64_t tok = th / heads;
-  const int head = (int)(th % heads);
+  const int head = blockIdx.y;
+  const bool is_v = blockIdx.z;
+  int64_t tok = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  bool live = tok < n;  // every lane stays for the shuffles
+  tok = live ? tok : 0;
+  const uint16_t* src = is_v ? v + tok * sv_t + head * sv_h : k + tok * sk_t + head * sk_h;
+  const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src) + sub);
   const int64_t slot = __ldg(slots + tok);
   const int64_t page = slot >> page_shift;
   live = live && slot >= 0;
@@ -65,100 +74,113 @@ __global__ void __launch_bounds__(kThreads) append_kernel(uint8_t* __restrict__ 
     if (sub == 0) d3b::record_device_error(err, kSiteBadSlot);
     live = false;
   }
-  const uint16_t* src = is_v ? v + tok * sv_t + head * sv_h : k + tok * sk_t + head * sk_h;
-  const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src) + sub);
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = widen<BF>(w[i] & 0xFFFFu);
-    x[2 * i + 1] = widen<BF>(w[i] >> 16);
-  }
   // largest magnitude as bits: ordered like the values, and a NaN or infinity is the largest
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-  uint32_t group = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  uint32_t top2 = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu),
+                           __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
+  uint32_t group = max(top2 & 0xFFFFu, top2 >> 16);
+  group = max(group, __shfl_xor_sync(0xffffffffu, group, 1));
   uint32_t most = group;
 #pragma unroll
   for (int o = 2; o < kLanes; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-  const bool bad = most >= 0x7F800000u;
-  // least e with most <= 2688 * 2^e: 2688 = 1.3125 * 2^11
-  int e = (int)(most >> 23) - 127 - 11 + ((most & 0x7FFFFFu) > 0x280000u ? 1 : 0);
-  e = max(e, kExpMin);  // also rows of zeros and fp32 subnormals (bf16 inputs)
+  const bool bad = most >= (BF ? 0x7F80u : 0x7C00u);
+  // least e with most <= 2688 * 2^e: 2688 = 1.3125 * 2^11; at least kExpMin (rows of zeros and subnormals too)
+  const uint32_t bits = __float_as_uint(widen<BF>(most));
+  const int e = max((int)(bits >> 23) - 127 - 11 + ((bits & 0x7FFFFFu) > 0x280000u ? 1 : 0), kExpMin);
   const float down = __uint_as_float((uint32_t)(127 - e) << 23);  // e in [-64, 117]
-  const uint32_t scale_byte = bad ? 0u : to_e4m3(__fdiv_rn(__uint_as_float(group) * down, 6.0f));
-  const uint32_t sh = decode_scales(scale_byte);
-  const float scale = __half2float(__ushort_as_half((unsigned short)(sh & 0xFFFFu)));
-  if (!live) return;
-  // x / scale to nearest, so that a quotient on the border of two codes is exactly that border
+  const uint32_t scale_byte = bad ? 0u : to_e4m3(round17(widen<BF>(group) * down * (1.0f / 6.0f)));
+  const float scale = __half2float(__ushort_as_half((unsigned short)(decode_scales(scale_byte) & 0xFFFFu)));
+  const float by = scale > 0.f ? __frcp_rn(scale) * down : 0.f;
+  float x[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = scale > 0.f ? __fdiv_rn(x[i] * down, scale) : 0.f;
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = round17(widen<BF>(w[i] & 0xFFFFu) * by);
+    x[2 * i + 1] = round17(widen<BF>(w[i] >> 16) * by);
+  }
+  if (bad) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  }
   const uint32_t codes = to_e2m1x8(x);
-  const int in_page = (int)(slot & ((1 << page_shift) - 1));
+  if (!live) return;
+  const int in_page = (int)slot & ((1 << page_shift) - 1);
   const int t = in_page & 15;
-  uint8_t* g = pool + page * page_bytes +
-               ((int64_t)head * (1 << (page_shift - 4)) + (in_page >> 4)) * granule_bytes(D) + (is_v ? off_v(D) : 0);
+  uint8_t* g = pool + page * page_bytes + ((head << (page_shift - 4)) + (in_page >> 4)) * (int64_t)granule_bytes(D) +
+               (is_v ? off_v(D) : 0);
   reinterpret_cast<uint32_t*>(g + t * (D / 2))[sub] = codes;
   if (!(sub & 1)) g[off_k_scale(D) + (is_v ? (sub >> 1) * 16 + t : t * (D / 16) + (sub >> 1))] = (uint8_t)scale_byte;
   if (sub == 0) g[off_k_exp(D) + t] = (uint8_t)(bad ? 255 : e + 127);
 }
 
+// eight values of one word of codes; `power` finite or NaN, `most` the magnitude that may not be passed
 template <bool BF>
-__device__ __forceinline__ uint32_t narrow2(float a, float b) {  // both finite or NaN; saturating
-  if constexpr (BF) {
-    const float m = 3.3895313892515355e38f;  // largest bf16
-    a = a > m ? m : (a < -m ? -m : a);
-    b = b > m ? m : (b < -m ? -m : b);
-    const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&r);
-  } else {
-    a = a > 65504.f ? 65504.f : (a < -65504.f ? -65504.f : a);
-    b = b > 65504.f ? 65504.f : (b < -65504.f ? -65504.f : b);
-    const __half2 r = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ uint4 widen_codes(uint32_t codes, uint32_t scale2, float power, bool clamp) {
+  uint32_t h[4], r[4];
+  decode8(codes, h);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t p = hmul2(h[i], scale2);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
+    float a = f.x * power, b = f.y * power;
+    if (clamp) {
+      constexpr float m = BF ? 3.3895313892515355e38f : 65504.f;  // the type's largest
+      a = a > m ? m : (a < -m ? -m : a);                          // a NaN stays
+      b = b > m ? m : (b < -m ? -m : b);
+    }
+    if constexpr (BF) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+      r[i] = *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+      const __half2 v = __floats2half2_rn(a, b);
+      r[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
   }
+  return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// one lane: 8 channels of one token of K or V
+// one lane: 8 channels of four tokens of K or V (a quarter of a granule)
 template <int D, bool BF>
 __global__ void __launch_bounds__(kThreads) read_kernel(const uint8_t* __restrict__ pool, int64_t page_bytes,
-                                                        int64_t pages, int heads, int page_shift,
+                                                        int64_t pages, int page_shift,
                                                         const int32_t* __restrict__ table, int64_t tokens,
                                                         uint16_t* __restrict__ k, uint16_t* __restrict__ v, int* err) {
   constexpr int kLanes = D / 8;
   const int sub = threadIdx.x % kLanes;
   const int head = blockIdx.y;
   const bool is_v = blockIdx.z;
-  const int64_t tok = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  const int64_t tok = 4 * ((int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes);
   if (tok >= tokens) return;
   const int64_t page = __ldg(table + (tok >> page_shift));
-  uint4 o = make_uint4(0, 0, 0, 0);
+  uint4 o[4] = {};
   if (page < 0 || page >= pages) {
     if (sub == 0) d3b::record_device_error(err, kSiteBadPage);
   } else {
-    const int in_page = (int)(tok & ((1 << page_shift) - 1));
-    const int t = in_page & 15;
-    const uint8_t* g = pool + page * page_bytes +
-                       ((int64_t)head * (1 << (page_shift - 4)) + (in_page >> 4)) * granule_bytes(D) +
+    const int in_page = (int)tok & ((1 << page_shift) - 1);
+    const int t = in_page & 15, group = sub >> 1;
+    const uint8_t* g = pool + page * page_bytes + ((head << (page_shift - 4)) + (in_page >> 4)) * (int64_t)granule_bytes(D) +
                        (is_v ? off_v(D) : 0);
-    const uint32_t codes = __ldg(reinterpret_cast<const uint32_t*>(g + t * (D / 2)) + sub);
-    const int group = sub >> 1;
-    const uint32_t sb = __ldg(g + off_k_scale(D) + (is_v ? group * 16 + t : t * (D / 16) + group));
-    const float power = row_power(__ldg(g + off_k_exp(D) + t));
-    const uint32_t s2 = decode_scales(sb | (sb << 8));
-    uint32_t h[4], r[4];
-    decode8(codes, h);
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(g + t * (D / 2)) + sub;
+    uint32_t c[4], scales = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t p = hmul2(h[i], s2);
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
-      r[i] = narrow2<BF>(f.x * power, f.y * power);
+    for (int i = 0; i < 4; ++i) c[i] = __ldg(codes + i * (D / 8));
+    if (is_v) {
+      scales = __ldg(reinterpret_cast<const uint32_t*>(g + off_k_scale(D) + group * 16 + t));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) scales |= (uint32_t)__ldg(g + off_k_scale(D) + (t + i) * (D / 16) + group) << (8 * i);
     }
-    o = make_uint4(r[0], r[1], r[2], r[3]);
+    const uint32_t exps = __ldg(reinterpret_cast<const uint32_t*>(g + off_k_exp(D) + t));
+    // only a row whose 2688 * 2^e passes the type's largest value can
+    const bool clamp = __vmaxu4(exps, BF ? 0xF3F3F3F3u : 0x83838383u) != (BF ? 0xF3F3F3F3u : 0x83838383u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      o[i] = widen_codes<BF>(c[i], decode_scales(((scales >> (8 * i)) & 0xFFu) * 0x101u),
+                             row_power((exps >> (8 * i)) & 0xFFu), clamp);
   }
-  uint16_t* out = is_v ? v : k;
-  reinterpret_cast<uint4*>(out + ((int64_t)head * tokens + tok) * D)[sub] = o;
+  uint4* out = reinterpret_cast<uint4*>((is_v ? v : k) + (head * tokens + tok) * D) + sub;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (tok + i < tokens) out[i * (D / 8)] = o[i];
 }
 
 constexpr int kMoveVec = 4;  // 16-byte loads in flight per thread
@@ -218,36 +240,36 @@ __global__ void __launch_bounds__(kThreads) move_kernel(uint8_t* __restrict__ po
 template <int D>
 int launch_append(const d3b_kv4_cache* c, int64_t layer, const void* k, const int64_t* ks, const void* v,
                   const int64_t* vs, const int64_t* slots, int64_t n, bool bf, int* err, cudaStream_t s) {
-  const int64_t rows = 2 * n * c->kv_heads, threads = rows * (D / 8);
-  const int64_t ctas = (threads + kThreads - 1) / kThreads;
+  const int64_t per = kThreads / (D / 8), ctas = (n + per - 1) / per;
   if (ctas > 0x7FFFFFFF) return D3B_EINVAL;
+  const dim3 grid((unsigned)ctas, (unsigned)c->kv_heads, 2);
   auto* kp = static_cast<const uint16_t*>(k);
   auto* vp = static_cast<const uint16_t*>(v);
   const int shift = log2_of(c->page_tokens);
   if (bf)
-    append_kernel<D, true><<<(unsigned)ctas, kThreads, 0, s>>>(layer_base(c, layer), page_bytes(c), c->pages, c->kv_heads,
-                                                               shift, kp, ks[0], ks[1], vp, vs[0], vs[1], slots, rows, err);
+    append_kernel<D, true><<<grid, kThreads, 0, s>>>(layer_base(c, layer), page_bytes(c), c->pages, shift, kp, ks[0], ks[1], vp,
+                                                 vs[0], vs[1], slots, n, err);
   else
-    append_kernel<D, false><<<(unsigned)ctas, kThreads, 0, s>>>(layer_base(c, layer), page_bytes(c), c->pages, c->kv_heads,
-                                                                shift, kp, ks[0], ks[1], vp, vs[0], vs[1], slots, rows, err);
+    append_kernel<D, false><<<grid, kThreads, 0, s>>>(layer_base(c, layer), page_bytes(c), c->pages, shift, kp, ks[0], ks[1], vp,
+                                                 vs[0], vs[1], slots, n, err);
   return d3b_host::check_launch();
 }
 
 template <int D>
 int launch_read(const d3b_kv4_cache* c, int64_t layer, const int32_t* table, int64_t tokens, void* k, void* v, bool bf,
                 int* err, cudaStream_t s) {
-  const int64_t per = kThreads / (D / 8), ctas = (tokens + per - 1) / per;
+  const int64_t per = 4 * (kThreads / (D / 8)), ctas = (tokens + per - 1) / per;
   if (ctas > 0x7FFFFFFF) return D3B_EINVAL;
   const dim3 grid((unsigned)ctas, (unsigned)c->kv_heads, 2);
   auto* kp = static_cast<uint16_t*>(k);
   auto* vp = static_cast<uint16_t*>(v);
   const int shift = log2_of(c->page_tokens);
   if (bf)
-    read_kernel<D, true><<<grid, kThreads, 0, s>>>(layer_base(c, layer), page_bytes(c), c->pages, c->kv_heads, shift, table,
-                                                   tokens, kp, vp, err);
+    read_kernel<D, true><<<grid, kThreads, 0, s>>>(layer_base(c, layer), page_bytes(c), c->pages, shift, table, tokens, kp, vp,
+                                                err);
   else
-    read_kernel<D, false><<<grid, kThreads, 0, s>>>(layer_base(c, layer), page_bytes(c), c->pages, c->kv_heads, shift, table,
-                                                    tokens, kp, vp, err);
+    read_kernel<D, false><<<grid, kThreads, 0, s>>>(layer_base(c, layer), page_bytes(c), c->pages, shift, table, tokens, kp, vp,
+                                                err);
   return d3b_host::check_launch();
 }
 

@@ -7,13 +7,17 @@
 //
 // All of it in fp32 and rounded once. The angle is formed and brought into one turn in fp64:
 // position * inv_freq in fp32 is off by half a unit of the product's last place, 0.004 rad at
-// position 100 000, and a turn is what sincospi takes. That is `half` products a token, shared by
-// all its heads: one CTA holds one token's heads, its first threads make the table in shared
-// memory while the others' rows are on their way.
+// position 100 000, and a turn is what sincospi takes.
 //
-// Bound: each value is read and written once, so bytes. A head of D values is D/8 lanes x 8
-// values (one 16-byte load and store each); the sum of squares is a shuffle reduction and a
-// rotary partner is half/8 lanes away.
+// A warp takes one token and a run of its heads. Cosines and sines of the channels that a lane
+// turns, and its channels' weights, stay in registers over the run; the next heads' rows are
+// loaded before the present ones are worked on. A head of D values is D/8 lanes x 8 values (one
+// 16-byte load and store each): the sum of squares is a shuffle reduction, a rotary partner is
+// half/8 lanes away. How many heads a warp takes is the host's choice: few tokens are spread over
+// as many warps as there are heads, many tokens share the table's cost.
+//
+// Bound: bytes, each value read and written once, with instructions close behind (about 90 for
+// the 256 values a warp holds, where memory leaves room for 170).
 #include "common.cuh"
 
 namespace {
@@ -42,44 +46,74 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
+constexpr int kWarps = 4;
+
 template <int D, bool BF>
-__global__ void __launch_bounds__(1024) qk_norm_mrope_kernel(
+__global__ void __launch_bounds__(32 * kWarps) qk_norm_mrope_kernel(
     const uint16_t* __restrict__ q, int64_t sq_r, int64_t sq_t, int64_t sq_h, int q_heads,
     const uint16_t* __restrict__ k, int64_t sk_r, int64_t sk_t, int64_t sk_h, int k_heads,
     const uint16_t* __restrict__ wq, const uint16_t* __restrict__ wk, const int64_t* __restrict__ pos, int64_t sp_a,
     int64_t sp_r, int64_t sp_t, const float* __restrict__ inv_freq, const __grid_constant__ Axes axis, int half,
-    uint16_t* __restrict__ q_out, uint16_t* __restrict__ k_out, int T, float eps) {
-  constexpr int kLanes = D / 8;
-  __shared__ __align__(16) float cos_t[kMaxHalf], sin_t[kMaxHalf];
-  const int64_t rt = blockIdx.x;
-  const int64_t r = rt / T;
-  const int t = (int)(rt % T);
-  const int sub = threadIdx.x % kLanes;
-  const int heads = q_heads + k_heads;
-  const int per_pass = blockDim.x / kLanes;
+    uint16_t* __restrict__ q_out, uint16_t* __restrict__ k_out, int T, int64_t tokens, int runs, int run, float eps) {
+  constexpr int kLanes = D / 8, kHeads = 32 / kLanes;  // heads a warp holds at once
+  __shared__ __align__(16) float2 table[kWarps][D / 2];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, sub = lane % kLanes;
+  const int64_t item = (int64_t)blockIdx.x * kWarps + warp;
+  const int64_t rt = item / runs;
+  if (rt >= tokens) return;
+  const int first = (int)(item - rt * runs) * run;
+  const int64_t r = rt / T, t = rt - r * T;
+  // passes: kHeads heads of q each, then of k
+  const int q_passes = (q_heads + kHeads - 1) / kHeads, passes = q_passes + (k_heads + kHeads - 1) / kHeads;
+  const int last = min(first + run, passes);
+  const uint16_t* q_row = q + r * sq_r + t * sq_t;
+  const uint16_t* k_row = k + r * sk_r + t * sk_t;
+  auto fetch = [&](int p) {
+    const bool is_k = p >= q_passes;
+    const int h = (is_k ? p - q_passes : p) * kHeads + lane / kLanes;
+    if (p >= last || h >= (is_k ? k_heads : q_heads)) return make_uint4(0, 0, 0, 0);
+    return __ldg(reinterpret_cast<const uint4*>(is_k ? k_row + h * sk_h : q_row + h * sq_h) + sub);
+  };
+  uint4 next = fetch(first), after = fetch(first + 1);
+  for (int i = lane; i < half; i += 32) {
+    const double turns =
+        (double)__ldg(pos + axis.of[i] * sp_a + r * sp_r + t * sp_t) * (double)__ldg(inv_freq + i) *
+        0.15915494309189533577;  // 1 / (2 pi)
+    float s, c;
+    sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+    table[warp][i] = make_float2(c, s);
+  }
+  __syncwarp();
   const int shift = half / 8;  // lanes to the rotary partner
-  for (int first = 0; first < heads; first += per_pass) {
-    const int h = first + threadIdx.x / kLanes;
-    const bool live = h < heads;
-    const bool is_k = live && h >= q_heads;
-    uint4 raw = make_uint4(0, 0, 0, 0), wraw = raw;
-    if (live) {
-      const uint16_t* src = is_k ? k + r * sk_r + t * sk_t + (h - q_heads) * sk_h : q + r * sq_r + t * sq_t + h * sq_h;
-      raw = __ldg(reinterpret_cast<const uint4*>(src) + sub);
-      wraw = __ldg(reinterpret_cast<const uint4*>(is_k ? wk : wq) + sub);
-    }
-    if (first == 0) {
-      for (int i = threadIdx.x; i < half; i += blockDim.x) {
-        const double turns = (double)pos[axis.of[i] * sp_a + r * sp_r + t * sp_t] * (double)inv_freq[i] *
-                             0.15915494309189533577;  // 1 / (2 pi)
-        const float x = (float)(2.0 * (turns - rint(turns)));
-        sincospif(x, &sin_t[i], &cos_t[i]);
+  const bool low = sub < shift, turned = sub < 2 * shift;
+  const int partner = lane - sub + (turned ? (low ? sub + shift : sub - shift) : sub);
+  float cs[8], sn[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 x = turned ? table[warp][8 * (low ? sub : sub - shift) + i] : make_float2(1.f, 0.f);
+    cs[i] = x.x;
+    sn[i] = low ? -x.y : x.y;
+  }
+  float w1[8];
+  int weights = -1;  // whose they are
+  for (int p = first; p < last; ++p) {
+    const bool is_k = p >= q_passes;
+    const uint4 raw = next;
+    next = after;
+    after = fetch(p + 2);
+    if (weights != (int)is_k) {
+      weights = is_k;
+      const uint4 wraw = __ldg(reinterpret_cast<const uint4*>(is_k ? wk : wq) + sub);
+      const uint32_t wr[4] = {wraw.x, wraw.y, wraw.z, wraw.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = widen2<BF>(wr[i]);
+        w1[2 * i] = 1.f + f.x;
+        w1[2 * i + 1] = 1.f + f.y;
       }
-      __syncthreads();
     }
-    const uint32_t xr[4] = {raw.x, raw.y, raw.z, raw.w}, wr[4] = {wraw.x, wraw.y, wraw.z, wraw.w};
-    float y[8];
-    float ss = 0.f;
+    const uint32_t xr[4] = {raw.x, raw.y, raw.z, raw.w};
+    float y[8], ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 f = widen2<BF>(xr[i]);
@@ -92,31 +126,19 @@ __global__ void __launch_bounds__(1024) qk_norm_mrope_kernel(
     for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     const float rs = rsqrtf(ss * (1.0f / D) + eps);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = widen2<BF>(wr[i]);
-      y[2 * i] *= rs * (1.f + f.x);
-      y[2 * i + 1] *= rs * (1.f + f.y);
-    }
-    const bool low = sub < shift, turned = sub < 2 * shift;
-    const int partner = turned ? (low ? sub + shift : sub - shift) : sub;
-    const int lane = (threadIdx.x & 31 & ~(kLanes - 1)) + partner;
-    uint32_t o[4];
-    float z[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) z[i] = __shfl_sync(0xffffffffu, y[i], lane);
-    if (turned) {
-      const int at = 8 * (low ? sub : sub - shift);
+    for (int i = 0; i < 8; ++i) y[i] *= rs * w1[i];
+    if (shift > 0) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float s = low ? -sin_t[at + i] : sin_t[at + i];
-        y[i] = fmaf(y[i], cos_t[at + i], z[i] * s);
+        const float z = __shfl_sync(0xffffffffu, y[i], partner);
+        y[i] = fmaf(y[i], cs[i], z * sn[i]);
       }
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = pack2<BF>(y[2 * i], y[2 * i + 1]);
-    if (live) {
-      uint16_t* dst = is_k ? k_out + (rt * k_heads + (h - q_heads)) * D : q_out + (rt * q_heads + h) * D;
-      reinterpret_cast<uint4*>(dst)[sub] = make_uint4(o[0], o[1], o[2], o[3]);
+    const int h = (is_k ? p - q_passes : p) * kHeads + lane / kLanes;
+    if (h < (is_k ? k_heads : q_heads)) {
+      uint16_t* dst = is_k ? k_out + (rt * k_heads + h) * D : q_out + (rt * q_heads + h) * D;
+      reinterpret_cast<uint4*>(dst)[sub] = make_uint4(pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3]),
+                                                      pack2<BF>(y[4], y[5]), pack2<BF>(y[6], y[7]));
     }
   }
 }
@@ -152,8 +174,16 @@ extern "C" int d3b_qk_norm_mrope(const void* q, const int64_t* q_strides, int q_
   }
   const int64_t zero[3] = {0, 0, 0};
   const int64_t *qs = q_heads ? q_strides : zero, *ks = k_heads ? k_strides : zero, *ps = half ? pos_strides : zero;
-  int threads = (q_heads + k_heads) * (head_dim / 8);
-  threads = threads > 1024 ? 1024 : (threads + 31) / 32 * 32;
+  // heads at once, passes over a token's heads, and how many of them a warp takes: enough warps for
+  // 32 an SM before a warp takes a second pass
+  const int at_once = 256 / head_dim;
+  const int passes = (q_heads + at_once - 1) / at_once + (k_heads + at_once - 1) / at_once;
+  const int64_t warps = 32ll * d3b_host::num_sms(d3b_host::current_device());
+  int64_t run = tokens * passes / warps;
+  run = run < 1 ? 1 : run > passes ? passes : run;
+  const int64_t runs = (passes + run - 1) / run;
+  const int64_t ctas = (tokens * runs + kWarps - 1) / kWarps;
+  if (ctas > 0x7FFFFFFF) return D3B_EINVAL;
   auto* qp = static_cast<const uint16_t*>(q);
   auto* kp = static_cast<const uint16_t*>(k);
   auto* wq = static_cast<const uint16_t*>(q_weight);
@@ -163,8 +193,9 @@ extern "C" int d3b_qk_norm_mrope(const void* q, const int64_t* q_strides, int q_
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = dtype == D3B_BF16;
   auto launch = [&](auto kernel) {
-    kernel<<<(unsigned)tokens, threads, 0, s>>>(qp, qs[0], qs[1], qs[2], q_heads, kp, ks[0], ks[1], ks[2], k_heads, wq,
-                                                wk, positions, ps[0], ps[1], ps[2], inv_freq, ax, half, qo, ko, T, eps);
+    kernel<<<(unsigned)ctas, 32 * kWarps, 0, s>>>(qp, qs[0], qs[1], qs[2], q_heads, kp, ks[0], ks[1], ks[2], k_heads, wq,
+                                                wk, positions, ps[0], ps[1], ps[2], inv_freq, ax, half, qo, ko, T, tokens, (int)runs,
+                                                  (int)run, eps);
     return d3b_host::check_launch();
   };
   switch (head_dim) {
