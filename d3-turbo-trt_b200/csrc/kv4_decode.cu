@@ -12,12 +12,13 @@
 // brought under a power of two a row, so S has no rounding but its fp32 sums. A V row's power of
 // two cannot be applied after the sum over keys; it goes into the weight's exponent instead:
 //
-//   s_j in base 2, t_j = s_j + e_j:  O = sum_j 2^(t_j - m') (code * scale)_j,  l = sum_j 2^(s_j - m)
-//   out = O * 2^(m' - m) / l
+//   s_j in base 2, t_j = s_j + e_j, m = max t:
+//   O = sum_j 2^(t_j - m) (code * scale)_j,  l = sum_j 2^(s_j - m),  out = O / l
 //
-// with m the running maximum of s and m' of t, so that weights stay at most 1 and keep fp16's 11
-// bits whatever the rows' powers are. The weights change from accumulator to operand layout by
-// movmatrix.
+// Weights 2^(t - m) stay at most 1 and keep fp16's 11 bits whatever the rows' powers are. The terms
+// of l are fp32 numbers up to 2^64 (e >= -64); with V values beyond 2^100 the least of them fall
+// below fp32's range, keys whose weight is under 2^-9 of the largest at the very end of bf16.
+// The weights change from accumulator to operand layout by movmatrix.
 //
 // Each warp walks its own 32-key pairs of granules through its own cp.async ring, without barriers;
 // the warps' and then the key shares' partial results are merged in a fixed order.
@@ -46,17 +47,17 @@ struct DecodeArgs {
   int kv_heads, group, L, causal, splits, row_tiles;
   float scale_log2;
   float* part_o;   // [units][splits][8 NT][D]
-  float* part_st;  // [units][splits][8 NT][4]: m, m', l, -
+  float* part_st;  // [units][splits][8 NT][2]: m, l
   int* err;
 };
 
 template <int D, int NT>
 struct Shape {
   static constexpr int kStage = (granule_bytes(D) + 127) / 128 * 128;  // V rows start on 128-byte lines
-  static constexpr int kPairs = D == 256 ? 2 : 3;                      // pairs of granules in a warp's ring
   static constexpr int kRows = 8 * NT;
-  static constexpr int kRing = kWarps * kPairs * 2 * kStage;
-  static constexpr int kMerge = kWarps * kRows * (D + 4) * 4;
+  static constexpr int kResident = NT == 1 ? (D == 64 ? 5 : D == 128 ? 4 : 3) : 2;  // CTAs an SM by registers
+  static constexpr int kRing = kWarps * 2 * 2 * kStage;  // two pairs of granules a warp
+  static constexpr int kMerge = kWarps * kRows * (D + 2) * 4;
   static constexpr int kQ = kRows * D * 2;
   static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kQ + kRows * 4;
   // where a granule's parts sit in a ring stage
@@ -127,6 +128,13 @@ __device__ __forceinline__ uint32_t lds_u16(uint32_t addr) {
   return v;
 }
 
+// the low half of every byte from a, the high half from b
+__device__ __forceinline__ uint32_t low_nibbles(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xCA;" : "=r"(r) : "r"(0x0F0F0F0Fu), "r"(a), "r"(b));
+  return r;
+}
+
 template <bool BF>
 __device__ __forceinline__ float2 widen2(uint32_t w) {
   if constexpr (BF) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
@@ -142,6 +150,36 @@ __device__ __forceinline__ uint16_t narrow(float x) {
     const __half r = __float2half_rn(x);
     return *reinterpret_cast<const uint16_t*>(&r);
   }
+}
+
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+
+// byte - 127 as a float, NaN for 255
+__device__ __forceinline__ float exponent(uint32_t byte) {
+  return byte == 255u ? __int_as_float(0x7FC00000) : __uint_as_float(0x4B000000u | byte) - 8388735.f;
+}
+
+// a partial result (O, (m, l)) brought to the reference `base` and added
+__device__ __forceinline__ void add_part(float4& acc, float& sum, const float4 o, const float2 st, float base) {
+  const float f = ex2(st.x - base);
+  sum = fmaf(st.y, f, sum);
+  acc.x = fmaf(o.x, f, acc.x);
+  acc.y = fmaf(o.y, f, acc.y);
+  acc.z = fmaf(o.z, f, acc.z);
+  acc.w = fmaf(o.w, f, acc.w);
+}
+
+// four channels of a finished row; zeros where there was no key
+template <bool BF>
+__device__ __forceinline__ void store_row(const DecodeArgs& a, int b, int kvh, int row, int d, const float4 acc, float sum) {
+  const float f = sum == 0.f ? 0.f : 1.f / sum;
+  const int l = row / a.group, h = kvh * a.group + row % a.group;
+  const uint32_t lo = narrow<BF>(acc.x * f) | ((uint32_t)narrow<BF>(acc.y * f) << 16);
+  const uint32_t hi = narrow<BF>(acc.z * f) | ((uint32_t)narrow<BF>(acc.w * f) << 16);
+  *reinterpret_cast<uint2*>(a.out + b * a.so_b + h * a.so_h + l * a.so_l + d) = make_uint2(lo, hi);
 }
 
 // Queries to shared memory in operand order, as fp16 under a power of two a row:
@@ -188,7 +226,7 @@ __device__ __forceinline__ void load_queries(const DecodeArgs& a, int b, int kvh
 }
 
 template <int D, int NT, bool BF>
-__global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant__ DecodeArgs a) {
+__global__ void __launch_bounds__(kThreads, Shape<D, NT>::kResident) decode_kernel(const __grid_constant__ DecodeArgs a) {
   using P = Shape<D, NT>;
   constexpr int kKWords = D / 32, kVWords = D / 64, kTiles = D / 16;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -211,68 +249,73 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
     len = len < 0 ? 0 : most;
   }
   const int grains = (int)((len + 15) / 16);
-  const int share = (grains + a.splits - 1) / a.splits;
-  const int g_first = min(split * share, grains), g_end = min(g_first + share, grains);
+  const int share = ((grains + a.splits - 1) / a.splits + 1) & ~1;  // even: a pair starts at an even granule
+  const int g_first = (int)min((int64_t)split * share, (int64_t)grains), g_end = min(g_first + share, grains);
   const int my_first = g_first + 2 * warp;  // the warp's pairs: my_first, my_first + 2 kWarps, ...
   const int pairs = my_first < g_end ? (g_end - my_first + 2 * kWarps - 1) / (2 * kWarps) : 0;
 
-  const uint32_t ring = d3b::smem_u32(smem) + warp * (P::kPairs * 2 * P::kStage);
+  const uint32_t ring = d3b::smem_u32(smem) + warp * (2 * 2 * P::kStage);
   const int32_t* table = a.table + b * a.table_stride;
-  const int grain_shift = a.page_shift - 4;
-  int ids[2];                 // page numbers of the pair that is loaded next
-  uint32_t loaded = 0;        // bit 2 * (pair % kPairs) + i: granule i's page is in the pool
-  auto look = [&](int pair) {
+  const int grain_shift = a.page_shift - 4, in_page = (1 << grain_shift) - 1;
+  // a lane copies units lane, lane + 32, ... of 16 bytes of a granule; where each goes in a stage
+  constexpr int kUnits = granule_bytes(D) / 16, kCopies = (kUnits + 31) / 32;
+  uint32_t place[kCopies];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int g = my_first + pair * 2 * kWarps + i;
-      ids[i] = g < g_end ? __ldg(table + (g >> grain_shift)) : 0;
-    }
-  };
-  auto load = [&](int pair) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int g = my_first + pair * 2 * kWarps + i, slot = 2 * (pair % P::kPairs) + i;
-      loaded &= ~(1u << slot);
-      if (g >= g_end) continue;
-      if (ids[i] < 0 || ids[i] >= a.pages) {
-        if (lane == 0) d3b::record_device_error(a.err, kSiteBadPage);
-        continue;
-      }
-      loaded |= 1u << slot;
-      const uint8_t* src = a.pool + ids[i] * a.page_bytes + kvh * a.head_bytes +
-                           (int64_t)(g & ((1 << grain_shift) - 1)) * granule_bytes(D);
-      const uint32_t dst = ring + slot * P::kStage;
-      constexpr int kUnits = granule_bytes(D) / 16, kHalf = off_v(D) / 16, kCodes = 8 * D / 16, kScales = D / 16;
-#pragma unroll
-      for (int u0 = 0; u0 < kUnits; u0 += 32) {
-        const int u = u0 + lane;
-        if (u < kUnits) {
-          const bool is_v = u >= kHalf;
-          const int x = is_v ? u - kHalf : u;  // unit within K's or V's part
-          int to;
-          if (x < kCodes) to = is_v ? P::kVc + v_swizzle<D>(16 * x) : P::kKc + 16 * x;
-          else if (x < kCodes + kScales) to = (is_v ? P::kVs : P::kKs) + 16 * (x - kCodes);
-          else to = is_v ? P::kVe : P::kKe;
-          cp16(dst + to, src + 16 * u);
-        }
-      }
-    }
-  };
-#pragma unroll
-  for (int p = 0; p < P::kPairs - 1; ++p) {
-    if (p < pairs) {
-      look(p);
-      load(p);
-    }
-    cp_commit();
+  for (int i = 0; i < kCopies; ++i) {
+    constexpr int kHalf = off_v(D) / 16, kCodes = 8 * D / 16, kScales = D / 16;
+    const int u = 32 * i + lane;
+    const bool is_v = u >= kHalf;
+    const int x = is_v ? u - kHalf : u;  // unit within K's or V's part
+    int to;
+    if (x < kCodes) to = is_v ? P::kVc + v_swizzle<D>(16 * x) : P::kKc + 16 * x;
+    else if (x < kCodes + kScales) to = (is_v ? P::kVs : P::kKs) + 16 * (x - kCodes);
+    else to = is_v ? P::kVe : P::kKe;
+    place[i] = ring + to;
+    asm volatile("" : "+r"(place[i]));  // kept, not worked out again at every copy
   }
-  if (P::kPairs - 1 < pairs) look(P::kPairs - 1);
+  const uint8_t* head_pool = a.pool + kvh * a.head_bytes + 16 * lane;
+  int ids[2];  // page numbers of the pair that is loaded next
+  auto look = [&](int pair) {
+    const int g = my_first + pair * 2 * kWarps;
+    ids[0] = __ldg(table + (g >> grain_shift));
+    // pairs start at even granules: both lie in one page unless a page is one granule
+    ids[1] = grain_shift || g + 1 >= g_end ? ids[0] : __ldg(table + g + 1);
+  };
+  // copies a pair to ring slot SLOT; 0, or one bit for each granule whose page is not in the pool
+  auto load = [&](int pair, auto slot) -> uint32_t {
+    constexpr int kSlot = decltype(slot)::value;
+    const int g = my_first + pair * 2 * kWarps;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if ((uint32_t)ids[i] < (uint32_t)a.pages) {
+        const uint8_t* src = head_pool + ids[i] * a.page_bytes + ((g + i) & in_page) * granule_bytes(D);
+        if (i == 0 || g + 1 < g_end) {
+#pragma unroll
+          for (int x = 0; x < kCopies; ++x)
+            if (32 * x + 31 < kUnits || 32 * x + lane < kUnits)
+              cp16(place[x] + (2 * kSlot + i) * P::kStage, src + 512 * x);
+        }
+      } else {
+        bad |= 1u << i;
+        if (lane == 0) d3b::record_device_error(a.err, kSiteBadPage);
+      }
+    }
+    return bad;
+  };
+  uint32_t bad_now = 0, bad_next = 0;
+  if (pairs > 0) {
+    look(0);
+    bad_now = load(0, Int<0>{});
+  }
+  cp_commit();
+  if (pairs > 1) look(1);
 
   load_queries<D, NT, BF>(a, b, kvh, row0, rows, qs, row_scale);
   __syncthreads();
 
   float o[NT][kTiles][4];
-  float m[NT][2], mv[NT][2], l[NT][2], qf[NT][2];
+  float m[NT][2], l[NT][2], qf[NT][2];
   int limit[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -283,53 +326,71 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int row = n * 8 + 2 * c + j;
-      m[n][j] = mv[n][j] = -INFINITY;
+      m[n][j] = -INFINITY;
       l[n][j] = 0.f;
       qf[n][j] = row_scale[row];
       limit[n][j] = a.causal ? (int)len - (a.L - 1 - (row0 + row) / a.group) : (int)len;
     }
   }
+  constexpr bool kHold = NT * D <= 256;  // queries stay in registers
+  uint4 qr[kHold ? NT : 1][kHold ? kKWords : 1];
+  if constexpr (kHold) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int w = 0; w < kKWords; ++w) qr[n][w] = qs[(n * kKWords + w) * 32 + lane];
+  }
   const int first_limit = a.causal ? (int)len - (a.L - 1) : (int)len;
+  const uint32_t k_at = ring + P::kKc + r * (D / 2) + c * (D == 256 ? 16 : D / 8);
+  const uint32_t ks_at = ring + P::kKs + r * (D / 16) + (D == 64 ? c : 2 * c);
+  const uint32_t e_at = ring + P::kKe + r;
+  const uint32_t vs_at = ring + P::kVs + (D == 64 ? r / 2 : D == 128 ? r : 2 * r) * 16 + 2 * c;
+  uint32_t v_at[4];  // V rows 2c, 2c + 1, 2c + 8, 2c + 9
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    v_at[x] = ring + P::kVc + v_swizzle<D>((2 * c + (x & 1) + 8 * (x >> 1)) * (D / 2) + r * (D / 16));
 
-  for (int pair = 0; pair < pairs; ++pair) {
-    __syncwarp();  // every lane is done with the stage that is loaded next
-    if (pair + P::kPairs - 1 < pairs) {
-      load(pair + P::kPairs - 1);
-      if (pair + P::kPairs < pairs) look(pair + P::kPairs);
+  auto step = [&](int pair, auto slot) {
+    constexpr int kAt = 2 * decltype(slot)::value * P::kStage;
+    __syncwarp();  // every lane is done with the slot that is loaded next
+    if (pair + 1 < pairs) {
+      bad_next = load(pair + 1, Int<1 - decltype(slot)::value>{});
+      if (pair + 2 < pairs) look(pair + 2);
     }
     cp_commit();
-    cp_wait<P::kPairs - 1>();
+    cp_wait<1>();
     __syncwarp();
 
+    const int key0 = 16 * (my_first + pair * 2 * kWarps);
+    const bool edge = key0 + 32 > first_limit || bad_now;  // some key is masked for some row
     float s[2][NT][4], t[2][NT][4];
-    int live[2];  // tokens of the granule that are keys at all
+    int live[2] = {16, 16};  // tokens of the granule that are keys at all
+    if (edge) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) live[i] = (bad_now >> i) & 1 ? 0 : min(16, (int)len - key0 - 16 * i);
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int g = my_first + pair * 2 * kWarps + i, slot = 2 * (pair % P::kPairs) + i;
-      const uint32_t st = ring + slot * P::kStage;
-      live[i] = (loaded >> slot) & 1 ? min(16, (int)len - 16 * g) : 0;
+      const int at = kAt + i * P::kStage;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[i][n][j] = 0.f;
       uint32_t k0[kKWords], k1[kKWords], s0[kKWords / 2], s1[kKWords / 2];  // keys r and r + 8; a scale per two words
+      lds_words<D == 256 ? 4 : kKWords>(k_at + at, k0);
+      lds_words<D == 256 ? 4 : kKWords>(k_at + at + 4 * D, k1);
       if constexpr (D == 256) {
-        lds_words<4>(st + P::kKc + r * 128 + c * 16, k0);
-        lds_words<4>(st + P::kKc + r * 128 + c * 16 + 64, k0 + 4);
-        lds_words<4>(st + P::kKc + (r + 8) * 128 + c * 16, k1);
-        lds_words<4>(st + P::kKc + (r + 8) * 128 + c * 16 + 64, k1 + 4);
-      } else {
-        lds_words<kKWords>(st + P::kKc + r * (D / 2) + c * (D / 8), k0);
-        lds_words<kKWords>(st + P::kKc + (r + 8) * (D / 2) + c * (D / 8), k1);
+        lds_words<4>(k_at + at + 64, k0 + 4);
+        lds_words<4>(k_at + at + 4 * D + 64, k1 + 4);
       }
       if constexpr (D == 64) {
-        s0[0] = decode_scales(lds_u8(st + P::kKs + r * 4 + c) * 0x101u);
-        s1[0] = decode_scales(lds_u8(st + P::kKs + (r + 8) * 4 + c) * 0x101u);
+        s0[0] = decode_scales(lds_u8(ks_at + at) * 0x101u);
+        s1[0] = decode_scales(lds_u8(ks_at + at + D / 2) * 0x101u);
       } else {
 #pragma unroll
         for (int w = 0; w < kKWords / 4; ++w) {
-          const uint32_t x0 = decode_scales(lds_u16(st + P::kKs + r * (D / 16) + 8 * w + 2 * c));
-          const uint32_t x1 = decode_scales(lds_u16(st + P::kKs + (r + 8) * (D / 16) + 8 * w + 2 * c));
+          const uint32_t x0 = decode_scales(lds_u16(ks_at + at + 8 * w));
+          const uint32_t x1 = decode_scales(lds_u16(ks_at + at + D / 2 + 8 * w));
           s0[2 * w] = __byte_perm(x0, 0, 0x1010);
           s0[2 * w + 1] = __byte_perm(x0, 0, 0x3232);
           s1[2 * w] = __byte_perm(x1, 0, 0x1010);
@@ -348,15 +409,16 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const uint4 qv = qs[(n * kKWords + w) * 32 + lane];
+          uint4 qv;
+          if constexpr (kHold) qv = qr[n][w];
+          else qv = qs[(n * kKWords + w) * 32 + lane];
           mma16816(s[i][n], d0[0], d1[0], d0[1], d1[1], qv.x, qv.y);
           mma16816(s[i][n], d0[2], d1[2], d0[3], d1[3], qv.z, qv.w);
         }
       }
-      const float kf0 = row_power(lds_u8(st + P::kKe + r)), kf1 = row_power(lds_u8(st + P::kKe + r + 8));
-      const uint32_t e0 = lds_u8(st + P::kVe + r), e1 = lds_u8(st + P::kVe + r + 8);
-      const float ev0 = e0 == 255u ? __int_as_float(0x7FC00000) : (float)((int)e0 - 127);
-      const float ev1 = e1 == 255u ? __int_as_float(0x7FC00000) : (float)((int)e1 - 127);
+      // a marked row (255) has codes of zero: its score is 0 * infinity here
+      const float kf0 = __uint_as_float(lds_u8(e_at + at) << 23), kf1 = __uint_as_float(lds_u8(e_at + at + 8) << 23);
+      const float ev0 = exponent(lds_u8(e_at + at + P::kVe - P::kKe)), ev1 = exponent(lds_u8(e_at + at + P::kVe - P::kKe + 8));
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -364,11 +426,11 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
           s[i][n][j] *= (j < 2 ? kf0 : kf1) * qf[n][j & 1];
           t[i][n][j] = s[i][n][j] + (j < 2 ? ev0 : ev1);
         }
-        if (live[i] < 16 || 16 * g + 16 > first_limit) {
+        if (edge) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int key = r + (j < 2 ? 0 : 8);
-            if (key >= live[i] || 16 * g + key >= limit[n][j & 1]) s[i][n][j] = t[i][n][j] = -INFINITY;
+            if (key >= live[i] || key0 + 16 * i + key >= limit[n][j & 1]) s[i][n][j] = t[i][n][j] = -INFINITY;
           }
         }
       }
@@ -380,19 +442,16 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
       float keep[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float top = max_over_rows(fmaxf(fmaxf(s[0][n][j], s[0][n][j + 2]), fmaxf(s[1][n][j], s[1][n][j + 2])));
-        const float topv = max_over_rows(fmaxf(fmaxf(t[0][n][j], t[0][n][j + 2]), fmaxf(t[1][n][j], t[1][n][j + 2])));
-        const float new_m = fmaxf(m[n][j], top), new_mv = fmaxf(mv[n][j], topv);
-        const float base = finite_or_zero(new_m), base_v = finite_or_zero(new_mv);
-        l[n][j] *= ex2(m[n][j] - base);
-        keep[j] = ex2(mv[n][j] - base_v);
+        const float top = max_over_rows(fmaxf(fmaxf(t[0][n][j], t[0][n][j + 2]), fmaxf(t[1][n][j], t[1][n][j + 2])));
+        const float new_m = fmaxf(m[n][j], top), base = finite_or_zero(new_m);
+        keep[j] = ex2(m[n][j] - base);
         m[n][j] = new_m;
-        mv[n][j] = new_mv;
+        l[n][j] *= keep[j];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           l[n][j] += ex2(s[i][n][j] - base) + ex2(s[i][n][j + 2] - base);
-          t[i][n][j] = ex2(t[i][n][j] - base_v);
-          t[i][n][j + 2] = ex2(t[i][n][j + 2] - base_v);
+          t[i][n][j] = ex2(t[i][n][j] - base);
+          t[i][n][j + 2] = ex2(t[i][n][j + 2] - base);
         }
       }
       if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
@@ -412,33 +471,27 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
 
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint32_t st = ring + (2 * (pair % P::kPairs) + i) * P::kStage;
-      uint32_t v[4][kVWords];  // rows 2c, 2c + 1, 2c + 8, 2c + 9
+      const int at = kAt + i * P::kStage;
+      uint32_t v[4][kVWords];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int key = 2 * c + (x & 1) + 8 * (x >> 1);
-        lds_words<kVWords>(st + P::kVc + v_swizzle<D>(key * (D / 2) + r * (D / 16)), v[x]);
-      }
-      // a granule's last rows may never have been written: their scales can be NaN
-      uint32_t keep01 = 0xFFFFu, keep89 = 0xFFFFu;
-      if (live[i] < 16) {
-        keep01 = (2 * c < live[i] ? 0xFFu : 0u) | (2 * c + 1 < live[i] ? 0xFF00u : 0u);
-        keep89 = (2 * c + 8 < live[i] ? 0xFFu : 0u) | (2 * c + 9 < live[i] ? 0xFF00u : 0u);
-      }
+      for (int x = 0; x < 4; ++x) lds_words<kVWords>(v_at[x] + at, v[x]);
       uint32_t sc01 = 0, sc89 = 0;
 #pragma unroll
       for (int w = 0; w < kVWords; ++w) {
-        if (D != 256 || w % 2 == 0) {
-          const int group = D == 64 ? r / 2 : D == 128 ? r : 2 * r + w / 2;
-          sc01 = decode_scales(lds_u16(st + P::kVs + group * 16 + 2 * c) & keep01);
-          sc89 = decode_scales(lds_u16(st + P::kVs + group * 16 + 2 * c + 8) & keep89);
-          if (D == 128 && w) {}  // one group for both words
+        if (w == 0 || (D == 256 && w == 2)) {
+          uint32_t b01 = lds_u16(vs_at + at + 8 * w), b89 = lds_u16(vs_at + at + 8 * w + 8);
+          if (edge) {  // a granule's last rows may never have been written: their scales can be NaN
+            b01 &= (2 * c < live[i] ? 0xFFu : 0u) | (2 * c + 1 < live[i] ? 0xFF00u : 0u);
+            b89 &= (2 * c + 8 < live[i] ? 0xFFu : 0u) | (2 * c + 9 < live[i] ? 0xFF00u : 0u);
+          }
+          sc01 = decode_scales(b01);
+          sc89 = decode_scales(b89);
         }
         uint32_t x0[4], x1[4], y0[4], y1[4];
-        decode8((v[0][w] & 0x0F0F0F0Fu) | ((v[1][w] & 0x0F0F0F0Fu) << 4), x0);
-        decode8(((v[0][w] >> 4) & 0x0F0F0F0Fu) | (v[1][w] & 0xF0F0F0F0u), x1);
-        decode8((v[2][w] & 0x0F0F0F0Fu) | ((v[3][w] & 0x0F0F0F0Fu) << 4), y0);
-        decode8(((v[2][w] >> 4) & 0x0F0F0F0Fu) | (v[3][w] & 0xF0F0F0F0u), y1);
+        decode8(low_nibbles(v[0][w], v[1][w] << 4), x0);
+        decode8(low_nibbles(v[0][w] >> 4, v[1][w]), x1);
+        decode8(low_nibbles(v[2][w], v[3][w] << 4), y0);
+        decode8(low_nibbles(v[2][w] >> 4, v[3][w]), y1);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const uint32_t a0 = hmul2(x0[x], sc01), a1 = hmul2(x1[x], sc01), a2 = hmul2(y0[x], sc89), a3 = hmul2(y1[x], sc89);
@@ -447,13 +500,18 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
         }
       }
     }
+    bad_now = bad_next;
+  };
+  for (int pair = 0; pair < pairs; pair += 2) {
+    step(pair, Int<0>{});
+    if (pair + 1 < pairs) step(pair + 1, Int<1>{});
   }
   cp_wait<0>();
 
-  // merge the warps: O and (m, m', l) through shared memory, where the rings were
+  // merge the warps: O and (m, l) through shared memory, where the rings were
   __syncthreads();
-  float* mo = reinterpret_cast<float*>(smem);                // [warp][row][D]
-  float* ms = mo + kWarps * P::kRows * D;                    // [warp][row][4]
+  float* mo = reinterpret_cast<float*>(smem);   // [warp][row][D]
+  float* ms = mo + kWarps * P::kRows * D;       // [warp][row][2]
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -463,11 +521,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
       sum += __shfl_xor_sync(0xffffffffu, sum, 8);
       sum += __shfl_xor_sync(0xffffffffu, sum, 16);
       const int row = warp * P::kRows + n * 8 + 2 * c + j;
-      if (r == 0) {
-        ms[row * 4] = m[n][j];
-        ms[row * 4 + 1] = mv[n][j];
-        ms[row * 4 + 2] = sum;
-      }
+      if (r == 0) *reinterpret_cast<float2*>(ms + row * 2) = make_float2(m[n][j], sum);
       float* dst = mo + row * D + r * (D / 8);
 #pragma unroll
       for (int x = 0; x < kTiles; x += 2)
@@ -477,36 +531,22 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
   for (int i = threadIdx.x; i < P::kRows * (D / 4); i += kThreads) {
     const int row = i / (D / 4), d = 4 * (i % (D / 4));
     if (row0 + row >= rows) continue;
-    float top = -INFINITY, topv = -INFINITY;
+    float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      top = fmaxf(top, ms[(w * P::kRows + row) * 4]);
-      topv = fmaxf(topv, ms[(w * P::kRows + row) * 4 + 1]);
-    }
-    const float base = finite_or_zero(top), base_v = finite_or_zero(topv);
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ms[(w * P::kRows + row) * 2]);
+    const float base = finite_or_zero(top);
     float sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float* st = ms + (w * P::kRows + row) * 4;
-      sum += st[2] * ex2(st[0] - base);
-      const float f = ex2(st[1] - base_v);
-      const float4 x = *reinterpret_cast<const float4*>(mo + (w * P::kRows + row) * D + d);
-      acc.x = fmaf(x.x, f, acc.x);
-      acc.y = fmaf(x.y, f, acc.y);
-      acc.z = fmaf(x.z, f, acc.z);
-      acc.w = fmaf(x.w, f, acc.w);
+      const float2 st = *reinterpret_cast<const float2*>(ms + (w * P::kRows + row) * 2);
+      add_part(acc, sum, *reinterpret_cast<const float4*>(mo + (w * P::kRows + row) * D + d), st, base);
     }
     if (a.splits == 1) {
-      const float f = sum == 0.f ? 0.f : ex2(base_v - base) / sum;
-      const int li = (row0 + row) / a.group, h = kvh * a.group + (row0 + row) % a.group;
-      const uint32_t lo = narrow<BF>(acc.x * f) | ((uint32_t)narrow<BF>(acc.y * f) << 16);
-      const uint32_t hi = narrow<BF>(acc.z * f) | ((uint32_t)narrow<BF>(acc.w * f) << 16);
-      *reinterpret_cast<uint2*>(a.out + b * a.so_b + h * a.so_h + li * a.so_l + d) = make_uint2(lo, hi);
+      store_row<BF>(a, b, kvh, row0 + row, d, acc, sum);
     } else {
       *reinterpret_cast<float4*>(a.part_o + (part * P::kRows + row) * D + d) = acc;
-      if (d == 0)
-        *reinterpret_cast<float4*>(a.part_st + (part * P::kRows + row) * 4) = make_float4(top, topv, sum, 0.f);
+      if (d == 0) *reinterpret_cast<float2*>(a.part_st + (part * P::kRows + row) * 2) = make_float2(top, sum);
     }
   }
 }
@@ -521,32 +561,19 @@ __global__ void __launch_bounds__(D / 4) merge_kernel(const __grid_constant__ De
   const int64_t b = bk / a.kv_heads;
   const int64_t unit = bk * a.row_tiles + row / tile_rows;
   const int64_t first = unit * a.splits * tile_rows + row % tile_rows;
-  float top = -INFINITY, topv = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) {
-    const float4 st = *reinterpret_cast<const float4*>(a.part_st + (first + (int64_t)s * tile_rows) * 4);
-    top = fmaxf(top, st.x);
-    topv = fmaxf(topv, st.y);
-  }
-  const float base = finite_or_zero(top), base_v = finite_or_zero(topv);
+  float top = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_st[(first + (int64_t)s * tile_rows) * 2]);
+  const float base = finite_or_zero(top);
   float sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   const int d = 4 * threadIdx.x;
+#pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
     const int64_t at = first + (int64_t)s * tile_rows;
-    const float4 st = *reinterpret_cast<const float4*>(a.part_st + at * 4);
-    const float4 x = *reinterpret_cast<const float4*>(a.part_o + at * D + d);
-    const float f = ex2(st.y - base_v);
-    sum += st.z * ex2(st.x - base);
-    acc.x = fmaf(x.x, f, acc.x);
-    acc.y = fmaf(x.y, f, acc.y);
-    acc.z = fmaf(x.z, f, acc.z);
-    acc.w = fmaf(x.w, f, acc.w);
+    const float2 st = *reinterpret_cast<const float2*>(a.part_st + at * 2);
+    add_part(acc, sum, *reinterpret_cast<const float4*>(a.part_o + at * D + d), st, base);
   }
-  const float f = sum == 0.f ? 0.f : ex2(base_v - base) / sum;
-  const int li = row / a.group, h = kvh * a.group + row % a.group;
-  const uint32_t lo = narrow<BF>(acc.x * f) | ((uint32_t)narrow<BF>(acc.y * f) << 16);
-  const uint32_t hi = narrow<BF>(acc.z * f) | ((uint32_t)narrow<BF>(acc.w * f) << 16);
-  *reinterpret_cast<uint2*>(a.out + b * a.so_b + h * a.so_h + li * a.so_l + d) = make_uint2(lo, hi);
+  store_row<BF>(a, (int)b, kvh, row, d, acc, sum);
 }
 
 struct Plan {
@@ -562,7 +589,7 @@ bool make_plan(const d3b_kv4_cache* c, int B, int H, int L, int64_t width, Plan*
   if (tiles > 0x7FFFFFFF || p->units > 0x7FFFFFFF) return false;
   p->row_tiles = (int)tiles;
   const int64_t grains = width * (c->page_tokens / kGrain);
-  const int64_t want = 4ll * d3b_host::num_sms(d3b_host::current_device());
+  const int64_t want = 8ll * d3b_host::num_sms(d3b_host::current_device());
   int64_t splits = (want + p->units - 1) / p->units;
   const int64_t most = (grains + 2 * kWarps - 1) / (2 * kWarps);
   splits = splits > most ? most : splits;
@@ -572,7 +599,7 @@ bool make_plan(const d3b_kv4_cache* c, int B, int H, int L, int64_t width, Plan*
 }
 
 size_t plan_bytes(const Plan& p, int D) {
-  return p.splits == 1 ? 0 : (size_t)p.units * p.splits * 8 * p.nt * (D + 4) * 4;
+  return p.splits == 1 ? 0 : (size_t)p.units * p.splits * 8 * p.nt * (D + 2) * 4;
 }
 
 template <int D, int NT, bool BF>
