@@ -114,6 +114,13 @@ SIGNATURES: list[tuple[str, Any, list[Any]]] = [
         _I,
         [_CACHE, _I64, _VP, _I64P, _VP, _I64, _I64, _VP, _I, _I, _I, _I, _I, _F, _VP, _I64P, _VP, _SZ, _VP],
     ),
+    ("d3b_kv4_question_workspace_size", _SZ, [_CACHE, _I, _I, _I, _I64]),
+    (
+        "d3b_kv4_question",
+        _I,
+        [_CACHE, _I64, _VP, _I64P, _VP, _I64, _I64, _VP, _I64P, _VP, _I64P, _VP, _I, _I, _I, _I, _F, _VP, _I64P, _VP, _SZ,
+         _VP],
+    ),
     (
         "d3b_qk_norm_mrope",
         _I,

@@ -24,7 +24,7 @@ PKG = CSRC.parent
 ROOT = PKG.parent
 BUILD = PKG / "_build"
 LIB = PKG / "libd3b200.so"
-SOURCES = ["capi.cu", "act_quant.cu", "norm_quant.cu", "readout.cu", "w8a8_gemm.cu", "prefix_bidir.cu", "snapshot.cu", "gated_delta.cu", "causal_conv.cu", "glue_quant.cu", "qk_norm_rope.cu", "kv4.cu", "kv4_decode.cu", "qk_norm_mrope.cu"]
+SOURCES = ["capi.cu", "act_quant.cu", "norm_quant.cu", "readout.cu", "w8a8_gemm.cu", "prefix_bidir.cu", "snapshot.cu", "gated_delta.cu", "causal_conv.cu", "glue_quant.cu", "qk_norm_rope.cu", "kv4.cu", "kv4_decode.cu", "kv4_thin.cu", "kv4_wide.cu", "qk_norm_mrope.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
     "-O3",

@@ -1,0 +1,332 @@
+// What the attention kernels over the 4-bit cache share: operand primitives, the queries' layout in
+// shared memory, how the work is dealt out, and the merge of partial results. Layout: kv4.cuh.
+//
+// A kv head's queries (its group's heads x L tokens) are rows. Products are m16n8k16 on fp16 with
+// fp32 sums, turned so that keys (then channels) are the 16 and query rows the 8:
+//
+//   S^T [16 keys x 8 rows]  = K [16 keys x D] . Q^T         A = decoded K codes
+//   O^T [D x 8 rows]       += V^T [D x 16 keys] . W^T       A = decoded V codes
+//
+// Every thread decodes its own operand from the bytes it needs (a K row's quarter is 16 bytes at
+// D = 128), so nothing is widened in shared memory. code * scale is exact in fp16 and queries are
+// brought under a power of two a row, so S has no rounding but its fp32 sums. A V row's power of
+// two cannot be applied after the sum over keys; it goes into the weight's exponent instead:
+//
+//   s_j in base 2, t_j = s_j + e_j, m = max t:
+//   O = sum_j 2^(t_j - m) (code * scale)_j,  l = sum_j 2^(s_j - m),  out = O / l
+//
+// Weights 2^(t - m) stay at most 1 and keep fp16's 11 bits whatever the rows' powers are. The terms
+// of l are fp32 numbers up to 2^64 (e >= -64); with V values beyond 2^100 the least of them fall
+// below fp32's range, keys whose weight is under 2^-9 of the largest at the very end of bf16.
+// The weights change from accumulator to operand layout by movmatrix.
+//
+// Work is dealt out evenly whatever the lengths are: all units (sequence, kv head, tile of rows)
+// are cut into pieces of keys, laid end to end, and every CTA takes the same number of pieces. A
+// unit that lies in one CTA is finished there; the others leave partial results, at most two a
+// CTA, which a second kernel adds in order.
+#pragma once
+
+#include "kv4.cuh"
+
+namespace d3b_kv4 {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kSiteOwnLength = 2010;  // a question block's length outside [0, L]
+
+struct AttnArgs {
+  const uint8_t* pool;
+  int64_t page_bytes, head_bytes;
+  int pages, page_shift;
+  const uint16_t* q;
+  int64_t sq_b, sq_h, sq_l;
+  uint16_t* out;
+  int64_t so_b, so_h, so_l;
+  const int32_t* table;
+  int64_t table_stride;    // 0: one table for all sequences
+  const int32_t* lengths;  // cached tokens of each sequence; NULL: `most` for all
+  int most;                // cached tokens a table can hold
+  // a block's own keys in 16 bits, or NULL: k, v [B, kv_heads, L, D]
+  const uint16_t *k_own, *v_own;
+  int64_t sk_b, sk_h, sk_l, sv_b, sv_h, sv_l;
+  const int32_t* own_lengths;
+  int B, kv_heads, group, L, causal, row_tiles;
+  float scale_log2;
+  float* part_o;   // [CTAs][2][rows][D]
+  float* part_st;  // [CTAs][2][rows][2]: m, l
+  int2* ranges;    // [units]: the first and the last CTA that hold a part of the unit
+  int* err;
+};
+
+int launch_thin(const AttnArgs& a, int D, int nt, bool bf, int ctas, cudaStream_t s);
+int launch_wide(const AttnArgs& a, int D, int nt, bool bf, int ctas, cudaStream_t s);
+int resident_thin(int D, int nt);  // CTAs an SM holds
+int resident_wide(int D, int nt);
+
+// 16-byte unit of a V code line (128 bytes): spread so that the four row pairs of a load's lanes hit all banks
+template <int D>
+__device__ __forceinline__ int v_swizzle(int byte) {
+  const int line = byte >> 7;
+  const int x = D == 64 ? (line & 1) : D == 128 ? (line & 3) : ((line >> 1) & 3);
+  return byte ^ (x << 5);
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float max_over_rows(float x) {  // over the 8 lanes that share lane % 4; a NaN gives way
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+}
+
+__device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
+
+template <int W>
+__device__ __forceinline__ void lds_words(uint32_t addr, uint32_t* w) {
+  if constexpr (W == 1)
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+  else if constexpr (W == 2)
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+  else
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+}
+__device__ __forceinline__ uint32_t lds_u8(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_u16(uint32_t addr) {
+  uint32_t v;
+  asm volatile("{\n\t.reg .b16 h;\n\tld.shared.b16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}" : "=r"(v) : "r"(addr));
+  return v;
+}
+
+// the low half of every byte from a, the high half from b
+__device__ __forceinline__ uint32_t low_nibbles(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xCA;" : "=r"(r) : "r"(0x0F0F0F0Fu), "r"(a), "r"(b));
+  return r;
+}
+
+template <bool BF>
+__device__ __forceinline__ float2 widen2(uint32_t w) {
+  if constexpr (BF) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+template <bool BF>
+__device__ __forceinline__ uint16_t narrow(float x) {
+  if constexpr (BF) {
+    const __nv_bfloat16 r = __float2bfloat16_rn(x);
+    return *reinterpret_cast<const uint16_t*>(&r);
+  } else {
+    const __half r = __float2half_rn(x);
+    return *reinterpret_cast<const uint16_t*>(&r);
+  }
+}
+
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+
+// byte - 127 as a float, NaN for 255
+__device__ __forceinline__ float exponent(uint32_t byte) {
+  return byte == 255u ? __int_as_float(0x7FC00000) : __uint_as_float(0x4B000000u | byte) - 8388735.f;
+}
+
+// the power of two that brings a row's largest magnitude to [2^14, 2^15), as far as 2^126 goes; rows
+// that are not finite stay
+__device__ __forceinline__ int row_up(float top) {
+  return top < INFINITY ? min(126, 14 - ((int)(__float_as_uint(top) >> 23) - 127)) : 0;
+}
+__device__ __forceinline__ float power_of(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // e in [-126, 127]
+
+// a partial result (O, (m, l)) brought to the reference `base` and added
+__device__ __forceinline__ void add_part(float4& acc, float& sum, const float4 o, const float2 st, float base) {
+  const float f = ex2(st.x - base);
+  sum = fmaf(st.y, f, sum);
+  acc.x = fmaf(o.x, f, acc.x);
+  acc.y = fmaf(o.y, f, acc.y);
+  acc.z = fmaf(o.z, f, acc.z);
+  acc.w = fmaf(o.w, f, acc.w);
+}
+
+// four channels of a finished row; zeros where there was no key or the token is behind its block's length
+template <bool BF>
+__device__ __forceinline__ void store_row(const AttnArgs& a, int b, int kvh, int row, int tokens, int d, const float4 acc,
+                                          float sum) {
+  const int l = row / a.group, h = kvh * a.group + row % a.group;
+  uint32_t lo = 0, hi = 0;
+  if (sum != 0.f && l < tokens) {
+    const float f = 1.f / sum;
+    lo = narrow<BF>(acc.x * f) | ((uint32_t)narrow<BF>(acc.y * f) << 16);
+    hi = narrow<BF>(acc.z * f) | ((uint32_t)narrow<BF>(acc.w * f) << 16);
+  }
+  *reinterpret_cast<uint2*>(a.out + b * a.so_b + h * a.so_h + l * a.so_l + d) = make_uint2(lo, hi);
+}
+
+// a sequence's lengths, and its units' pieces
+struct Sequence {
+  int len, own, tokens;  // cached keys, own keys, tokens of the block that are real
+  int cached, pieces;    // pieces of cached keys; of all keys, at least one
+  int live;              // row tiles with real tokens; each other tile is one piece that writes zeros
+  int per_head, total;   // pieces of a kv head and of the sequence
+};
+
+template <int KEYS, int ROWS>
+__device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b, bool report) {
+  Sequence s;
+  s.len = a.most;
+  if (a.lengths) {
+    s.len = __ldg(a.lengths + b);
+    if (s.len < 0 || s.len > a.most) {
+      if (report) d3b::record_device_error(a.err, kSiteBadLength);
+      s.len = s.len < 0 ? 0 : a.most;
+    }
+  }
+  s.own = 0;
+  s.tokens = a.L;
+  if (a.own_lengths) {
+    s.own = __ldg(a.own_lengths + b);
+    if (s.own < 0 || s.own > a.L) {
+      if (report) d3b::record_device_error(a.err, kSiteOwnLength);
+      s.own = s.own < 0 ? 0 : a.L;
+    }
+    s.tokens = s.own;
+  }
+  s.cached = (s.len + KEYS - 1) / KEYS;
+  s.pieces = max(1, s.cached + (s.own + KEYS - 1) / KEYS);
+  s.live = (s.tokens * a.group + ROWS - 1) / ROWS;
+  s.per_head = s.live * s.pieces + a.row_tiles - s.live;
+  s.total = a.kv_heads * s.per_head;
+  return s;
+}
+
+// where a CTA's pieces begin
+struct Deal {
+  int first, last;  // its pieces
+  int share;
+  int b, offset;  // the sequence of the first, and how far into it
+};
+
+// Sums the sequences' pieces and finds the CTA's share; all threads, `box` in shared memory.
+template <int KEYS, int ROWS>
+__device__ __forceinline__ Deal deal(const AttnArgs& a, int at_least, int* box) {
+  const int per = (a.B + kThreads - 1) / kThreads, t = threadIdx.x, warp = t / 32, lane = t % 32;
+  const int b0 = min(t * per, a.B), b1 = min(b0 + per, a.B);
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) mine += sequence<KEYS, ROWS>(a, b, blockIdx.x == 0).total;
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 31) box[warp] = upto;
+  __syncthreads();
+  int before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    before += w < warp ? box[w] : 0;
+    total += box[w];
+  }
+  before += upto - mine;
+  Deal d;
+  d.share = max(at_least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+  d.first = (int)min((int64_t)blockIdx.x * d.share, (int64_t)total);
+  d.last = min(d.first + d.share, total);  // shares are far below 2^31 when first is not the total
+  if (d.first >= before && d.first < before + mine) {
+    int b = b0, at = before;
+    for (;; ++b) {
+      const int n = sequence<KEYS, ROWS>(a, b, false).total;
+      if (d.first < at + n) break;
+      at += n;
+    }
+    box[kWarps] = b;
+    box[kWarps + 1] = d.first - at;
+  }
+  __syncthreads();
+  d.b = box[kWarps];
+  d.offset = box[kWarps + 1];
+  return d;
+}
+
+// Queries to shared memory in operand order, as fp16 under a power of two a row:
+// [nt][word][lane] x 16 bytes, lane = 4 * row + quarter; row_scale = scale * log2(e) * 2^power.
+template <int D, int NT, bool BF>
+__device__ __forceinline__ void load_queries(const AttnArgs& a, int b, int kvh, int row0, int rows, uint4* qs,
+                                             float* row_scale) {
+  constexpr int kLanes = D / 8;  // a lane takes 8 channels
+  constexpr int kWords = D / 32;
+  for (int i = threadIdx.x; i < 8 * NT * kLanes; i += kThreads) {
+    const int row = i / kLanes, sub = i % kLanes;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (row0 + row < rows) {
+      const int l = (row0 + row) / a.group, g = (row0 + row) % a.group;
+      raw = __ldg(reinterpret_cast<const uint4*>(a.q + b * a.sq_b + (int64_t)(kvh * a.group + g) * a.sq_h + l * a.sq_l) + sub);
+    }
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    float2 f[4];
+    float top = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f[j] = widen2<BF>(w[j]);
+      top = fmaxf(top, fmaxf(fabsf(f[j].x), fabsf(f[j].y)));
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int up = row_up(top);
+    const float by = power_of(up);
+    uint32_t h[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __half2 v = __floats2half2_rn(f[j].x * by, f[j].y * by);
+      h[j] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    // channels 8 sub ...: which word of which quarter they are (see the K loads)
+    const int half = D == 256 ? sub / 16 : 0, in = D == 256 ? sub % 16 : sub;
+    const int per = D == 256 ? 4 : kWords;
+    const int quarter = in / per, word = half * 4 + in % per;
+    qs[((row / 8) * kWords + word) * 32 + (row % 8) * 4 + quarter] = make_uint4(h[0], h[1], h[2], h[3]);
+    if (sub == 0) row_scale[row] = a.scale_log2 * power_of(-up);
+  }
+}
+
+// lets `kernel` have `bytes` of dynamic shared memory, once a device (`ready` by device; twice is harmless)
+template <typename K>
+inline int allow_smem(K kernel, int bytes, bool (&ready)[64]) {
+  const int dev = d3b_host::current_device();
+  if (bytes <= 48 * 1024 || (dev >= 0 && dev < 64 && ready[dev])) return D3B_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return D3B_ECUDA;
+  if (dev >= 0 && dev < 64) ready[dev] = true;
+  return D3B_OK;
+}
+
+}  // namespace d3b_kv4

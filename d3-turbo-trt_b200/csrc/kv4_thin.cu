@@ -1,0 +1,389 @@
+// Attention over the 4-bit cache for few query rows a kv head (up to 16): decoding.
+//
+// A warp takes pairs of granules (32 keys) by itself, from its own cp.async ring of two pairs and
+// without barriers, and keeps all of O for its rows; a unit's warps are merged at the end of the
+// CTA's share. One m16n8k16 serves 8 rows, so a group of up to 8 heads costs one product.
+//
+// Bound: the cache's bytes, 18 D + 32 for 16 tokens and kv head, with the ALU close behind: a code
+// pair costs a conversion (64 lanes a clock and SM) and a product with its scale.
+#include "kv4_attn.cuh"
+
+namespace d3b_kv4 {
+namespace {
+
+constexpr int kKeys = 32;
+constexpr int kLeast = kWarps;  // pieces a CTA takes at least: one a warp
+
+template <int D, int NT>
+struct Thin {
+  static constexpr int kStage = (granule_bytes(D) + 127) / 128 * 128;  // V rows start on 128-byte lines
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kResident = NT == 1 ? (D == 64 ? 5 : D == 128 ? 4 : 3) : 2;  // CTAs an SM by registers
+  static constexpr int kRing = kWarps * 2 * 2 * kStage;                             // two pairs of granules a warp
+  static constexpr int kMerge = kWarps * kRows * (D + 2) * 4;
+  static constexpr int kQ = kRows * D * 2;
+  static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kQ + kRows * 4;
+  // where a granule's parts sit in a ring stage
+  static constexpr int kKc = 0, kVc = 8 * D, kKs = 16 * D, kVs = 17 * D, kKe = 18 * D, kVe = 18 * D + 16;
+};
+
+template <int D, int NT, bool BF>
+__global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(const __grid_constant__ AttnArgs a) {
+  using P = Thin<D, NT>;
+  constexpr int kKWords = D / 32, kVWords = D / 64, kTiles = D / 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int box[kWarps + 2];
+  uint4* qs = reinterpret_cast<uint4*>(smem + (P::kRing > P::kMerge ? P::kRing : P::kMerge));
+  float* row_scale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(qs) + P::kQ);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
+  const int rows = a.group * a.L;
+  const Deal mine = deal<kKeys, P::kRows>(a, kLeast, box);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may take its place; it waits for our end
+  const uint32_t ring = d3b::smem_u32(smem) + warp * (2 * 2 * P::kStage);
+  const int grain_shift = a.page_shift - 4, in_page = (1 << grain_shift) - 1;
+  // a lane copies units lane, lane + 32, ... of 16 bytes of a granule; where each goes in a stage
+  constexpr int kUnits = granule_bytes(D) / 16, kCopies = (kUnits + 31) / 32;
+  uint32_t place[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    constexpr int kHalf = off_v(D) / 16, kCodes = 8 * D / 16, kScales = D / 16;
+    const int u = 32 * i + lane;
+    const bool is_v = u >= kHalf;
+    const int x = is_v ? u - kHalf : u;  // unit within K's or V's part
+    int to;
+    if (x < kCodes) to = is_v ? P::kVc + v_swizzle<D>(16 * x) : P::kKc + 16 * x;
+    else if (x < kCodes + kScales) to = (is_v ? P::kVs : P::kKs) + 16 * (x - kCodes);
+    else to = is_v ? P::kVe : P::kKe;
+    place[i] = ring + to;
+    asm volatile("" : "+r"(place[i]));  // kept, not worked out again at every copy
+  }
+
+  int pos = mine.first, b = mine.b, offset = mine.offset;
+  while (pos < mine.last) {
+    const Sequence seq = sequence<kKeys, P::kRows>(a, b, false);
+    const int kvh = offset / seq.per_head, tile = (offset - kvh * seq.per_head) / seq.pieces;  // every tile is live
+    const int piece0 = offset - kvh * seq.per_head - tile * seq.pieces, piece1 = min(seq.pieces, piece0 + mine.last - pos);
+    const int row0 = tile * P::kRows, len = seq.len, grains = (len + 15) / 16;
+    const int my_first = 2 * (piece0 + warp), g_end = min(2 * piece1, grains);  // pairs my_first, + 2 kWarps, ...
+    const int pairs = my_first < g_end ? (g_end - my_first + 2 * kWarps - 1) / (2 * kWarps) : 0;
+    const uint8_t* head_pool = a.pool + kvh * a.head_bytes + 16 * lane;
+    const int32_t* table = a.table + b * a.table_stride;
+    int ids[2];  // page numbers of the pair that is loaded next
+    auto look = [&](int pair) {
+      const int g = my_first + pair * 2 * kWarps;
+      ids[0] = __ldg(table + (g >> grain_shift));
+      // pairs start at even granules: both lie in one page unless a page is one granule
+      ids[1] = grain_shift || g + 1 >= g_end ? ids[0] : __ldg(table + g + 1);
+    };
+    // copies a pair to ring slot SLOT; 0, or one bit for each granule whose page is not in the pool
+    auto load = [&](int pair, auto slot) -> uint32_t {
+      constexpr int kSlot = decltype(slot)::value;
+      const int g = my_first + pair * 2 * kWarps;
+      uint32_t bad = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if ((uint32_t)ids[i] < (uint32_t)a.pages) {
+          const uint8_t* src = head_pool + ids[i] * a.page_bytes + ((g + i) & in_page) * granule_bytes(D);
+          if (i == 0 || g + 1 < g_end) {
+#pragma unroll
+            for (int x = 0; x < kCopies; ++x)
+              if (32 * x + 31 < kUnits || 32 * x + lane < kUnits)
+                cp16(place[x] + (2 * kSlot + i) * P::kStage, src + 512 * x);
+          }
+        } else {
+          bad |= 1u << i;
+          if (lane == 0) d3b::record_device_error(a.err, kSiteBadPage);
+        }
+      }
+      return bad;
+    };
+    uint32_t bad_now = 0, bad_next = 0;
+    if (pairs > 0) {
+      look(0);
+      bad_now = load(0, Int<0>{});
+    }
+    cp_commit();
+    if (pairs > 1) look(1);
+
+    load_queries<D, NT, BF>(a, b, kvh, row0, rows, qs, row_scale);
+    __syncthreads();
+
+    float o[NT][kTiles][4];
+    float m[NT][2], l[NT][2], qf[NT][2];
+    int limit[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][t][j] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = n * 8 + 2 * c + j;
+        m[n][j] = -INFINITY;
+        l[n][j] = 0.f;
+        qf[n][j] = row_scale[row];
+        limit[n][j] = a.causal ? len - (a.L - 1 - (row0 + row) / a.group) : len;
+      }
+    }
+    constexpr bool kHold = NT * D <= 256;  // queries stay in registers
+    uint4 qr[kHold ? NT : 1][kHold ? kKWords : 1];
+    if constexpr (kHold) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int w = 0; w < kKWords; ++w) qr[n][w] = qs[(n * kKWords + w) * 32 + lane];
+    }
+    const int first_limit = a.causal ? len - (a.L - 1) : len;
+    const uint32_t k_at = ring + P::kKc + r * (D / 2) + c * (D == 256 ? 16 : D / 8);
+    const uint32_t ks_at = ring + P::kKs + r * (D / 16) + (D == 64 ? c : 2 * c);
+    const uint32_t e_at = ring + P::kKe + r;
+    const uint32_t vs_at = ring + P::kVs + (D == 64 ? r / 2 : D == 128 ? r : 2 * r) * 16 + 2 * c;
+    uint32_t v_at[4];  // V rows 2c, 2c + 1, 2c + 8, 2c + 9
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      v_at[x] = ring + P::kVc + v_swizzle<D>((2 * c + (x & 1) + 8 * (x >> 1)) * (D / 2) + r * (D / 16));
+
+    auto step = [&](int pair, auto slot) {
+      constexpr int kAt = 2 * decltype(slot)::value * P::kStage;
+      __syncwarp();  // every lane is done with the slot that is loaded next
+      if (pair + 1 < pairs) {
+        bad_next = load(pair + 1, Int<1 - decltype(slot)::value>{});
+        if (pair + 2 < pairs) look(pair + 2);
+      }
+      cp_commit();
+      cp_wait<1>();
+      __syncwarp();
+
+      const int key0 = 16 * (my_first + pair * 2 * kWarps);
+      const bool edge = key0 + 32 > first_limit || bad_now;  // some key is masked for some row
+      float s[2][NT][4], t[2][NT][4];
+      int live[2] = {16, 16};  // tokens of the granule that are keys at all
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) live[i] = (bad_now >> i) & 1 ? 0 : min(16, len - key0 - 16 * i);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = kAt + i * P::kStage;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[i][n][j] = 0.f;
+        uint32_t k0[kKWords], k1[kKWords], s0[kKWords / 2], s1[kKWords / 2];  // keys r and r + 8; a scale per two words
+        lds_words<D == 256 ? 4 : kKWords>(k_at + at, k0);
+        lds_words<D == 256 ? 4 : kKWords>(k_at + at + 4 * D, k1);
+        if constexpr (D == 256) {
+          lds_words<4>(k_at + at + 64, k0 + 4);
+          lds_words<4>(k_at + at + 4 * D + 64, k1 + 4);
+        }
+        if constexpr (D == 64) {
+          s0[0] = decode_scales(lds_u8(ks_at + at) * 0x101u);
+          s1[0] = decode_scales(lds_u8(ks_at + at + D / 2) * 0x101u);
+        } else {
+#pragma unroll
+          for (int w = 0; w < kKWords / 4; ++w) {
+            const uint32_t x0 = decode_scales(lds_u16(ks_at + at + 8 * w));
+            const uint32_t x1 = decode_scales(lds_u16(ks_at + at + D / 2 + 8 * w));
+            s0[2 * w] = __byte_perm(x0, 0, 0x1010);
+            s0[2 * w + 1] = __byte_perm(x0, 0, 0x3232);
+            s1[2 * w] = __byte_perm(x1, 0, 0x1010);
+            s1[2 * w + 1] = __byte_perm(x1, 0, 0x3232);
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < kKWords; ++w) {
+          uint32_t d0[4], d1[4];
+          decode8(k0[w], d0);
+          decode8(k1[w], d1);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            d0[j] = hmul2(d0[j], s0[w / 2]);
+            d1[j] = hmul2(d1[j], s1[w / 2]);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            uint4 qv;
+            if constexpr (kHold) qv = qr[n][w];
+            else qv = qs[(n * kKWords + w) * 32 + lane];
+            mma16816(s[i][n], d0[0], d1[0], d0[1], d1[1], qv.x, qv.y);
+            mma16816(s[i][n], d0[2], d1[2], d0[3], d1[3], qv.z, qv.w);
+          }
+        }
+        // a marked row (255) has codes of zero: its score is 0 * infinity here
+        const float kf0 = __uint_as_float(lds_u8(e_at + at) << 23), kf1 = __uint_as_float(lds_u8(e_at + at + 8) << 23);
+        const float ev0 = exponent(lds_u8(e_at + at + P::kVe - P::kKe)), ev1 = exponent(lds_u8(e_at + at + P::kVe - P::kKe + 8));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[i][n][j] *= (j < 2 ? kf0 : kf1) * qf[n][j & 1];
+            t[i][n][j] = s[i][n][j] + (j < 2 ? ev0 : ev1);
+          }
+          if (edge) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int key = r + (j < 2 ? 0 : 8);
+              if (key >= live[i] || key0 + 16 * i + key >= limit[n][j & 1]) s[i][n][j] = t[i][n][j] = -INFINITY;
+            }
+          }
+        }
+      }
+
+      uint32_t wf[2][NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float keep[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float top = max_over_rows(fmaxf(fmaxf(t[0][n][j], t[0][n][j + 2]), fmaxf(t[1][n][j], t[1][n][j + 2])));
+          const float new_m = fmaxf(m[n][j], top), base = finite_or_zero(new_m);
+          keep[j] = ex2(m[n][j] - base);
+          m[n][j] = new_m;
+          l[n][j] *= keep[j];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            l[n][j] += ex2(s[i][n][j] - base) + ex2(s[i][n][j + 2] - base);
+            t[i][n][j] = ex2(t[i][n][j] - base);
+            t[i][n][j + 2] = ex2(t[i][n][j + 2] - base);
+          }
+        }
+        if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
+#pragma unroll
+          for (int x = 0; x < kTiles; ++x)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[n][x][j] *= keep[j & 1];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const __half2 h = __floats2half2_rn(t[i][n][2 * j], t[i][n][2 * j + 1]);
+            wf[i][n][j] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h));
+          }
+      }
+
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = kAt + i * P::kStage;
+        uint32_t v[4][kVWords];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) lds_words<kVWords>(v_at[x] + at, v[x]);
+        uint32_t sc01 = 0, sc89 = 0;
+#pragma unroll
+        for (int w = 0; w < kVWords; ++w) {
+          if (w == 0 || (D == 256 && w == 2)) {
+            uint32_t b01 = lds_u16(vs_at + at + 8 * w), b89 = lds_u16(vs_at + at + 8 * w + 8);
+            if (edge) {  // a granule's last rows may never have been written: their scales can be NaN
+              b01 &= (2 * c < live[i] ? 0xFFu : 0u) | (2 * c + 1 < live[i] ? 0xFF00u : 0u);
+              b89 &= (2 * c + 8 < live[i] ? 0xFFu : 0u) | (2 * c + 9 < live[i] ? 0xFF00u : 0u);
+            }
+            sc01 = decode_scales(b01);
+            sc89 = decode_scales(b89);
+          }
+          uint32_t x0[4], x1[4], y0[4], y1[4];
+          decode8(low_nibbles(v[0][w], v[1][w] << 4), x0);
+          decode8(low_nibbles(v[0][w] >> 4, v[1][w]), x1);
+          decode8(low_nibbles(v[2][w], v[3][w] << 4), y0);
+          decode8(low_nibbles(v[2][w] >> 4, v[3][w]), y1);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint32_t a0 = hmul2(x0[x], sc01), a1 = hmul2(x1[x], sc01), a2 = hmul2(y0[x], sc89), a3 = hmul2(y1[x], sc89);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816(o[n][4 * w + x], a0, a1, a2, a3, wf[i][n][0], wf[i][n][1]);
+          }
+        }
+      }
+      bad_now = bad_next;
+    };
+    for (int pair = 0; pair < pairs; pair += 2) {
+      step(pair, Int<0>{});
+      if (pair + 1 < pairs) step(pair + 1, Int<1>{});
+    }
+    cp_wait<0>();
+
+    // merge the warps: O and (m, l) through shared memory, where the rings were
+    __syncthreads();
+    float* mo = reinterpret_cast<float*>(smem);   // [warp][row][D]
+    float* ms = mo + kWarps * P::kRows * D;       // [warp][row][2]
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float sum = l[n][j];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const int row = warp * P::kRows + n * 8 + 2 * c + j;
+        if (r == 0) *reinterpret_cast<float2*>(ms + row * 2) = make_float2(m[n][j], sum);
+        float* dst = mo + row * D + r * (D / 8);
+#pragma unroll
+        for (int x = 0; x < kTiles; x += 2)
+          *reinterpret_cast<float4*>(dst + 2 * x) =
+              make_float4(o[n][x][j], o[n][x][j + 2], o[n][x + 1][j], o[n][x + 1][j + 2]);
+      }
+    __syncthreads();
+    const bool whole = piece0 == 0 && piece1 == seq.pieces;
+    const int64_t part = 2 * (int64_t)blockIdx.x + (piece0 == 0);
+    for (int i = threadIdx.x; i < P::kRows * (D / 4); i += kThreads) {
+      const int row = i / (D / 4), d = 4 * (i % (D / 4));
+      if (row0 + row >= rows) continue;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ms[(w * P::kRows + row) * 2]);
+      const float base = finite_or_zero(top);
+      float sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 st = *reinterpret_cast<const float2*>(ms + (w * P::kRows + row) * 2);
+        add_part(acc, sum, *reinterpret_cast<const float4*>(mo + (w * P::kRows + row) * D + d), st, base);
+      }
+      if (whole) {
+        store_row<BF>(a, b, kvh, row0 + row, seq.tokens, d, acc, sum);
+      } else {
+        *reinterpret_cast<float4*>(a.part_o + (part * P::kRows + row) * D + d) = acc;
+        if (d == 0) *reinterpret_cast<float2*>(a.part_st + (part * P::kRows + row) * 2) = make_float2(top, sum);
+      }
+    }
+    if (piece0 == 0 && threadIdx.x == 0)
+      a.ranges[((int64_t)b * a.kv_heads + kvh) * a.row_tiles + tile] =
+          make_int2(pos / mine.share, (pos + seq.pieces - 1) / mine.share);
+    __syncthreads();  // the rings and the queries are free again
+    pos += piece1 - piece0;
+    offset += piece1 - piece0;
+    if (offset == seq.total) {
+      offset = 0;
+      ++b;
+    }
+  }
+}
+
+template <int D, int NT, bool BF>
+int launch(const AttnArgs& a, int ctas, cudaStream_t s) {
+  constexpr int smem = Thin<D, NT>::kSmem;
+  static bool ready[64];
+  if (int rc = allow_smem(thin_kernel<D, NT, BF>, smem, ready)) return rc;
+  thin_kernel<D, NT, BF><<<(unsigned)ctas, kThreads, smem, s>>>(a);
+  return d3b_host::check_launch();
+}
+
+template <int D>
+int pick(const AttnArgs& a, int nt, bool bf, int ctas, cudaStream_t s) {
+  if (nt == 1) return bf ? launch<D, 1, true>(a, ctas, s) : launch<D, 1, false>(a, ctas, s);
+  if constexpr (D < 256) return bf ? launch<D, 2, true>(a, ctas, s) : launch<D, 2, false>(a, ctas, s);
+  return D3B_EUNSUPPORTED;
+}
+
+}  // namespace
+
+int launch_thin(const AttnArgs& a, int D, int nt, bool bf, int ctas, cudaStream_t s) {
+  return D == 64 ? pick<64>(a, nt, bf, ctas, s) : D == 128 ? pick<128>(a, nt, bf, ctas, s) : pick<256>(a, nt, bf, ctas, s);
+}
+
+int resident_thin(int D, int nt) {
+  return nt == 1 ? (D == 64 ? Thin<64, 1>::kResident : D == 128 ? Thin<128, 1>::kResident : Thin<256, 1>::kResident)
+                 : Thin<128, 2>::kResident;
+}
+
+}  // namespace d3b_kv4

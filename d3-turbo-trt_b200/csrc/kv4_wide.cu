@@ -1,0 +1,520 @@
+// Attention over the 4-bit cache for up to 32 query rows at a time: several new tokens a sequence, wide
+// groups, and question blocks with their own keys beside the cached state.
+//
+// A CTA's four warps share tiles of 64 keys. Each takes the scores of 16 of them against all rows,
+// so every K code is decoded once for 32 rows; the weights go through shared memory in operand
+// layout, and each warp then adds a quarter of the channels over all 64 keys, so every V code is
+// decoded once too and O is 1/4 of the rows' channels in a warp's registers. Two barriers a tile:
+// maxima, weights.
+//
+// A block's own keys are tiles of the same kind whose operands come from the 16-bit rows: brought
+// under a power of two a row, so that bf16 values fit fp16 without rounding.
+//
+// Bound: products. 32 rows x 64 keys are 4 D m16n8k16, 8 clocks each on one of four tensor pipes;
+// at D = 256 they take 1.3 times as long as the cache's bytes.
+#include "kv4_attn.cuh"
+
+namespace d3b_kv4 {
+namespace {
+
+constexpr int kKeys = 64;
+
+template <int D, int NT>
+struct Wide {
+  static constexpr int kStage = (granule_bytes(D) + 127) / 128 * 128;
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kResident = 3;
+  static constexpr int kRing = 2 * 4 * kStage;  // two tiles of four granules
+  static constexpr int kQ = kRows * D * 2;
+  static constexpr int kW = 4 * NT * 32 * 8;    // weights: [granule][nt][lane] x 8 bytes
+  static constexpr int kMax = kWarps * kRows * 4;
+  static constexpr int kSmem = kRing + kQ + kW + kMax + kRows * 4 + kKeys * 4;
+  static constexpr int kKc = 0, kVc = 8 * D, kKs = 16 * D, kVs = 17 * D, kKe = 18 * D, kVe = 18 * D + 16;
+};
+
+__device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int D, int NT, bool BF>
+__global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(const __grid_constant__ AttnArgs a) {
+  using P = Wide<D, NT>;
+  constexpr int kKWords = D / 32, kTiles = D / 64;  // a lane's K words; a warp's 16-channel tiles
+  constexpr int kRun = D / 32;                      // channels of V a lane has
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int box[kWarps + 2];
+  uint4* qs = reinterpret_cast<uint4*>(smem + P::kRing);
+  uint2* ws = reinterpret_cast<uint2*>(smem + P::kRing + P::kQ);
+  float* maxima = reinterpret_cast<float*>(smem + P::kRing + P::kQ + P::kW);  // [warp][row]
+  float* row_scale = maxima + kWarps * P::kRows;
+  float* own_scale = row_scale + P::kRows;  // [key]: what an own V row is multiplied by
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
+  const int rows = a.group * a.L;
+  const Deal mine = deal<kKeys, P::kRows>(a, 1, box);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may take its place; it waits for our end
+  const uint32_t ring = d3b::smem_u32(smem);
+  const int grain_shift = a.page_shift - 4, in_page = (1 << grain_shift) - 1;
+  // a lane copies units lane, lane + 32, ... of 16 bytes of its warp's granule; where each goes in a tile
+  constexpr int kUnits = granule_bytes(D) / 16, kCopies = (kUnits + 31) / 32;
+  uint32_t place[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    constexpr int kHalf = off_v(D) / 16, kCodes = 8 * D / 16, kScales = D / 16;
+    const int u = 32 * i + lane;
+    const bool is_v = u >= kHalf;
+    const int x = is_v ? u - kHalf : u;
+    int to;
+    if (x < kCodes) to = is_v ? P::kVc + v_swizzle<D>(16 * x) : P::kKc + 16 * x;
+    else if (x < kCodes + kScales) to = (is_v ? P::kVs : P::kKs) + 16 * (x - kCodes);
+    else to = is_v ? P::kVe : P::kKe;
+    place[i] = ring + warp * P::kStage + to;
+    asm volatile("" : "+r"(place[i]));  // kept, not worked out again at every copy
+  }
+  const uint32_t stage = ring + warp * P::kStage;
+  const uint32_t k_at = stage + P::kKc + r * (D / 2) + c * (D == 256 ? 16 : D / 8);
+  const uint32_t ks_at = stage + P::kKs + r * (D / 16) + (D == 64 ? c : 2 * c);
+  const uint32_t e_at = stage + P::kKe + r;
+  // V: channels warp * D/4 + r * D/32 ...; rows 2c, 2c + 1, 2c + 8, 2c + 9 of every granule
+  uint32_t v_at[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    v_at[x] = ring + P::kVc + v_swizzle<D>((2 * c + (x & 1) + 8 * (x >> 1)) * (D / 2) + warp * (D / 8) + r * (D / 64));
+  const uint32_t vs_at = ring + P::kVs + ((warp * (D / 4) + r * kRun) / 16) * 16 + 2 * c;
+
+  int pos = mine.first, b = mine.b, offset = mine.offset;
+  while (pos < mine.last) {
+    const Sequence seq = sequence<kKeys, P::kRows>(a, b, false);
+    const int kvh = offset / seq.per_head;
+    const int in_head = offset - kvh * seq.per_head;
+    // live tiles have seq.pieces pieces each, the others one
+    const bool dead = in_head >= seq.live * seq.pieces;
+    const int tile = dead ? seq.live + in_head - seq.live * seq.pieces : in_head / seq.pieces;
+    const int pieces = dead ? 1 : seq.pieces;
+    const int piece0 = dead ? 0 : in_head - tile * seq.pieces, piece1 = min(pieces, piece0 + mine.last - pos);
+    const int row0 = tile * P::kRows, len = seq.len, grains = (len + 15) / 16;
+    const int last_cached = dead ? piece0 : min(piece1, seq.cached);
+    const uint8_t* head_pool = a.pool + kvh * a.head_bytes + 16 * lane;
+    const int32_t* table = a.table + b * a.table_stride;
+    int id = 0;  // page of the warp's granule of the tile that is loaded next
+    auto look = [&](int p) {
+      const int g = 4 * p + warp;
+      if (g < grains) id = __ldg(table + (g >> grain_shift));
+    };
+    // copies the warp's granule of tile p to ring half HALF; how many of its tokens are keys
+    auto load = [&](int p, uint32_t half) -> int {
+      const int g = 4 * p + warp;
+      if (g >= grains) return 0;
+      if ((uint32_t)id >= (uint32_t)a.pages) {
+        if (lane == 0) d3b::record_device_error(a.err, kSiteBadPage);
+        return 0;
+      }
+      const uint8_t* src = head_pool + id * a.page_bytes + (g & in_page) * granule_bytes(D);
+#pragma unroll
+      for (int x = 0; x < kCopies; ++x)
+        if (32 * x + 31 < kUnits || 32 * x + lane < kUnits) cp16(place[x] + half, src + 512 * x);
+      return min(16, len - 16 * g);
+    };
+    int live_now = 0, live_next = 0;
+    if (piece0 < last_cached) {
+      look(piece0);
+      live_now = load(piece0, 0);
+    }
+    cp_commit();
+    if (piece0 + 1 < last_cached) look(piece0 + 1);
+
+    load_queries<D, NT, BF>(a, b, kvh, row0, rows, qs, row_scale);
+    __syncthreads();
+
+    float o[NT][kTiles][4];
+    float m[NT][2], l[NT][2], qf[NT][2];
+    int limit[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n][t][j] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = n * 8 + 2 * c + j;
+        m[n][j] = -INFINITY;
+        l[n][j] = 0.f;
+        qf[n][j] = row_scale[row];
+        limit[n][j] = a.causal ? len - (a.L - 1 - (row0 + row) / a.group) : len;
+      }
+    }
+    const int first_limit = a.causal ? len - (a.L - 1) : len;
+
+    // scores in s, with the V rows' powers added in t, to weights in shared memory; l and m follow
+    auto weigh = [&](float (&s)[NT][4], float (&t)[NT][4], auto between) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float top = max_over_rows(fmaxf(t[n][j], t[n][j + 2]));
+          if (r == 0) maxima[warp * P::kRows + n * 8 + 2 * c + j] = top;
+        }
+      __syncthreads();  // every warp's copies have landed too, and its work on the other half is done
+      between();
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float keep[2];
+        float2 top = make_float2(m[n][0], m[n][1]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 x = *reinterpret_cast<const float2*>(maxima + w * P::kRows + n * 8 + 2 * c);
+          top.x = fmaxf(top.x, x.x);
+          top.y = fmaxf(top.y, x.y);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float new_m = j ? top.y : top.x, base = finite_or_zero(new_m);
+          keep[j] = ex2(m[n][j] - base);
+          m[n][j] = new_m;
+          l[n][j] = l[n][j] * keep[j] + (ex2(s[n][j] - base) + ex2(s[n][j + 2] - base));
+          t[n][j] = ex2(t[n][j] - base);
+          t[n][j + 2] = ex2(t[n][j + 2] - base);
+        }
+        if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
+#pragma unroll
+          for (int x = 0; x < kTiles; ++x)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[n][x][j] *= keep[j & 1];
+        }
+        uint2 w;
+        w.x = transpose8x8(pack_half2(t[n][0], t[n][1]));
+        w.y = transpose8x8(pack_half2(t[n][2], t[n][3]));
+        ws[(warp * NT + n) * 32 + lane] = w;
+      }
+      __syncthreads();
+    };
+
+    for (int p = piece0; p < last_cached; ++p) {
+      const uint32_t half = ((p - piece0) & 1) * (4 * P::kStage);
+      cp_wait<0>();
+      __syncwarp();
+      const int key0 = 64 * p + 16 * warp;
+      float s[NT][4], t[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] = 0.f;
+      if (live_now < 16) {
+        // rows that were never written may have scales that are not numbers: their weights are zero,
+        // their values have to be finite
+        for (int i = lane; i < D / 4; i += 32) {
+          const int keep = live_now - 4 * (i & 3);  // bytes of the word that are of keys
+          const uint32_t at = stage + half + P::kVs + 4 * i;
+          uint32_t v[1];
+          lds_words<1>(at, v);
+          sts32(at, keep <= 0 ? 0u : keep >= 4 ? v[0] : v[0] & ((1u << (8 * keep)) - 1u));
+        }
+      }
+      if (live_now > 0) {
+        uint32_t k0[kKWords], k1[kKWords], s0[kKWords / 2], s1[kKWords / 2];  // keys r and r + 8
+        lds_words<D == 256 ? 4 : kKWords>(k_at + half, k0);
+        lds_words<D == 256 ? 4 : kKWords>(k_at + half + 4 * D, k1);
+        if constexpr (D == 256) {
+          lds_words<4>(k_at + half + 64, k0 + 4);
+          lds_words<4>(k_at + half + 4 * D + 64, k1 + 4);
+        }
+        if constexpr (D == 64) {
+          s0[0] = decode_scales(lds_u8(ks_at + half) * 0x101u);
+          s1[0] = decode_scales(lds_u8(ks_at + half + D / 2) * 0x101u);
+        } else {
+#pragma unroll
+          for (int w = 0; w < kKWords / 4; ++w) {
+            const uint32_t x0 = decode_scales(lds_u16(ks_at + half + 8 * w));
+            const uint32_t x1 = decode_scales(lds_u16(ks_at + half + D / 2 + 8 * w));
+            s0[2 * w] = __byte_perm(x0, 0, 0x1010);
+            s0[2 * w + 1] = __byte_perm(x0, 0, 0x3232);
+            s1[2 * w] = __byte_perm(x1, 0, 0x1010);
+            s1[2 * w + 1] = __byte_perm(x1, 0, 0x3232);
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < kKWords; ++w) {
+          uint32_t d0[4], d1[4];
+          decode8(k0[w], d0);
+          decode8(k1[w], d1);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            d0[j] = hmul2(d0[j], s0[w / 2]);
+            d1[j] = hmul2(d1[j], s1[w / 2]);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint4 qv = qs[(n * kKWords + w) * 32 + lane];
+            mma16816(s[n], d0[0], d1[0], d0[1], d1[1], qv.x, qv.y);
+            mma16816(s[n], d0[2], d1[2], d0[3], d1[3], qv.z, qv.w);
+          }
+        }
+      }
+      // a marked row (255) has codes of zero: its score is 0 * infinity here
+      const float kf0 = __uint_as_float(lds_u8(e_at + half) << 23), kf1 = __uint_as_float(lds_u8(e_at + half + 8) << 23);
+      const float ev0 = exponent(lds_u8(e_at + half + P::kVe - P::kKe));
+      const float ev1 = exponent(lds_u8(e_at + half + P::kVe - P::kKe + 8));
+      const bool edge = live_now < 16 || key0 + 16 > first_limit;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[n][j] *= (j < 2 ? kf0 : kf1) * qf[n][j & 1];
+          t[n][j] = s[n][j] + (j < 2 ? ev0 : ev1);
+        }
+        if (edge) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = r + (j < 2 ? 0 : 8);
+            if (key >= live_now || key0 + key >= limit[n][j & 1]) s[n][j] = t[n][j] = -INFINITY;
+          }
+        }
+      }
+      weigh(s, t, [&] {
+        if (p + 1 < last_cached) {
+          live_next = load(p + 1, 4 * P::kStage - half);
+          if (p + 2 < last_cached) look(p + 2);
+        }
+        cp_commit();
+      });
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t at = half + i * P::kStage;
+        const uint32_t sc01 = decode_scales(lds_u16(vs_at + at)), sc89 = decode_scales(lds_u16(vs_at + at + 8));
+        uint2 wf[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) wf[n] = ws[(i * NT + n) * 32 + lane];
+        auto add = [&](int x, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+          a0 = hmul2(a0, sc01), a1 = hmul2(a1, sc01), a2 = hmul2(a2, sc89), a3 = hmul2(a3, sc89);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816(o[n][x], a0, a1, a2, a3, wf[n].x, wf[n].y);
+        };
+        if constexpr (D == 256) {  // 8 channels a lane: one word of each row
+          uint32_t v[4], x0[4], x1[4], y0[4], y1[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) lds_words<1>(v_at[x] + at, v + x);
+          decode8(low_nibbles(v[0], v[1] << 4), x0);
+          decode8(low_nibbles(v[0] >> 4, v[1]), x1);
+          decode8(low_nibbles(v[2], v[3] << 4), y0);
+          decode8(low_nibbles(v[2] >> 4, v[3]), y1);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) add(x, x0[x], x1[x], y0[x], y1[x]);
+        } else if constexpr (D == 128) {  // 4 channels: two bytes of each row, two rows a word
+          const uint32_t u = lds_u16(v_at[0] + at) | (lds_u16(v_at[2] + at) << 16);
+          const uint32_t w = lds_u16(v_at[1] + at) | (lds_u16(v_at[3] + at) << 16);
+          uint32_t x0[4], x1[4];
+          decode8(low_nibbles(u, w << 4), x0);
+          decode8(low_nibbles(u >> 4, w), x1);
+          add(0, x0[0], x1[0], x0[2], x1[2]);
+          add(1, x0[1], x1[1], x0[3], x1[3]);
+        } else {  // 2 channels: one byte of each row
+          const uint32_t u = lds_u8(v_at[0] + at) | (lds_u8(v_at[2] + at) << 8);
+          const uint32_t w = lds_u8(v_at[1] + at) | (lds_u8(v_at[3] + at) << 8);
+          uint32_t x0[4];
+          decode8((low_nibbles(u, w << 4) & 0xFFFFu) | (low_nibbles(u >> 4, w) << 16), x0);
+          add(0, x0[0], x0[2], x0[1], x0[3]);
+        }
+      }
+      live_now = live_next;
+    }
+    cp_wait<0>();
+
+    // the block's own keys
+    for (int p = dead ? piece1 : max(piece0, seq.cached); p < piece1 && a.k_own; ++p) {
+      const int key0 = 64 * (p - seq.cached) + 16 * warp;  // the warp's 16 keys
+      if (64 * (p - seq.cached) >= seq.own) break;         // a unit without any key has one empty piece
+      const uint16_t* k_base = a.k_own + b * a.sk_b + kvh * a.sk_h;
+      const uint16_t* v_base = a.v_own + b * a.sv_b + kvh * a.sv_h;
+      float s[NT][4], t[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] = 0.f;
+      int up_k[2] = {0, 0}, up_v[2] = {0, 0};  // of keys r and r + 8
+      auto channel = [&](int w) { return D == 256 ? 128 * (w / 4) + 32 * c + 8 * (w % 4) : c * (D / 4) + 8 * w; };
+      auto fetch = [&](const uint16_t* base, int64_t stride, int i, int w) {
+        const int key = key0 + r + 8 * i;
+        return key < seq.own ? __ldg(reinterpret_cast<const uint4*>(base + key * stride + channel(w))) : make_uint4(0, 0, 0, 0);
+      };
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float top_k = 0.f, top_v = 0.f;
+        if constexpr (BF) {
+#pragma unroll
+          for (int w = 0; w < kKWords; ++w) {
+            const uint4 k4 = fetch(k_base, a.sk_l, i, w), v4 = fetch(v_base, a.sv_l, i, w);
+            const uint32_t kw[4] = {k4.x, k4.y, k4.z, k4.w}, vw[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 fk = widen2<BF>(kw[j]), fv = widen2<BF>(vw[j]);
+              top_k = fmaxf(top_k, fmaxf(fabsf(fk.x), fabsf(fk.y)));
+              top_v = fmaxf(top_v, fmaxf(fabsf(fv.x), fabsf(fv.y)));
+            }
+          }
+        }
+        if constexpr (BF) {
+#pragma unroll
+          for (int o_ = 1; o_ < 4; o_ <<= 1) {
+            top_k = fmaxf(top_k, __shfl_xor_sync(0xffffffffu, top_k, o_));
+            top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, o_));
+          }
+          up_k[i] = row_up(top_k);
+          up_v[i] = min(row_up(top_v), 64);  // as for cached rows, so that l's terms stay in range
+          if (c == 0) own_scale[16 * warp + r + 8 * i] = power_of(up_v[i]);
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < kKWords; ++w) {
+        uint32_t d[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint4 k4 = fetch(k_base, a.sk_l, i, w);
+          const uint32_t kw[4] = {k4.x, k4.y, k4.z, k4.w};
+          const float by = power_of(up_k[i]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (BF) {
+              const float2 f = widen2<BF>(kw[j]);
+              d[i][j] = pack_half2(f.x * by, f.y * by);
+            } else {
+              d[i][j] = kw[j];
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint4 qv = qs[(n * kKWords + w) * 32 + lane];
+          mma16816(s[n], d[0][0], d[1][0], d[0][1], d[1][1], qv.x, qv.y);
+          mma16816(s[n], d[0][2], d[1][2], d[0][3], d[1][3], qv.z, qv.w);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = j < 2 ? 0 : 1;
+          s[n][j] *= power_of(-up_k[i]) * qf[n][j & 1];
+          t[n][j] = s[n][j] - (float)up_v[i];
+          if (key0 + r + 8 * i >= seq.own) s[n][j] = t[n][j] = -INFINITY;
+        }
+      weigh(s, t, [] {});
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint2 wf[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) wf[n] = ws[(i * NT + n) * 32 + lane];
+        uint32_t h[4][kRun / 2];  // channels of keys 2c, 2c + 1, 2c + 8, 2c + 9, as fp16
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int in_tile = 16 * i + 2 * c + (x & 1) + 8 * (x >> 1), key = 64 * (p - seq.cached) + in_tile;
+          const uint32_t* src = reinterpret_cast<const uint32_t*>(v_base + key * a.sv_l + warp * (D / 4) + r * kRun);
+#pragma unroll
+          for (int j = 0; j < kRun / 2; ++j) {
+            const uint32_t w = key < seq.own ? __ldg(src + j) : 0u;
+            if constexpr (BF) {
+              const float2 f = widen2<BF>(w);
+              h[x][j] = pack_half2(f.x * own_scale[in_tile], f.y * own_scale[in_tile]);
+            } else {
+              h[x][j] = w;
+            }
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < kTiles; ++x) {
+          const uint32_t a0 = __byte_perm(h[0][x], h[1][x], 0x5410), a1 = __byte_perm(h[0][x], h[1][x], 0x7632);
+          const uint32_t a2 = __byte_perm(h[2][x], h[3][x], 0x5410), a3 = __byte_perm(h[2][x], h[3][x], 0x7632);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816(o[n][x], a0, a1, a2, a3, wf[n].x, wf[n].y);
+        }
+      }
+      __syncthreads();  // own_scale and the weights are free again
+    }
+
+    // the rows' sums over the warps; O goes out from where it is
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float sum = l[n][j];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        l[n][j] = sum;
+      }
+    __syncthreads();  // the last maxima have been read
+    if (r == 0) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) maxima[warp * P::kRows + n * 8 + 2 * c + j] = l[n][j];
+    }
+    __syncthreads();
+    const bool whole = piece0 == 0 && piece1 == pieces;
+    const int64_t part = 2 * (int64_t)blockIdx.x + (piece0 == 0);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = n * 8 + 2 * c + j;
+        if (row0 + row >= rows) continue;
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) sum += maxima[w * P::kRows + row];
+        const int d = warp * (D / 4) + r * kRun;
+        if (whole) {
+          const int li = (row0 + row) / a.group, h = kvh * a.group + (row0 + row) % a.group;
+          const bool real = sum != 0.f && li < seq.tokens;
+          const float f = real ? 1.f / sum : 0.f;
+          uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + b * a.so_b + h * a.so_h + li * a.so_l + d);
+#pragma unroll
+          for (int x = 0; x < kTiles; ++x)
+            dst[x] = real ? narrow<BF>(o[n][x][j] * f) | ((uint32_t)narrow<BF>(o[n][x][j + 2] * f) << 16) : 0u;
+        } else {
+          float2* dst = reinterpret_cast<float2*>(a.part_o + (part * P::kRows + row) * D + d);
+#pragma unroll
+          for (int x = 0; x < kTiles; ++x) dst[x] = make_float2(o[n][x][j], o[n][x][j + 2]);
+          if (warp == 0 && r == 0)
+            *reinterpret_cast<float2*>(a.part_st + (part * P::kRows + row) * 2) = make_float2(m[n][j], sum);
+        }
+      }
+    if (piece0 == 0 && threadIdx.x == 0)
+      a.ranges[((int64_t)b * a.kv_heads + kvh) * a.row_tiles + tile] =
+          make_int2(pos / mine.share, (pos + pieces - 1) / mine.share);
+    __syncthreads();  // ring, queries and sums are free again
+    pos += piece1 - piece0;
+    offset += piece1 - piece0;
+    if (offset == seq.total) {
+      offset = 0;
+      ++b;
+    }
+  }
+}
+
+template <int D, int NT, bool BF>
+int launch(const AttnArgs& a, int ctas, cudaStream_t s) {
+  constexpr int smem = Wide<D, NT>::kSmem;
+  static bool ready[64];
+  if (int rc = allow_smem(wide_kernel<D, NT, BF>, smem, ready)) return rc;
+  wide_kernel<D, NT, BF><<<(unsigned)ctas, kThreads, smem, s>>>(a);
+  return d3b_host::check_launch();
+}
+
+template <int D>
+int pick(const AttnArgs& a, int nt, bool bf, int ctas, cudaStream_t s) {
+  if (nt == 2) return bf ? launch<D, 2, true>(a, ctas, s) : launch<D, 2, false>(a, ctas, s);
+  return bf ? launch<D, 4, true>(a, ctas, s) : launch<D, 4, false>(a, ctas, s);
+}
+
+}  // namespace
+
+int launch_wide(const AttnArgs& a, int D, int nt, bool bf, int ctas, cudaStream_t s) {
+  return D == 64 ? pick<64>(a, nt, bf, ctas, s) : D == 128 ? pick<128>(a, nt, bf, ctas, s) : pick<256>(a, nt, bf, ctas, s);
+}
+
+int resident_wide(int, int) { return Wide<128, 4>::kResident; }
+
+}  // namespace d3b_kv4

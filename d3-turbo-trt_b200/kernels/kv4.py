@@ -298,11 +298,30 @@ def question_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torc
         _check_out(out, q)
     if rows == 0 or width == 0:
         return out
-    with _lib.on_device(cache.device):
-        lens = block_offsets(lengths, q.device)
-        k, v = cache.read(layer, table, state_len, dtype=q.dtype)
-        k_q, v_q = _lib.rows16(k_q), _lib.rows16(v_q)
-        if k_q.stride() != v_q.stride():
-            k_q, v_q = (x.clone(memory_format=torch.contiguous_format) for x in (k_q, v_q))
-        _prefix_bidir(_lib.rows16(q), k, v, k_q, v_q, lens, scale, out)
+    device = cache.device
+    with _lib.on_device(device):
+        lens = block_offsets(lengths, device)
+        q, k_q, v_q = _lib.rows16(q), _lib.rows16(k_q), _lib.rows16(v_q)
+        if _reads_codes(rows, heads, cache.kv_heads, width, state_len, dim):
+            lib, table = _lib.lib(), table.contiguous()
+            need = lib.d3b_kv4_question_workspace_size(cache._ref, rows, heads, width, state_len)
+            work = cache.pool.new_empty(need)
+            status = lib.d3b_kv4_question(
+                cache._ref, layer, q.data_ptr(), _lib.strides(q.stride(), 3), table.data_ptr(), table.shape[0], state_len,
+                k_q.data_ptr(), _lib.strides(k_q.stride(), 3), v_q.data_ptr(), _lib.strides(v_q.stride(), 3), lens.data_ptr(),
+                rows, heads, width, _TYPES[q.dtype], scale, out.data_ptr(), _lib.strides(out.stride(), 3), work.data_ptr(),
+                need, _lib.raw_stream(device.index))
+            if status:
+                _lib.check(status, "d3b_kv4_question")
+        else:
+            k, v = cache.read(layer, table, state_len, dtype=q.dtype)
+            if k_q.stride() != v_q.stride():
+                k_q, v_q = (x.clone(memory_format=torch.contiguous_format) for x in (k_q, v_q))
+            _prefix_bidir(q, k, v, k_q, v_q, lens, scale, out)
     return out
+
+
+def _reads_codes(rows: int, heads: int, kv_heads: int, width: int, state_len: int, dim: int) -> bool:
+    """Whether a question batch is small enough to read the state's codes in place."""
+    return _ROUTE
+_ROUTE = True

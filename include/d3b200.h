@@ -475,19 +475,37 @@ D3B_API int d3b_kv4_move_pages(const d3b_kv4_cache* cache, const int32_t* src, c
  *   its sequence and sees itself and what stands before it. Rows with no key are zero.
  *   q, out [B, H, L, D] dtype f16 or bf16, strides {b, h, l} in elements (multiples of 8; rows
  *     16-byte aligned); kv head of head h: h / (H / kv_heads)
- *   table [B, width] int32, row stride table_stride; lengths [B] int32, both on the device.
- *     Entries behind a sequence's last page are not read. A page number outside the pool leaves
- *     its tokens out; a length outside [0, width * page_tokens] is clamped.
+ *   table [B, width] int32, row stride table_stride (0: one table for all); lengths [B] int32,
+ *     both on the device. Entries behind a sequence's last page are not read. A page number
+ *     outside the pool leaves its tokens out; a length outside [0, width * page_tokens] is
+ *     clamped.
  *   workspace: d3b_kv4_decode_workspace_size() bytes, 16-byte aligned (need not be zeroed;
- *     launches that may overlap need one each). NULL where that is 0.
+ *     launches that may overlap need one each)
  * Q, K and V enter the products exactly, in fp16 (queries under a power of two a row); softmax
- * weights are rounded to fp16; sums are fp32.
+ * weights are rounded to fp16; sums are fp32. Results do not change from call to call.
  */
 D3B_API size_t d3b_kv4_decode_workspace_size(const d3b_kv4_cache* cache, int B, int H, int L, int64_t width);
 D3B_API int d3b_kv4_decode(const d3b_kv4_cache* cache, int64_t layer, const void* q, const int64_t* q_strides,
                            const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lengths, int B,
                            int H, int L, int causal, int dtype, float scale, void* out, const int64_t* out_strides,
                            void* workspace, size_t workspace_bytes, d3b_stream_t stream);
+
+/*
+ * Question attention over a state in the cache: d3b_prefix_bidir whose state keys are the first
+ * state_len tokens of one sequence's pages, read as they are (for question batches too small to
+ * pay for widening the state; larger ones read it with d3b_kv4_read and call d3b_prefix_bidir).
+ *   table [width] int32 on the device, width * page_tokens >= state_len
+ *   k_q, v_q [B, kv_heads, L, D], strides {b, h, l}, 16-bit like q; lengths [B] int32 on the
+ *     device; an entry outside [0, L] is clamped (device error word 2010). Tokens i >= lengths[b]
+ *     get zero rows.
+ * Own keys enter as the cached ones do: rows under a power of two, in fp16.
+ */
+D3B_API size_t d3b_kv4_question_workspace_size(const d3b_kv4_cache* cache, int B, int H, int L, int64_t state_len);
+D3B_API int d3b_kv4_question(const d3b_kv4_cache* cache, int64_t layer, const void* q, const int64_t* q_strides,
+                             const int32_t* table, int64_t width, int64_t state_len, const void* k_q,
+                             const int64_t* k_strides, const void* v_q, const int64_t* v_strides,
+                             const int32_t* lengths, int B, int H, int L, int dtype, float scale, void* out,
+                             const int64_t* out_strides, void* workspace, size_t workspace_bytes, d3b_stream_t stream);
 
 /*
  * Per-head RMSNorm of queries and keys, then a rotary embedding whose frequencies take their
