@@ -15,7 +15,9 @@
 //   s_j in base 2, t_j = s_j + e_j, m = max t:
 //   O = sum_j 2^(t_j - m) (code * scale)_j,  l = sum_j 2^(s_j - m),  out = O / l
 //
-// Weights 2^(t - m) stay at most 1 and keep fp16's 11 bits whatever the rows' powers are. The terms
+// m follows the maximum only when it has to: while no t passes m by more than kRoom, weights up to
+// 2^kRoom are as exact as others (fp16 holds 2^15), and nothing is reduced over keys, rescaled or,
+// where warps share rows, exchanged. Whatever the rows' powers are, weights keep fp16's 11 bits. The terms
 // of l are fp32 numbers up to 2^64 (e >= -64); with V values beyond 2^100 the least of them fall
 // below fp32's range, keys whose weight is under 2^-9 of the largest at the very end of bf16.
 // The weights change from accumulator to operand layout by movmatrix.
@@ -32,6 +34,7 @@ namespace d3b_kv4 {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
+constexpr float kRoom = 12.f;
 constexpr int kSiteOwnLength = 2010;  // a question block's length outside [0, L]
 
 struct AttnArgs {
@@ -239,7 +242,25 @@ struct Deal {
 // Sums the sequences' pieces and finds the CTA's share; all threads, `box` in shared memory.
 template <int KEYS, int ROWS>
 __device__ __forceinline__ Deal deal(const AttnArgs& a, int at_least, int* box) {
-  const int per = (a.B + kThreads - 1) / kThreads, t = threadIdx.x, warp = t / 32, lane = t % 32;
+  const int t = threadIdx.x, warp = t / 32, lane = t % 32;
+  if (a.B <= 32) {  // a lane a sequence, every warp for itself: no barrier
+    const int mine = lane < a.B ? sequence<KEYS, ROWS>(a, lane, t < 32 && blockIdx.x == 0).total : 0;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const int total = __shfl_sync(0xffffffffu, upto, 31);
+    Deal d;
+    d.share = max(at_least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    d.first = (int)min((int64_t)blockIdx.x * d.share, (int64_t)total);
+    d.last = min(d.first + d.share, total);
+    d.b = min(__popc(__ballot_sync(0xffffffffu, upto <= d.first)), 31);
+    d.offset = d.first - __shfl_sync(0xffffffffu, upto - mine, d.b);
+    return d;
+  }
+  const int per = (a.B + kThreads - 1) / kThreads;
   const int b0 = min(t * per, a.B), b1 = min(b0 + per, a.B);
   int mine = 0;
   for (int b = b0; b < b1; ++b) mine += sequence<KEYS, ROWS>(a, b, blockIdx.x == 0).total;
@@ -278,36 +299,49 @@ __device__ __forceinline__ Deal deal(const AttnArgs& a, int at_least, int* box) 
   return d;
 }
 
-// Queries to shared memory in operand order, as fp16 under a power of two a row:
-// [nt][word][lane] x 16 bytes, lane = 4 * row + quarter; row_scale = scale * log2(e) * 2^power.
+// Queries to shared memory in operand order, as fp16 under one power of two for the tile's rows:
+// [nt][word][lane] x 16 bytes, lane = 4 * row + quarter. Returns scale * log2(e) * 2^power. The largest
+// magnitude goes to 2^14 or above; what is 2^-29 of it or less loses bits, scores by 2^-40 of the
+// largest row's. All threads, with a barrier; `box` kWarps floats.
 template <int D, int NT, bool BF>
-__device__ __forceinline__ void load_queries(const AttnArgs& a, int b, int kvh, int row0, int rows, uint4* qs,
-                                             float* row_scale) {
+__device__ __forceinline__ float load_queries(const AttnArgs& a, int b, int kvh, int row0, int rows, uint4* qs, float* box) {
   constexpr int kLanes = D / 8;  // a lane takes 8 channels
   constexpr int kWords = D / 32;
-  for (int i = threadIdx.x; i < 8 * NT * kLanes; i += kThreads) {
-    const int row = i / kLanes, sub = i % kLanes;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (row0 + row < rows) {
+  constexpr int kItems = (8 * NT * kLanes + kThreads - 1) / kThreads;
+  uint4 raw[kItems];
+  float top = 0.f;
+#pragma unroll
+  for (int x = 0; x < kItems; ++x) {
+    const int i = x * kThreads + threadIdx.x, row = i / kLanes, sub = i % kLanes;
+    raw[x] = make_uint4(0, 0, 0, 0);
+    if (row < 8 * NT && row0 + row < rows) {
       const int l = (row0 + row) / a.group, g = (row0 + row) % a.group;
-      raw = __ldg(reinterpret_cast<const uint4*>(a.q + b * a.sq_b + (int64_t)(kvh * a.group + g) * a.sq_h + l * a.sq_l) + sub);
+      raw[x] = __ldg(reinterpret_cast<const uint4*>(a.q + b * a.sq_b + (int64_t)(kvh * a.group + g) * a.sq_h + l * a.sq_l) + sub);
     }
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    float2 f[4];
-    float top = 0.f;
+    const uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      f[j] = widen2<BF>(w[j]);
-      top = fmaxf(top, fmaxf(fabsf(f[j].x), fabsf(f[j].y)));
+      const float2 f = widen2<BF>(w[j]);
+      top = fabsf(f.x) < INFINITY ? fmaxf(top, fabsf(f.x)) : top;
+      top = fabsf(f.y) < INFINITY ? fmaxf(top, fabsf(f.y)) : top;
     }
+  }
+  const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));  // not negative: ordered as bits
+  if (threadIdx.x % 32 == 0) box[threadIdx.x / 32] = __uint_as_float(most);
+  __syncthreads();
+  top = fmaxf(fmaxf(box[0], box[1]), fmaxf(box[2], box[3]));
+  const int up = row_up(top);
+  const float by = power_of(up);
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const int up = row_up(top);
-    const float by = power_of(up);
+  for (int x = 0; x < kItems; ++x) {
+    const int i = x * kThreads + threadIdx.x, row = i / kLanes, sub = i % kLanes;
+    if (row >= 8 * NT) continue;
+    const uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
     uint32_t h[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const __half2 v = __floats2half2_rn(f[j].x * by, f[j].y * by);
+      const float2 f = widen2<BF>(w[j]);
+      const __half2 v = __floats2half2_rn(f.x * by, f.y * by);
       h[j] = *reinterpret_cast<const uint32_t*>(&v);
     }
     // channels 8 sub ...: which word of which quarter they are (see the K loads)
@@ -315,8 +349,8 @@ __device__ __forceinline__ void load_queries(const AttnArgs& a, int b, int kvh, 
     const int per = D == 256 ? 4 : kWords;
     const int quarter = in / per, word = half * 4 + in % per;
     qs[((row / 8) * kWords + word) * 32 + (row % 8) * 4 + quarter] = make_uint4(h[0], h[1], h[2], h[3]);
-    if (sub == 0) row_scale[row] = a.scale_log2 * power_of(-up);
   }
+  return a.scale_log2 * power_of(-up);
 }
 
 // lets `kernel` have `bytes` of dynamic shared memory, once a device (`ready` by device; twice is harmless)

@@ -8,39 +8,63 @@ using namespace d3b_kv4;
 
 constexpr int kMergeThreads = 256;
 
-// One CTA a query row: the parts of its unit, added in a fixed order (a group of D/4 threads takes
-// every kGroups-th part, then the groups in turn). Launched before the attention kernel has
-// finished; it waits for it here.
+// One CTA a query row: the parts of its unit, added in a fixed order. The parts' factors are worked
+// out first, a thread a part; then groups of D/4 threads add every kGroups-th part, then the groups in
+// turn. Launched before the attention kernel has finished; it waits for it here.
 template <int D, bool BF>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ AttnArgs a, int tile_rows) {
   constexpr int kGroups = kMergeThreads / (D / 4);
   __shared__ float4 part[kGroups][D / 4];
-  __shared__ float sums[kGroups];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ float factor[kMergeThreads], tops[kMergeThreads / 32], sums[kMergeThreads / 32];
   const int rows = a.group * a.L;
   const int row = blockIdx.x % rows, bk = blockIdx.x / rows;
   const int kvh = bk % a.kv_heads, b = bk / a.kv_heads;
+  const int t = threadIdx.x, d4 = t % (D / 4), group = t / (D / 4);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int2 range = a.ranges[(int64_t)bk * a.row_tiles + row / tile_rows];
   if (range.x == range.y) return;  // finished where it was computed
-  const int d4 = threadIdx.x % (D / 4), group = threadIdx.x / (D / 4);
   // the unit's first CTA began it (slot 1), the others went on with it (slot 0)
   auto at = [&](int cta) { return (2 * (int64_t)cta + (cta == range.x)) * tile_rows + row % tile_rows; };
   float top = -INFINITY;
-#pragma unroll 8
-  for (int c = range.x; c <= range.y; ++c) top = fmaxf(top, a.part_st[at(c) * 2]);
+  for (int c = range.x + t; c <= range.y; c += kMergeThreads) top = fmaxf(top, a.part_st[at(c) * 2]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (t % 32 == 0) tops[t / 32] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kMergeThreads / 32; ++w) top = fmaxf(top, tops[w]);
   const float base = finite_or_zero(top);
   float sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c0 = range.x; c0 <= range.y; c0 += kMergeThreads) {
+    const int n = min(kMergeThreads, range.y + 1 - c0);
+    __syncthreads();
+    if (t < n) {
+      const float2 st = *reinterpret_cast<const float2*>(a.part_st + at(c0 + t) * 2);
+      const float f = ex2(st.x - base);
+      factor[t] = f;
+      sum = fmaf(st.y, f, sum);
+    }
+    __syncthreads();
 #pragma unroll 8
-  for (int c = range.x + group; c <= range.y; c += kGroups) {
-    const int64_t i = at(c);
-    add_part(acc, sum, *reinterpret_cast<const float4*>(a.part_o + i * D + 4 * d4),
-             *reinterpret_cast<const float2*>(a.part_st + i * 2), base);
+    for (int i = group; i < n; i += kGroups) {
+      const float4 x = *reinterpret_cast<const float4*>(a.part_o + at(c0 + i) * D + 4 * d4);
+      const float f = factor[i];
+      acc.x = fmaf(x.x, f, acc.x);
+      acc.y = fmaf(x.y, f, acc.y);
+      acc.z = fmaf(x.z, f, acc.z);
+      acc.w = fmaf(x.w, f, acc.w);
+    }
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (t % 32 == 0) sums[t / 32] = sum;
   part[group][d4] = acc;
-  if (d4 == 0) sums[group] = sum;
   __syncthreads();
   if (group) return;
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kMergeThreads / 32; ++w) sum += sums[w];
 #pragma unroll
   for (int g = 1; g < kGroups; ++g) {
     const float4 x = part[g][d4];
@@ -48,7 +72,6 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
     acc.y += x.y;
     acc.z += x.z;
     acc.w += x.w;
-    sum += sums[g];
   }
   int tokens = a.L;
   if (a.own_lengths) tokens = min(max(__ldg(a.own_lengths + b), 0), a.L);

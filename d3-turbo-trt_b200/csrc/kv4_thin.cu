@@ -22,7 +22,7 @@ struct Thin {
   static constexpr int kRing = kWarps * 2 * 2 * kStage;                             // two pairs of granules a warp
   static constexpr int kMerge = kWarps * kRows * (D + 2) * 4;
   static constexpr int kQ = kRows * D * 2;
-  static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kQ + kRows * 4;
+  static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kQ;
   // where a granule's parts sit in a ring stage
   static constexpr int kKc = 0, kVc = 8 * D, kKs = 16 * D, kVs = 17 * D, kKe = 18 * D, kVe = 18 * D + 16;
 };
@@ -33,8 +33,8 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
   constexpr int kKWords = D / 32, kVWords = D / 64, kTiles = D / 16;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int box[kWarps + 2];
+  __shared__ float tops[kWarps];
   uint4* qs = reinterpret_cast<uint4*>(smem + (P::kRing > P::kMerge ? P::kRing : P::kMerge));
-  float* row_scale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(qs) + P::kQ);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
   const int rows = a.group * a.L;
   const Deal mine = deal<kKeys, P::kRows>(a, kLeast, box);
@@ -105,11 +105,11 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
     cp_commit();
     if (pairs > 1) look(1);
 
-    load_queries<D, NT, BF>(a, b, kvh, row0, rows, qs, row_scale);
+    const float q_scale = load_queries<D, NT, BF>(a, b, kvh, row0, rows, qs, tops);
     __syncthreads();
 
     float o[NT][kTiles][4];
-    float m[NT][2], l[NT][2], qf[NT][2];
+    float m[NT][2], l[NT][2];
     int limit[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -122,7 +122,6 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
         const int row = n * 8 + 2 * c + j;
         m[n][j] = -INFINITY;
         l[n][j] = 0.f;
-        qf[n][j] = row_scale[row];
         limit[n][j] = a.causal ? len - (a.L - 1 - (row0 + row) / a.group) : len;
       }
     }
@@ -157,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
 
       const int key0 = 16 * (my_first + pair * 2 * kWarps);
       const bool edge = key0 + 32 > first_limit || bad_now;  // some key is masked for some row
-      float s[2][NT][4], t[2][NT][4];
+      float s[2][NT][4], kq[2][2], ev[2][2];  // of keys r and r + 8 of both granules: factor of the score, V's power
       int live[2] = {16, 16};  // tokens of the granule that are keys at all
       if (edge) {
 #pragma unroll
@@ -211,57 +210,73 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
           }
         }
         // a marked row (255) has codes of zero: its score is 0 * infinity here
-        const float kf0 = __uint_as_float(lds_u8(e_at + at) << 23), kf1 = __uint_as_float(lds_u8(e_at + at + 8) << 23);
-        const float ev0 = exponent(lds_u8(e_at + at + P::kVe - P::kKe)), ev1 = exponent(lds_u8(e_at + at + P::kVe - P::kKe + 8));
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            s[i][n][j] *= (j < 2 ? kf0 : kf1) * qf[n][j & 1];
-            t[i][n][j] = s[i][n][j] + (j < 2 ? ev0 : ev1);
-          }
-          if (edge) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int key = r + (j < 2 ? 0 : 8);
-              if (key >= live[i] || key0 + 16 * i + key >= limit[n][j & 1]) s[i][n][j] = t[i][n][j] = -INFINITY;
-            }
-          }
-        }
+        kq[i][0] = __uint_as_float(lds_u8(e_at + at) << 23) * q_scale;
+        kq[i][1] = __uint_as_float(lds_u8(e_at + at + 8) << 23) * q_scale;
+        ev[i][0] = exponent(lds_u8(e_at + at + P::kVe - P::kKe));
+        ev[i][1] = exponent(lds_u8(e_at + at + P::kVe - P::kKe + 8));
       }
 
-      uint32_t wf[2][NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float keep[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float top = max_over_rows(fmaxf(fmaxf(t[0][n][j], t[0][n][j + 2]), fmaxf(t[1][n][j], t[1][n][j + 2])));
-          const float new_m = fmaxf(m[n][j], top), base = finite_or_zero(new_m);
-          keep[j] = ex2(m[n][j] - base);
-          m[n][j] = new_m;
-          l[n][j] *= keep[j];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            l[n][j] += ex2(s[i][n][j] - base) + ex2(s[i][n][j + 2] - base);
-            t[i][n][j] = ex2(t[i][n][j] - base);
-            t[i][n][j + 2] = ex2(t[i][n][j + 2] - base);
-          }
-        }
-        if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
-#pragma unroll
-          for (int x = 0; x < kTiles; ++x)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[n][x][j] *= keep[j & 1];
-        }
+      // exponents of l's terms and of the weights, masked keys at -infinity
+      float x[2][NT][4], y[2][NT][4];
+      auto exponents = [&] {
+        float most = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              x[i][n][j] = fmaf(s[i][n][j], kq[i][j >> 1], -m[n][j & 1]);
+              y[i][n][j] = x[i][n][j] + ev[i][j >> 1];
+              if (edge) {
+                const int key = r + 8 * (j >> 1);
+                if (key >= live[i] || key0 + 16 * i + key >= limit[n][j & 1]) x[i][n][j] = y[i][n][j] = -INFINITY;
+              }
+              most = fmaxf(most, y[i][n][j]);
+            }
+        return most;
+      };
+      // m = -infinity (no key yet) makes every exponent +infinity
+      if (__any_sync(0xffffffffu, exponents() > kRoom)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const __half2 h = __floats2half2_rn(t[i][n][2 * j], t[i][n][2 * j + 1]);
+            const float old = m[n][j];
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int key = r + 8 * h;
+                const bool in = !edge || (key < live[i] && key0 + 16 * i + key < limit[n][j]);
+                if (in) top = fmaxf(top, fmaf(s[i][n][j + 2 * h], kq[i][h], ev[i][h]));
+              }
+            const float now = fmaxf(old, max_over_rows(top));
+            const float keep = ex2(old - finite_or_zero(now));
+            m[n][j] = now;
+            l[n][j] *= keep;
+#pragma unroll
+            for (int z = 0; z < kTiles; ++z) {
+              o[n][z][j] *= keep;
+              o[n][z][j + 2] *= keep;
+            }
+          }
+        exponents();
+      }
+      uint32_t wf[2][NT][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) l[n][j] += ex2(x[i][n][j]) + ex2(x[i][n][j + 2]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const __half2 h = __floats2half2_rn(ex2(y[i][n][2 * j]), ex2(y[i][n][2 * j + 1]));
             wf[i][n][j] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h));
           }
-      }
+        }
 
 #pragma unroll
       for (int i = 0; i < 2; ++i) {

@@ -28,7 +28,7 @@ struct Wide {
   static constexpr int kQ = kRows * D * 2;
   static constexpr int kW = 4 * NT * 32 * 8;    // weights: [granule][nt][lane] x 8 bytes
   static constexpr int kMax = kWarps * kRows * 4;
-  static constexpr int kSmem = kRing + kQ + kW + kMax + kRows * 4 + kKeys * 4;
+  static constexpr int kSmem = kRing + kQ + kW + kMax + kKeys * 4;
   static constexpr int kKc = 0, kVc = 8 * D, kKs = 16 * D, kVs = 17 * D, kKe = 18 * D, kVe = 18 * D + 16;
 };
 
@@ -47,11 +47,11 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
   constexpr int kRun = D / 32;                      // channels of V a lane has
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int box[kWarps + 2];
+  __shared__ float tops[kWarps];
   uint4* qs = reinterpret_cast<uint4*>(smem + P::kRing);
   uint2* ws = reinterpret_cast<uint2*>(smem + P::kRing + P::kQ);
   float* maxima = reinterpret_cast<float*>(smem + P::kRing + P::kQ + P::kW);  // [warp][row]
-  float* row_scale = maxima + kWarps * P::kRows;
-  float* own_scale = row_scale + P::kRows;  // [key]: what an own V row is multiplied by
+  float* own_scale = maxima + kWarps * P::kRows;  // [key]: what an own V row is multiplied by
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
   const int rows = a.group * a.L;
   const Deal mine = deal<kKeys, P::kRows>(a, 1, box);
@@ -126,11 +126,11 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
     cp_commit();
     if (piece0 + 1 < last_cached) look(piece0 + 1);
 
-    load_queries<D, NT, BF>(a, b, kvh, row0, rows, qs, row_scale);
+    const float q_scale = load_queries<D, NT, BF>(a, b, kvh, row0, rows, qs, tops);
     __syncthreads();
 
     float o[NT][kTiles][4];
-    float m[NT][2], l[NT][2], qf[NT][2];
+    float m[NT][2], l[NT][2];
     int limit[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -143,51 +143,76 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
         const int row = n * 8 + 2 * c + j;
         m[n][j] = -INFINITY;
         l[n][j] = 0.f;
-        qf[n][j] = row_scale[row];
         limit[n][j] = a.causal ? len - (a.L - 1 - (row0 + row) / a.group) : len;
       }
     }
     const int first_limit = a.causal ? len - (a.L - 1) : len;
 
-    // scores in s, with the V rows' powers added in t, to weights in shared memory; l and m follow
-    auto weigh = [&](float (&s)[NT][4], float (&t)[NT][4], auto between) {
+    // Products in s, of keys r and r + 8 of the warp's 16, to weights in shared memory; l and m follow.
+    // kq: factors of the scores; ev: powers of the V rows; masked(j, n): key r + 8 * (j >> 1) is none for
+    // row n * 8 + 2 * c + (j & 1). `between` runs behind the first barrier.
+    auto weigh = [&](const float (&s)[NT][4], const float (&kq)[2], const float (&ev)[2], bool edge, auto masked, auto between) {
+      float x[NT][4], y[NT][4];  // exponents of l's terms and of the weights
+      auto exponents = [&] {
+        float most = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float top = max_over_rows(fmaxf(t[n][j], t[n][j + 2]));
-          if (r == 0) maxima[warp * P::kRows + n * 8 + 2 * c + j] = top;
-        }
-      __syncthreads();  // every warp's copies have landed too, and its work on the other half is done
+          for (int j = 0; j < 4; ++j) {
+            x[n][j] = fmaf(s[n][j], kq[j >> 1], -m[n][j & 1]);
+            y[n][j] = x[n][j] + ev[j >> 1];
+            if (edge && masked(n, j)) x[n][j] = y[n][j] = -INFINITY;
+            most = fmaxf(most, y[n][j]);
+          }
+        return most;
+      };
+      // m = -infinity (no key yet) makes every exponent +infinity. Behind this barrier every warp's copies have
+      // landed and its work on the other half is done.
+      const bool move = __syncthreads_or(exponents() > kRoom);
       between();
+      if (move) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (!edge || !masked(n, j + 2 * h)) top = fmaxf(top, fmaf(s[n][j + 2 * h], kq[h], ev[h]));
+            top = max_over_rows(top);
+            if (r == 0) maxima[warp * P::kRows + n * 8 + 2 * c + j] = top;
+          }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float2 top = make_float2(m[n][0], m[n][1]);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float2 z = *reinterpret_cast<const float2*>(maxima + w * P::kRows + n * 8 + 2 * c);
+            top.x = fmaxf(top.x, z.x);
+            top.y = fmaxf(top.y, z.y);
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float now = j ? top.y : top.x, keep = ex2(m[n][j] - finite_or_zero(now));
+            m[n][j] = now;
+            l[n][j] *= keep;
+#pragma unroll
+            for (int z = 0; z < kTiles; ++z) {
+              o[n][z][j] *= keep;
+              o[n][z][j + 2] *= keep;
+            }
+          }
+        }
+        exponents();
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float keep[2];
-        float2 top = make_float2(m[n][0], m[n][1]);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float2 x = *reinterpret_cast<const float2*>(maxima + w * P::kRows + n * 8 + 2 * c);
-          top.x = fmaxf(top.x, x.x);
-          top.y = fmaxf(top.y, x.y);
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float new_m = j ? top.y : top.x, base = finite_or_zero(new_m);
-          keep[j] = ex2(m[n][j] - base);
-          m[n][j] = new_m;
-          l[n][j] = l[n][j] * keep[j] + (ex2(s[n][j] - base) + ex2(s[n][j + 2] - base));
-          t[n][j] = ex2(t[n][j] - base);
-          t[n][j + 2] = ex2(t[n][j + 2] - base);
-        }
-        if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
-#pragma unroll
-          for (int x = 0; x < kTiles; ++x)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[n][x][j] *= keep[j & 1];
-        }
+        for (int j = 0; j < 2; ++j) l[n][j] += ex2(x[n][j]) + ex2(x[n][j + 2]);
         uint2 w;
-        w.x = transpose8x8(pack_half2(t[n][0], t[n][1]));
-        w.y = transpose8x8(pack_half2(t[n][2], t[n][3]));
+        w.x = transpose8x8(pack_half2(ex2(y[n][0]), ex2(y[n][1])));
+        w.y = transpose8x8(pack_half2(ex2(y[n][2]), ex2(y[n][3])));
         ws[(warp * NT + n) * 32 + lane] = w;
       }
       __syncthreads();
@@ -198,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
       cp_wait<0>();
       __syncwarp();
       const int key0 = 64 * p + 16 * warp;
-      float s[NT][4], t[NT][4];
+      float s[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -255,26 +280,15 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
         }
       }
       // a marked row (255) has codes of zero: its score is 0 * infinity here
-      const float kf0 = __uint_as_float(lds_u8(e_at + half) << 23), kf1 = __uint_as_float(lds_u8(e_at + half + 8) << 23);
-      const float ev0 = exponent(lds_u8(e_at + half + P::kVe - P::kKe));
-      const float ev1 = exponent(lds_u8(e_at + half + P::kVe - P::kKe + 8));
-      const bool edge = live_now < 16 || key0 + 16 > first_limit;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[n][j] *= (j < 2 ? kf0 : kf1) * qf[n][j & 1];
-          t[n][j] = s[n][j] + (j < 2 ? ev0 : ev1);
-        }
-        if (edge) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int key = r + (j < 2 ? 0 : 8);
-            if (key >= live_now || key0 + key >= limit[n][j & 1]) s[n][j] = t[n][j] = -INFINITY;
-          }
-        }
-      }
-      weigh(s, t, [&] {
+      const float kq[2] = {__uint_as_float(lds_u8(e_at + half) << 23) * q_scale,
+                           __uint_as_float(lds_u8(e_at + half + 8) << 23) * q_scale};
+      const float ev[2] = {exponent(lds_u8(e_at + half + P::kVe - P::kKe)),
+                           exponent(lds_u8(e_at + half + P::kVe - P::kKe + 8))};
+      auto masked = [&](int n, int j) {
+        const int key = r + 8 * (j >> 1);
+        return key >= live_now || key0 + key >= limit[n][j & 1];
+      };
+      weigh(s, kq, ev, live_now < 16 || key0 + 16 > first_limit, masked, [&] {
         if (p + 1 < last_cached) {
           live_next = load(p + 1, 4 * P::kStage - half);
           if (p + 2 < last_cached) look(p + 2);
@@ -329,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
       if (64 * (p - seq.cached) >= seq.own) break;         // a unit without any key has one empty piece
       const uint16_t* k_base = a.k_own + b * a.sk_b + kvh * a.sk_h;
       const uint16_t* v_base = a.v_own + b * a.sv_b + kvh * a.sv_h;
-      float s[NT][4], t[NT][4];
+      float s[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -392,16 +406,9 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
           mma16816(s[n], d[0][2], d[1][2], d[0][3], d[1][3], qv.z, qv.w);
         }
       }
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = j < 2 ? 0 : 1;
-          s[n][j] *= power_of(-up_k[i]) * qf[n][j & 1];
-          t[n][j] = s[n][j] - (float)up_v[i];
-          if (key0 + r + 8 * i >= seq.own) s[n][j] = t[n][j] = -INFINITY;
-        }
-      weigh(s, t, [] {});
+      const float kq[2] = {power_of(-up_k[0]) * q_scale, power_of(-up_k[1]) * q_scale};
+      const float ev[2] = {-(float)up_v[0], -(float)up_v[1]};
+      weigh(s, kq, ev, true, [&](int, int j) { return key0 + r + 8 * (j >> 1) >= seq.own; }, [] {});
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint2 wf[NT];
