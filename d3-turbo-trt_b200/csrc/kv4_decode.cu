@@ -93,7 +93,7 @@ bool make_plan(const d3b_kv4_cache* c, int B, int H, int L, int64_t keys, bool o
   p->nt = rows <= 8 && !p->wide ? 1 : rows <= 16 ? 2 : 4;
   const int64_t tiles = (rows + 8 * p->nt - 1) / (8 * p->nt);
   p->units = (int64_t)B * c->kv_heads * tiles;
-  const int64_t piece = p->wide ? 64 : 32, least = p->wide ? 1 : 4;
+  const int64_t piece = p->wide ? 64 : D == 256 ? 16 : 32, least = p->wide ? 1 : 4;
   // own keys add at most L / 64 pieces, which `keys` holds
   const int64_t most = p->units * (keys / piece + 3);
   if (p->units > (1 << 28) || most > (1 << 30)) return false;

@@ -1,8 +1,8 @@
 // Attention over the 4-bit cache for few query rows a kv head (up to 16): decoding.
 //
-// A warp takes pairs of granules (32 keys) by itself, from its own cp.async ring of two pairs and
-// without barriers, and keeps all of O for its rows; a unit's warps are merged at the end of the
-// CTA's share. One m16n8k16 serves 8 rows, so a group of up to 8 heads costs one product.
+// A warp takes GP granules (32 keys, 16 at D = 256) a step by itself, from its own cp.async ring of
+// three steps and without barriers, and keeps all of O for its rows; a unit's warps are merged at the
+// end of the CTA's share. One m16n8k16 serves 8 rows, so a group of up to 8 heads costs one product.
 //
 // Bound: the cache's bytes, 18 D + 32 for 16 tokens and kv head, with the ALU close behind: a code
 // pair costs a conversion (64 lanes a clock and SM) and a product with its scale.
@@ -11,15 +11,18 @@
 namespace d3b_kv4 {
 namespace {
 
-constexpr int kKeys = 32;
 constexpr int kLeast = kWarps;  // pieces a CTA takes at least: one a warp
+constexpr int kDepth = 3;       // steps in a warp's ring
 
 template <int D, int NT>
 struct Thin {
+  static constexpr int GP = D == 256 ? 1 : 2;                          // granules a step
+  static constexpr int kKeys = 16 * GP;                                // keys of a piece
   static constexpr int kStage = (granule_bytes(D) + 127) / 128 * 128;  // V rows start on 128-byte lines
   static constexpr int kRows = 8 * NT;
-  static constexpr int kResident = NT == 1 ? (D == 64 ? 5 : D == 128 ? 4 : 3) : 2;  // CTAs an SM by registers
-  static constexpr int kRing = kWarps * 2 * 2 * kStage;                             // two pairs of granules a warp
+  static constexpr int kResident = NT == 1 ? (D == 64 ? 5 : 3) : 2;    // CTAs an SM
+  static constexpr int kWarpRing = kDepth * GP * kStage;
+  static constexpr int kRing = kWarps * kWarpRing;
   static constexpr int kMerge = kWarps * kRows * (D + 2) * 4;
   static constexpr int kQ = kRows * D * 2;
   static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kQ;
@@ -37,9 +40,9 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
   uint4* qs = reinterpret_cast<uint4*>(smem + (P::kRing > P::kMerge ? P::kRing : P::kMerge));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
   const int rows = a.group * a.L;
-  const Deal mine = deal<kKeys, P::kRows>(a, kLeast, box);
+  const Deal mine = deal<P::kKeys, P::kRows>(a, kLeast, box);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may take its place; it waits for our end
-  const uint32_t ring = d3b::smem_u32(smem) + warp * (2 * 2 * P::kStage);
+  const uint32_t ring = d3b::smem_u32(smem) + warp * P::kWarpRing;
   const int grain_shift = a.page_shift - 4, in_page = (1 << grain_shift) - 1;
   // a lane copies units lane, lane + 32, ... of 16 bytes of a granule; where each goes in a stage
   constexpr int kUnits = granule_bytes(D) / 16, kCopies = (kUnits + 31) / 32;
@@ -60,50 +63,63 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
 
   int pos = mine.first, b = mine.b, offset = mine.offset;
   while (pos < mine.last) {
-    const Sequence seq = sequence<kKeys, P::kRows>(a, b, false);
+    const Sequence seq = sequence<P::kKeys, P::kRows>(a, b, false);
     const int kvh = offset / seq.per_head, tile = (offset - kvh * seq.per_head) / seq.pieces;  // every tile is live
     const int piece0 = offset - kvh * seq.per_head - tile * seq.pieces, piece1 = min(seq.pieces, piece0 + mine.last - pos);
     const int row0 = tile * P::kRows, len = seq.len, grains = (len + 15) / 16;
-    const int my_first = 2 * (piece0 + warp), g_end = min(2 * piece1, grains);  // pairs my_first, + 2 kWarps, ...
-    const int pairs = my_first < g_end ? (g_end - my_first + 2 * kWarps - 1) / (2 * kWarps) : 0;
+    // the warp's steps: granules my_first + step * kStride ...
+    constexpr int kStride = P::GP * kWarps;
+    const int my_first = P::GP * (piece0 + warp), g_end = min(P::GP * piece1, grains);
+    const int steps = my_first < g_end ? (g_end - my_first + kStride - 1) / kStride : 0;
     const uint8_t* head_pool = a.pool + kvh * a.head_bytes + 16 * lane;
     const int32_t* table = a.table + b * a.table_stride;
-    int ids[2];  // page numbers of the pair that is loaded next
-    auto look = [&](int pair) {
-      const int g = my_first + pair * 2 * kWarps;
+    int ids[P::GP];  // page numbers of the step that is loaded next
+    // two granules of a step start at an even one: they lie in one page unless a page is one granule
+    auto look = [&](int step) {
+      const int g = my_first + step * kStride;
+      if (step >= steps) return;
       ids[0] = __ldg(table + (g >> grain_shift));
-      // pairs start at even granules: both lie in one page unless a page is one granule
-      ids[1] = grain_shift || g + 1 >= g_end ? ids[0] : __ldg(table + g + 1);
+      if constexpr (P::GP == 2) ids[1] = grain_shift || g + 1 >= g_end ? ids[0] : __ldg(table + g + 1);
     };
-    // copies a pair to ring slot SLOT; 0, or one bit for each granule whose page is not in the pool
-    auto load = [&](int pair, auto slot) -> uint32_t {
-      constexpr int kSlot = decltype(slot)::value;
-      const int g = my_first + pair * 2 * kWarps;
+    // copies a step to ring slot SLOT; a bit for each granule whose page is not in the pool
+    auto load = [&](int step, auto slot) -> uint32_t {
+      constexpr int kAt = decltype(slot)::value * P::GP * P::kStage;
+      if (step >= steps) return 0;
+      const int g = my_first + step * kStride;
       uint32_t bad = 0;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if ((uint32_t)ids[i] < (uint32_t)a.pages) {
-          const uint8_t* src = head_pool + ids[i] * a.page_bytes + ((g + i) & in_page) * granule_bytes(D);
-          if (i == 0 || g + 1 < g_end) {
+      for (int i = 0; i < P::GP; ++i) bad |= (uint32_t)ids[i] < (uint32_t)a.pages ? 0u : 1u << i;
+      const uint8_t* src = head_pool + ids[0] * a.page_bytes + (g & in_page) * granule_bytes(D);
+      if (!bad && (P::GP == 1 || grain_shift)) {  // behind a sequence's last granule: the page's next, not used
 #pragma unroll
-            for (int x = 0; x < kCopies; ++x)
-              if (32 * x + 31 < kUnits || 32 * x + lane < kUnits)
-                cp16(place[x] + (2 * kSlot + i) * P::kStage, src + 512 * x);
-          }
-        } else {
-          bad |= 1u << i;
+        for (int i = 0; i < P::GP; ++i)
+#pragma unroll
+          for (int x = 0; x < kCopies; ++x)
+            if (32 * x + 31 < kUnits || 32 * x + lane < kUnits)
+              cp16(place[x] + kAt + i * P::kStage, src + i * granule_bytes(D) + 512 * x);
+        return 0;
+      }
+#pragma unroll 1
+      for (int i = 0; i < P::GP; ++i) {
+        if ((bad >> i) & 1) {
           if (lane == 0) d3b::record_device_error(a.err, kSiteBadPage);
+          continue;
         }
+        src = head_pool + (i ? ids[P::GP - 1] : ids[0]) * a.page_bytes + ((g + i) & in_page) * granule_bytes(D);
+#pragma unroll
+        for (int x = 0; x < kCopies; ++x)
+          if (32 * x + 31 < kUnits || 32 * x + lane < kUnits) cp16(place[x] + kAt + i * P::kStage, src + 512 * x);
       }
       return bad;
     };
-    uint32_t bad_now = 0, bad_next = 0;
-    if (pairs > 0) {
-      look(0);
-      bad_now = load(0, Int<0>{});
-    }
+    uint32_t bad_now = 0, bad_next = 0, bad_after = 0;
+    look(0);
+    bad_now = load(0, Int<0>{});
     cp_commit();
-    if (pairs > 1) look(1);
+    look(1);
+    bad_next = load(1, Int<1>{});
+    cp_commit();
+    look(2);
 
     const float q_scale = load_queries<D, NT, BF>(a, b, kvh, row0, rows, qs, tops);
     __syncthreads();
@@ -125,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
         limit[n][j] = a.causal ? len - (a.L - 1 - (row0 + row) / a.group) : len;
       }
     }
-    constexpr bool kHold = NT * D <= 256;  // queries stay in registers
+    constexpr bool kHold = NT * D <= 128;  // queries stay in registers
     uint4 qr[kHold ? NT : 1][kHold ? kKWords : 1];
     if constexpr (kHold) {
 #pragma unroll
@@ -143,27 +159,24 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
     for (int x = 0; x < 4; ++x)
       v_at[x] = ring + P::kVc + v_swizzle<D>((2 * c + (x & 1) + 8 * (x >> 1)) * (D / 2) + r * (D / 16));
 
-    auto step = [&](int pair, auto slot) {
-      constexpr int kAt = 2 * decltype(slot)::value * P::kStage;
+    auto step = [&](int now, auto slot) {
+      constexpr int kSlot = decltype(slot)::value, kAt = kSlot * P::GP * P::kStage;
       __syncwarp();  // every lane is done with the slot that is loaded next
-      if (pair + 1 < pairs) {
-        bad_next = load(pair + 1, Int<1 - decltype(slot)::value>{});
-        if (pair + 2 < pairs) look(pair + 2);
-      }
+      bad_after = load(now + 2, Int<(kSlot + 2) % kDepth>{});
       cp_commit();
-      cp_wait<1>();
+      look(now + 3);
+      cp_wait<kDepth - 1>();
       __syncwarp();
 
-      const int key0 = 16 * (my_first + pair * 2 * kWarps);
-      const bool edge = key0 + 32 > first_limit || bad_now;  // some key is masked for some row
-      float s[2][NT][4], kq[2][2], ev[2][2];  // of keys r and r + 8 of both granules: factor of the score, V's power
-      int live[2] = {16, 16};  // tokens of the granule that are keys at all
-      if (edge) {
+      const int key0 = 16 * (my_first + now * kStride);
+      const bool edge = key0 + P::kKeys > first_limit || bad_now;  // some key is masked for some row
+      float s[P::GP][NT][4], kq[P::GP][2], ev[P::GP][2];  // of keys r and r + 8: products, factor of the score, V's power
+      int live[P::GP];  // tokens of the granule that are keys at all
 #pragma unroll
-        for (int i = 0; i < 2; ++i) live[i] = (bad_now >> i) & 1 ? 0 : min(16, len - key0 - 16 * i);
-      }
+      for (int i = 0; i < P::GP; ++i)
+        live[i] = edge ? ((bad_now >> i) & 1 ? 0 : min(16, len - key0 - 16 * i)) : 16;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < P::GP; ++i) {
         const int at = kAt + i * P::kStage;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -217,11 +230,11 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
       }
 
       // exponents of l's terms and of the weights, masked keys at -infinity
-      float x[2][NT][4], y[2][NT][4];
+      float x[P::GP][NT][4], y[P::GP][NT][4];
       auto exponents = [&] {
         float most = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < P::GP; ++i)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -245,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
             const float old = m[n][j];
             float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < P::GP; ++i)
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const int key = r + 8 * h;
@@ -264,9 +277,9 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
           }
         exponents();
       }
-      uint32_t wf[2][NT][2];
+      uint32_t wf[P::GP][NT][2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < P::GP; ++i)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -279,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
         }
 
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < P::GP; ++i) {
         const int at = kAt + i * P::kStage;
         uint32_t v[4][kVWords];
 #pragma unroll
@@ -310,10 +323,12 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
         }
       }
       bad_now = bad_next;
+      bad_next = bad_after;
     };
-    for (int pair = 0; pair < pairs; pair += 2) {
-      step(pair, Int<0>{});
-      if (pair + 1 < pairs) step(pair + 1, Int<1>{});
+    for (int now = 0; now < steps; now += kDepth) {
+      step(now, Int<0>{});
+      if (now + 1 < steps) step(now + 1, Int<1>{});
+      if (now + 2 < steps) step(now + 2, Int<2>{});
     }
     cp_wait<0>();
 
