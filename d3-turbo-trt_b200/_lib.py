@@ -195,9 +195,14 @@ def strides(values: tuple[int, ...], n: int) -> Any:
     return (ctypes.c_int64 * n)(*values[:n])
 
 
+@functools.lru_cache(maxsize=4096)
+def _whole_rows(values: tuple[int, ...]) -> bool:
+    return values[-1] == 1 and not any(s % 8 for s in values[:-1])
+
+
 def rows16(t: torch.Tensor) -> torch.Tensor:
     """``t`` where its last dimension is contiguous and every row starts on 16 bytes (16-bit types), else a copy."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in t.stride()[:-1]):
+    if t.data_ptr() % 16 == 0 and _whole_rows(t.stride()):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

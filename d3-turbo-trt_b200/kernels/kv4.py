@@ -36,6 +36,7 @@ HEAD_DIMS = (64, 128, 256)
 PAGE_TOKENS = (16, 32, 64, 128, 256)
 SITE_BAD_SLOT, SITE_BAD_PAGE, SITE_BAD_LENGTH, SITE_BAD_MOVE = 2101, 2102, 2103, 2104
 
+append_key = "append"  # tells a plan's kind from the others'
 _TYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
@@ -93,10 +94,21 @@ class Kv4Cache:
         self.device = pool.device
         self._c = _lib.Kv4CacheStruct(pool.data_ptr(), self.layers, self.pages, kv_heads, head_dim, page_tokens)
         self._ref = ctypes.byref(self._c)
+        self._plans: dict = {}  # checked calls, by what the checks look at: shapes, strides, types, devices
 
     @property
     def nbytes(self) -> int:
         return self.pool.numel()
+
+    def _plan(self, key: tuple, make):
+        """What ``make()`` checked and worked out for calls of this key, kept for the next one."""
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = make()
+            if len(self._plans) >= 512:
+                self._plans.clear()
+            self._plans[key] = plan
+        return plan
 
     def _check_layer(self, layer: int) -> None:
         if not 0 <= layer < self.layers:
@@ -116,6 +128,19 @@ class Kv4Cache:
         ``slots`` [n] int64 on the device; a negative slot leaves its row out. Slots must differ: one
         that is named twice holds a mixture of the rows."""
         self._check_layer(layer)
+        key = (append_key, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, slots.shape,
+               slots.dtype, slots.device)
+        n, code, index, fn = self._plan(key, lambda: self._plan_append(k, v, slots))
+        if n == 0:
+            return
+        k, v, slots = _lib.rows16(k), _lib.rows16(v), slots.contiguous()
+        with _lib.on_device(self.device):
+            status = fn(self._ref, layer, k.data_ptr(), _lib.strides(k.stride(), 2), v.data_ptr(),
+                        _lib.strides(v.stride(), 2), slots.data_ptr(), n, code, _lib.raw_stream(index))
+        if status:
+            _lib.check(status, "d3b_kv4_append")
+
+    def _plan_append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> tuple:
         n, device, dtype = slots.numel(), self.device, k.dtype
         shape = (n, self.kv_heads, self.head_dim)
         if slots.dim() != 1 or k.shape != shape or v.shape != shape:
@@ -125,15 +150,7 @@ class Kv4Cache:
             raise RuntimeError(f"k and v must be fp16 or bf16 on {device}, got {dtype} on {k.device} and "
                                f"{v.dtype} on {v.device}")
         _index(slots, torch.int64, device, "slots")
-        if n == 0:
-            return
-        k, v, slots = _lib.rows16(k), _lib.rows16(v), slots.contiguous()
-        with _lib.on_device(device):
-            status = _lib.lib().d3b_kv4_append(
-                self._ref, layer, k.data_ptr(), _lib.strides(k.stride(), 2), v.data_ptr(), _lib.strides(v.stride(), 2),
-                slots.data_ptr(), n, _TYPES[dtype], _lib.raw_stream(device.index))
-        if status:
-            _lib.check(status, "d3b_kv4_append")
+        return n, _TYPES[dtype], device.index, _lib.lib().d3b_kv4_append
 
     def read(self, layer: int, table: torch.Tensor, tokens: int, *, dtype: torch.dtype = torch.bfloat16,
              ) -> tuple[torch.Tensor, torch.Tensor]:
@@ -142,7 +159,8 @@ class Kv4Cache:
         if dtype not in _TYPES:
             raise RuntimeError(f"read gives fp16 or bf16, not {dtype}")
         self._check_table(table, tokens)
-        k, v = torch.empty((2, self.kv_heads, tokens, self.head_dim), dtype=dtype, device=self.device).unbind(0)
+        k = torch.empty((self.kv_heads, tokens, self.head_dim), dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
         if tokens:
             table = table.contiguous()
             with _lib.on_device(self.device):
@@ -202,12 +220,11 @@ class Kv4Cache:
             _lib.check(status, "d3b_kv4_move_pages")
 
 
-def _check_query(q: torch.Tensor, cache: Kv4Cache, layer: int) -> None:
+def _check_query(q: torch.Tensor, cache: Kv4Cache) -> None:
     if not q.is_cuda or q.device != cache.device:
         raise RuntimeError(f"q is on {q.device}, the cache on {cache.device}")
     if q.dtype not in _TYPES:
         raise RuntimeError("the 4-bit cache's attention needs fp16 or bf16 queries")
-    cache._check_layer(layer)
     if q.shape[-1] != cache.head_dim:
         raise RuntimeError(f"q has head_dim {q.shape[-1]}, the cache {cache.head_dim}")
     if q.shape[1] == 0 or q.shape[1] % cache.kv_heads:
@@ -229,42 +246,53 @@ def decode_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torch.
     tokens in the cache, the L newest among them already appended. Every token sees all ``lengths[b]``
     tokens, or with ``causal`` those up to itself. Rows without a key are zero. Returns a tensor like q.
     """
-    single = q.dim() == 3
-    if single:
-        q = q.unsqueeze(2)
+    if q.dim() == 3:
         out = None if out is None else out.unsqueeze(2)
+        return decode_attention(q.unsqueeze(2), cache, layer, table, lengths, scale=scale, causal=causal, out=out).squeeze(2)
+    key = (decode_attention, q.shape, q.dtype, q.device, table.shape, table.stride(), table.dtype, table.device,
+           lengths.shape, lengths.stride(), lengths.dtype, lengths.device)
+    rows, heads, width, code, index, need, fn = cache._plan(key, lambda: _plan_decode(q, cache, table, lengths))
+    cache._check_layer(layer)
+    q = _lib.rows16(q)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        _check_out(out, q)
+    if need:
+        if table.stride(1) != 1 or table.stride(0) < 0:
+            table = table.contiguous()
+        if lengths.stride(0) != 1:
+            lengths = lengths.contiguous()
+        # from the caching allocator at every call: calls on other streams and captured graphs get
+        # their own, and it is ordered with the stream like any tensor
+        with _lib.on_device(cache.device):
+            work = cache.pool.new_empty(need)
+            status = fn(cache._ref, layer, q.data_ptr(), _lib.strides(q.stride(), 3), table.data_ptr(), table.stride(0),
+                        table.shape[1], lengths.data_ptr(), rows, heads, width, causal, code, scale, out.data_ptr(),
+                        _lib.strides(out.stride(), 3), work.data_ptr(), need, _lib.raw_stream(index))
+        if status:
+            _lib.check(status, "d3b_kv4_decode")
+    return out
+
+
+def _plan_decode(q: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, lengths: torch.Tensor) -> tuple:
     if q.dim() != 4:
         raise RuntimeError(f"q must be [B, H, L, D] or [B, H, D], got {tuple(q.shape)}")
-    _check_query(q, cache, layer)
+    _check_query(q, cache)
     rows, heads, width, _ = q.shape
-    device = cache.device
+    device, lib = cache.device, _lib.lib()
     _index(table, torch.int32, device, "table")
     _index(lengths, torch.int32, device, "lengths")
     if table.dim() != 2 or table.shape[0] != rows or tuple(lengths.shape) != (rows,):
         raise RuntimeError(f"table must be [{rows}, width] and lengths [{rows}], got {tuple(table.shape)}, "
                            f"{tuple(lengths.shape)}")
-    q = _lib.rows16(q)
-    if out is None:
-        out = q.new_empty(q.shape)
-    else:
-        _check_out(out, q)
+    need = 0
     if rows and width:
-        if table.shape[1] and (table.stride(1) != 1 or table.stride(0) < 0):
-            table = table.contiguous()
-        lengths = lengths.contiguous()
-        lib = _lib.lib()
         with _lib.on_device(device):
             need = lib.d3b_kv4_decode_workspace_size(cache._ref, rows, heads, width, table.shape[1])
-            # from the caching allocator at every call: calls on other streams and captured graphs
-            # get their own, and it is ordered with the stream like any tensor
-            work = cache.pool.new_empty(need) if need else None
-            status = lib.d3b_kv4_decode(
-                cache._ref, layer, q.data_ptr(), _lib.strides(q.stride(), 3), table.data_ptr(), table.stride(0),
-                table.shape[1], lengths.data_ptr(), rows, heads, width, causal, _TYPES[q.dtype], scale, out.data_ptr(),
-                _lib.strides(out.stride(), 3), work.data_ptr() if need else None, need, _lib.raw_stream(device.index))
-        if status:
-            _lib.check(status, "d3b_kv4_decode")
-    return out.squeeze(2) if single else out
+        if need == 0:
+            raise RuntimeError(f"decode_attention: queries {tuple(q.shape)} over tables {tuple(table.shape)} are too many")
+    return rows, heads, width, _TYPES[q.dtype], device.index, need, lib.d3b_kv4_decode
 
 
 def question_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torch.Tensor, state_len: int,
@@ -276,24 +304,19 @@ def question_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torc
     q [B, H, L, D], k_q/v_q [B, H_kv, L, D], ``lengths`` as there. Returns [B, H, L, D], zero rows
     for padding.
     """
-    if q.dim() != 4:
-        raise RuntimeError(f"q must be [B, H, L, D], got {tuple(q.shape)}")
-    _check_query(q, cache, layer)
-    rows, heads, width, dim = q.shape
-    cache._check_table(table, state_len)
-    if k_q.dtype != q.dtype or v_q.dtype != q.dtype or k_q.device != q.device or v_q.device != q.device:
-        raise RuntimeError("q, k and v must share a dtype and a device")
-    if tuple(k_q.shape) != (rows, cache.kv_heads, width, dim) or v_q.shape != k_q.shape:
-        raise RuntimeError(f"k_q/v_q must be [B, H_kv, L, D] = {(rows, cache.kv_heads, width, dim)}")
-    if isinstance(lengths, torch.Tensor):
-        if lengths.numel() != rows:
-            raise RuntimeError(f"{lengths.numel()} lengths for {rows} question blocks")
-    else:
-        lengths = [int(n) for n in lengths]
-        if len(lengths) != rows or any(not 0 <= n <= width for n in lengths):
-            raise RuntimeError(f"lengths must be {rows} values in [0, {width}]")
+    cache._check_layer(layer)
+    key = (question_attention, q.shape, q.dtype, q.device, k_q.shape, k_q.dtype, k_q.device, v_q.shape, v_q.dtype,
+           v_q.device, table.shape, table.dtype, table.device, state_len)
+    rows, heads, width, code, index, need, fn = cache._plan(key, lambda: _plan_question(q, cache, table, state_len, k_q, v_q))
+    if not (isinstance(lengths, torch.Tensor) and lengths.is_cuda):
+        lengths = [int(n) for n in (lengths.tolist() if isinstance(lengths, torch.Tensor) else lengths)]
+        if any(not 0 <= n <= width for n in lengths):
+            raise RuntimeError(f"lengths must lie in [0, {width}]")
+    if len(lengths) != rows:
+        raise RuntimeError(f"{len(lengths)} lengths for {rows} question blocks")
+    q, k_q, v_q = _lib.rows16(q), _lib.rows16(k_q), _lib.rows16(v_q)
     if out is None:
-        out = q.new_empty((rows, heads, width, dim))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check_out(out, q)
     if rows == 0 or width == 0:
@@ -301,16 +324,12 @@ def question_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torc
     device = cache.device
     with _lib.on_device(device):
         lens = block_offsets(lengths, device)
-        q, k_q, v_q = _lib.rows16(q), _lib.rows16(k_q), _lib.rows16(v_q)
-        if _reads_codes(rows, heads, cache.kv_heads, width, state_len, dim):
-            lib, table = _lib.lib(), table.contiguous()
-            need = lib.d3b_kv4_question_workspace_size(cache._ref, rows, heads, width, state_len)
-            work = cache.pool.new_empty(need)
-            status = lib.d3b_kv4_question(
-                cache._ref, layer, q.data_ptr(), _lib.strides(q.stride(), 3), table.data_ptr(), table.shape[0], state_len,
-                k_q.data_ptr(), _lib.strides(k_q.stride(), 3), v_q.data_ptr(), _lib.strides(v_q.stride(), 3), lens.data_ptr(),
-                rows, heads, width, _TYPES[q.dtype], scale, out.data_ptr(), _lib.strides(out.stride(), 3), work.data_ptr(),
-                need, _lib.raw_stream(device.index))
+        if need:
+            table, work = table.contiguous(), cache.pool.new_empty(need)
+            status = fn(cache._ref, layer, q.data_ptr(), _lib.strides(q.stride(), 3), table.data_ptr(), table.shape[0],
+                        state_len, k_q.data_ptr(), _lib.strides(k_q.stride(), 3), v_q.data_ptr(),
+                        _lib.strides(v_q.stride(), 3), lens.data_ptr(), rows, heads, width, code, scale, out.data_ptr(),
+                        _lib.strides(out.stride(), 3), work.data_ptr(), need, _lib.raw_stream(index))
             if status:
                 _lib.check(status, "d3b_kv4_question")
         else:
@@ -319,6 +338,24 @@ def question_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torc
                 k_q, v_q = (x.clone(memory_format=torch.contiguous_format) for x in (k_q, v_q))
             _prefix_bidir(q, k, v, k_q, v_q, lens, scale, out)
     return out
+
+
+def _plan_question(q: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, state_len: int, k_q: torch.Tensor,
+                   v_q: torch.Tensor) -> tuple:
+    if q.dim() != 4:
+        raise RuntimeError(f"q must be [B, H, L, D], got {tuple(q.shape)}")
+    _check_query(q, cache)
+    rows, heads, width, dim = q.shape
+    cache._check_table(table, state_len)
+    if k_q.dtype != q.dtype or v_q.dtype != q.dtype or k_q.device != q.device or v_q.device != q.device:
+        raise RuntimeError("q, k and v must share a dtype and a device")
+    if tuple(k_q.shape) != (rows, cache.kv_heads, width, dim) or v_q.shape != k_q.shape:
+        raise RuntimeError(f"k_q/v_q must be [B, H_kv, L, D] = {(rows, cache.kv_heads, width, dim)}")
+    need, lib = 0, _lib.lib()
+    if rows and width and _reads_codes(rows, heads, cache.kv_heads, width, state_len, dim):
+        with _lib.on_device(cache.device):
+            need = lib.d3b_kv4_question_workspace_size(cache._ref, rows, heads, width, state_len)
+    return rows, heads, width, _TYPES[q.dtype], cache.device.index, need, lib.d3b_kv4_question
 
 
 def _reads_codes(rows: int, heads: int, kv_heads: int, width: int, state_len: int, dim: int) -> bool:

@@ -281,8 +281,8 @@ def qk_norm_mrope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_we
     rounded once, where ``qk_norm_rope`` rounds after each of the reference's bf16 operations.
     """
     # the checks go by shapes, strides and types alone: once for each set of them
-    key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device, q_weight.shape, q_weight.dtype,
-           k_weight.shape, k_weight.dtype, positions.shape, positions.dtype, positions.device, inv_freq.shape,
+    key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device, q_weight.shape,
+           q_weight.stride(), k_weight.shape, k_weight.stride(), positions.shape, positions.dtype, positions.device, inv_freq.shape,
            inv_freq.stride(), inv_freq.dtype, inv_freq.device, tuple(axes))
     plan = _ROPE_PLANS.get(key)
     if plan is None:
@@ -290,13 +290,14 @@ def qk_norm_mrope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_we
         if len(_ROPE_PLANS) >= 1024:
             _ROPE_PLANS.clear()
         _ROPE_PLANS[key] = plan
-    q_shape, k_shape, axis, fn = plan
+    q_shape, k_shape, axis, ready, fn = plan
     device, dtype = q.device, q.dtype
     if q_weight.dtype != dtype or q_weight.device != device:
         q_weight = q_weight.to(device=device, dtype=dtype)
     if k_weight.dtype != dtype or k_weight.device != device:
         k_weight = k_weight.to(device=device, dtype=dtype)
-    q, k, q_weight, k_weight = (_lib.rows16(x) for x in (q, k, q_weight, k_weight))
+    if not ready or (q.data_ptr() | k.data_ptr() | q_weight.data_ptr() | k_weight.data_ptr()) & 15:
+        q, k, q_weight, k_weight = (_lib.rows16(x) for x in (q, k, q_weight, k_weight))
     q_out, k_out = q.new_empty(q_shape), q.new_empty(k_shape)
     if q_out.numel() + k_out.numel():
         with _lib.on_device(device):
@@ -340,7 +341,9 @@ def _plan_mrope(q, k, q_weight, k_weight, positions, inv_freq, axes):
         raise RuntimeError(f"qk_norm_mrope: positions and inv_freq must be on {q.device}")
     if q_weight.numel() != D or k_weight.numel() != D or q_weight.dim() != 1 or k_weight.dim() != 1:
         raise RuntimeError(f"qk_norm_mrope: weights must be [{D}], got {tuple(q_weight.shape)} and {tuple(k_weight.shape)}")
-    return (rows, T, heads, D), (rows, T, kv_heads, D), bytes(axes), _lib.lib().d3b_qk_norm_mrope
+    ready = (all(x.stride(-1) == 1 and not any(s % 8 for s in x.stride()[:-1]) for x in (q, k))
+             and q_weight.stride(0) == 1 and k_weight.stride(0) == 1)
+    return (rows, T, heads, D), (rows, T, kv_heads, D), bytes(axes), ready, _lib.lib().d3b_qk_norm_mrope
 
 
 def gdn_gates(a: torch.Tensor, b: torch.Tensor, neg_exp_a: torch.Tensor, dt_bias: torch.Tensor):
