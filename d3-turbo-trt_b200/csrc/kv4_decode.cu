@@ -127,6 +127,8 @@ int launch_merge(const AttnArgs& a, int nt, bool bf, cudaStream_t s) {
 
 int run(AttnArgs& a, const d3b_kv4_cache* c, const Plan& p, bool bf, void* workspace, cudaStream_t s) {
   const int D = c->head_dim;
+  a.err = d3b_host::device_error_word();
+  if (!a.err) return D3B_ECUDA;
   a.row_tiles = p.row_tiles;
   a.part_o = static_cast<float*>(workspace);
   a.part_st = a.part_o + (size_t)p.ctas * 2 * 8 * p.nt * D;
@@ -146,7 +148,7 @@ int check_shape(const d3b_kv4_cache* c, int B, int H, int L, int64_t width) {
   return D3B_OK;
 }
 
-// what both entry points share; D3B_OK with a->err == nullptr: nothing to do
+// what both entry points check; D3B_OK with a->q == nullptr: nothing to do
 int prepare(const d3b_kv4_cache* cache, int64_t layer, const void* q, const int64_t* q_strides, const int32_t* table,
             int64_t table_stride, int64_t width, int B, int H, int L, int dtype, float scale, void* out,
             const int64_t* out_strides, AttnArgs* a) {
@@ -178,8 +180,7 @@ int prepare(const d3b_kv4_cache* cache, int64_t layer, const void* q, const int6
   a->group = H / cache->kv_heads;
   a->L = L;
   a->scale_log2 = scale * 1.4426950408889634f;
-  a->err = d3b_host::device_error_word();
-  return a->err ? D3B_OK : D3B_ECUDA;
+  return D3B_OK;
 }
 
 int check_workspace(const void* workspace, size_t have, size_t need) {
@@ -205,7 +206,7 @@ int d3b_kv4_decode(const d3b_kv4_cache* cache, int64_t layer, const void* q, con
   AttnArgs a;
   if (int rc = prepare(cache, layer, q, q_strides, table, table_stride, width, B, H, L, dtype, scale, out, out_strides, &a))
     return rc;
-  if (!a.err) return D3B_OK;
+  if (!a.q) return D3B_OK;
   if (!lengths || table_stride < 0 || (B > 1 && table_stride < width && table_stride != 0)) return D3B_EINVAL;
   if (reinterpret_cast<uintptr_t>(lengths) % 4) return D3B_EALIGN;
   a.lengths = lengths;
@@ -230,7 +231,7 @@ int d3b_kv4_question(const d3b_kv4_cache* cache, int64_t layer, const void* q, c
                      d3b_stream_t stream) {
   AttnArgs a;
   if (int rc = prepare(cache, layer, q, q_strides, table, 0, width, B, H, L, dtype, scale, out, out_strides, &a)) return rc;
-  if (!a.err) return D3B_OK;
+  if (!a.q) return D3B_OK;
   if (state_len < 0 || state_len > a.most) return D3B_EINVAL;
   if (!k_q || !v_q || !k_strides || !v_strides || !lengths) return D3B_EINVAL;
   if (reinterpret_cast<uintptr_t>(k_q) % 16 || reinterpret_cast<uintptr_t>(v_q) % 16) return D3B_EALIGN;

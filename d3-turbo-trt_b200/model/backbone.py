@@ -16,7 +16,7 @@ library:
   GDN input projections, or gate/up_proj);
 * every Linear: ``QuantLinear`` (W8A8, tcgen05 GEMM, dequant fused);
 * attention: ``state_attention`` for the state pass, ``prefix_bidir_attention``
-  for the question pass, then ``out * sigmoid(gate)`` fused with o_proj's
+  for the question pass (``kv4.question_attention`` over a state kept in 4 bits), then ``out * sigmoid(gate)`` fused with o_proj's
   quantisation (``fused.sigmoid_gate_quant``);
 * the GDN layers' causal convolution + SiLU: ``conv.causal_conv1d_silu`` on the
   in_proj output as the GEMM writes it (token-major; reads the snapshot's tail in
@@ -47,9 +47,10 @@ from typing import Callable, Mapping, Sequence
 import torch
 import torch.nn.functional as F
 
-from ..kernels import prefix_bidir as pb
+from ..kernels import kv4, prefix_bidir as pb
 from . import fused, gdn
 from .conv import causal_conv1d_silu
+from .pages import Kv4Entry, Kv4States
 from .quant import QuantLinear, quantizable, quantize_rows
 from .readout import probabilities_tensor
 from .snapshot import AttentionEntry, DeltaEntry
@@ -74,6 +75,9 @@ class BackboneConfig:
     rms_norm_eps: float = 1e-6
     rope_theta: float = 10_000_000.0
     partial_rotary_factor: float = 0.25
+    # rotary frequencies of each position axis (time, height, width), for positions on several axes
+    mrope_section: tuple | None = None
+    mrope_interleaved: bool = True
     layer_types: list = field(default_factory=lambda: (["linear_attention"] * 3 + ["full_attention"]) * 16)
 
     @property
@@ -100,6 +104,24 @@ def rotary_tables(config: BackboneConfig, positions: torch.Tensor, dtype: torch.
     freqs = positions.float()[..., None] * inv_freq  # [B, T, dim/2]
     emb = torch.cat((freqs, freqs), dim=-1)
     return emb.cos().to(dtype), emb.sin().to(dtype)
+
+
+class AxisPositions:
+    """Rotary positions [axes, B, T] int64 with the frequencies and their axes, for ``fused.qk_norm_mrope``."""
+
+    def __init__(self, config: BackboneConfig, positions: torch.Tensor):
+        dim = int(config.head_dim * config.partial_rotary_factor)
+        self.positions = positions
+        self.inv_freq = 1.0 / (config.rope_theta ** (torch.arange(0, dim, 2, dtype=torch.int64, device=positions.device)
+                                                     .float() / dim))
+        if positions.shape[0] == 1:
+            self.axes: tuple[int, ...] = (0,) * (dim // 2)
+        else:
+            if config.mrope_section is None or sum(config.mrope_section) != dim // 2 or (
+                    len(config.mrope_section) != positions.shape[0]):
+                raise ValueError(f"positions on {positions.shape[0]} axes need as many mrope_section counts that sum to "
+                                 f"{dim // 2}, got {config.mrope_section}")
+            self.axes = fused.rotary_axes(config.mrope_section, interleaved=config.mrope_interleaved)
 
 
 def apply_rotary(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor):
@@ -221,29 +243,49 @@ class D3Backbone:
     def embed_ids(self, ids: torch.Tensor) -> torch.Tensor:
         return F.embedding(ids.to(self.device), self.embed)
 
-    def state(self, ids: torch.Tensor) -> Snapshot:
-        """``ids`` [1, S] -> snapshot (one entry per layer), as core.py:146-156."""
+    def _rope(self, positions: torch.Tensor, axis_positions: torch.Tensor | None, dtype: torch.dtype):
+        """What the attention layers turn queries and keys by: cos/sin tables of text positions [B, T]
+        (head_dim 128), or positions per axis."""
+        if axis_positions is None:
+            if self.config.head_dim == 128:
+                return rotary_tables(self.config, positions, dtype)
+            return AxisPositions(self.config, positions[None])
+        if axis_positions.dim() != 3 or axis_positions.shape[1:] != positions.shape:
+            raise ValueError(f"positions must be [axes, {positions.shape[0]}, {positions.shape[1]}], got "
+                             f"{tuple(axis_positions.shape)}")
+        return AxisPositions(self.config, axis_positions.to(device=self.device, dtype=torch.int64))
+
+    def state(self, ids: torch.Tensor, *, positions: torch.Tensor | None = None, states: Kv4States | None = None) -> Snapshot:
+        """``ids`` [1, S] -> snapshot (one entry per layer), as core.py:146-156.
+
+        ``positions`` [axes, 1, S] gives the tokens' rotary positions on several axes (default: their
+        place on every axis). With ``states`` the attention layers' K/V go into its pages in 4 bits
+        (``RuntimeError`` where none are free) and the snapshot reads them there."""
         embeds = self.embed_ids(ids)
-        positions = torch.arange(ids.shape[1], device=self.device)[None]
-        rope = rotary_tables(self.config, positions, embeds.dtype)
+        rope = self._rope(torch.arange(ids.shape[1], device=self.device)[None], positions, embeds.dtype)
         snapshot: Snapshot = []
         hidden, delta = embeds, None
         for L in self.layers:
             hidden, delta, entry = self._layer(L, hidden, delta, rope, None, None, None)
             snapshot.append(entry)
+        if states is not None:
+            snapshot = states.store(snapshot)
+            if snapshot is None:
+                raise RuntimeError(f"no pages for a state of {ids.shape[1]} tokens: {states.stats()}")
         return snapshot
 
     def questions(self, snapshot: Snapshot, ids: torch.Tensor, lengths: Sequence[int], *,
-                  state_len: int) -> torch.Tensor:
+                  state_len: int, positions: torch.Tensor | None = None) -> torch.Tensor:
         """``ids`` [B, W] right-padded -> final-norm hidden [B, hidden] at each block's last
-        token, as core.py:158-181 (padding rows zeroed at the embedding)."""
+        token, as core.py:158-181 (padding rows zeroed at the embedding). ``positions`` [axes, B, W]
+        as in ``state``; the default goes on from ``state_len`` on every axis."""
         rows, width = ids.shape
         lengths = [int(n) for n in lengths]
         lens_t = torch.tensor(lengths, device=self.device)
         present = torch.arange(width, device=self.device)[None, :] < lens_t[:, None]
         embeds = self.embed_ids(ids) * present[..., None].to(torch.bfloat16)
-        positions = (state_len + torch.arange(width, device=self.device))[None].expand(rows, -1)
-        rope = rotary_tables(self.config, positions, embeds.dtype)
+        text = (state_len + torch.arange(width, device=self.device))[None].expand(rows, -1)
+        rope = self._rope(text, positions, embeds.dtype)
         lens_d = lens_t.to(torch.int32)
         hidden, delta = embeds, None
         for L, entry in zip(self.layers, snapshot):
@@ -280,12 +322,17 @@ class D3Backbone:
         D, Hq, Hkv = c.head_dim, c.num_attention_heads, c.num_key_value_heads
         qg = L["q_proj"].from_codes(q, s, None).view(rows, T, Hq, 2 * D)
         gate = qg[..., D:]
-        cos, sin = rope
-        # q_norm / k_norm and the partial rotary embedding in one kernel each, written
-        # token-major [rows, T, heads, D]; the attention reads [rows, heads, T, D] views
-        query = fused.qk_norm_rope(qg[..., :D], L["q_norm"], cos, sin, c.rms_norm_eps).transpose(1, 2)
-        key = fused.qk_norm_rope(L["k_proj"].from_codes(q, s, None).view(rows, T, Hkv, D), L["k_norm"], cos, sin,
-                                 c.rms_norm_eps).transpose(1, 2)
+        key = L["k_proj"].from_codes(q, s, None).view(rows, T, Hkv, D)
+        # q_norm / k_norm and the partial rotary embedding, written token-major [rows, T, heads, D]; the
+        # attention reads [rows, heads, T, D] views
+        if isinstance(rope, AxisPositions):  # one kernel for both
+            query, key = fused.qk_norm_mrope(qg[..., :D], key, L["q_norm"], L["k_norm"], rope.positions, rope.inv_freq,
+                                             rope.axes, c.rms_norm_eps)
+        else:  # one each
+            cos, sin = rope
+            query = fused.qk_norm_rope(qg[..., :D], L["q_norm"], cos, sin, c.rms_norm_eps)
+            key = fused.qk_norm_rope(key, L["k_norm"], cos, sin, c.rms_norm_eps)
+        query, key = query.transpose(1, 2), key.transpose(1, 2)
         # the kernels read K and V through one set of strides: v_proj's output is already
         # token-major like K, so V is a view of it
         value = L["v_proj"].from_codes(q, s, None).view(rows, T, Hkv, D).transpose(1, 2)
@@ -293,6 +340,9 @@ class D3Backbone:
         if entry is None:
             out = pb.state_attention(query, key, value, scale=scale)
             entry = AttentionEntry(keys=key, values=value)
+        elif isinstance(entry, Kv4Entry):
+            out = kv4.question_attention(query, entry.cache, entry.layer, entry.table, entry.tokens, key, value, lens_d,
+                                         scale=scale)
         else:
             out = pb.prefix_bidir_attention(query, entry.keys[0], entry.values[0], key, value, lens_d, scale=scale)
         qo, so = fused.sigmoid_gate_quant(out.transpose(1, 2), gate, self.mode)

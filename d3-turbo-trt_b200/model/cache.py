@@ -49,6 +49,8 @@ def tensor_bytes(obj: Any) -> int:
         item = pending.pop()
         if hasattr(item, "numel") and hasattr(item, "element_size"):
             total += int(item.numel()) * int(item.element_size())
+        elif hasattr(item, "held_bytes"):  # K/V in pages: the pages it holds, not the pool they are in
+            total += int(item.held_bytes)
         elif isinstance(item, (list, tuple)):
             pending.extend(item)
         elif hasattr(item, "__dict__"):
@@ -169,7 +171,8 @@ class StateCache:
             return entry
 
     def put(self, key: str, snapshot: Any, state_len: int, media_hash: str = "") -> StateEntry | None:
-        layout = SnapshotLayout.of(snapshot) if self.arena is not None else None
+        packs = self.arena is not None and getattr(snapshot, "packable", True)
+        layout = SnapshotLayout.of(snapshot) if packs else None
         nbytes = tensor_bytes(snapshot) if layout is None else layout.tensor_bytes
         if self.capacity_bytes == 0 or nbytes > self.capacity_bytes:
             self.rejected += 1
