@@ -232,7 +232,6 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
       // exponents of l's terms and of the weights, masked keys at -infinity
       float x[P::GP][NT][4], y[P::GP][NT][4];
       auto exponents = [&] {
-        float most = -INFINITY;
 #pragma unroll
         for (int i = 0; i < P::GP; ++i)
 #pragma unroll
@@ -241,12 +240,25 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
             for (int j = 0; j < 4; ++j) {
               x[i][n][j] = fmaf(s[i][n][j], kq[i][j >> 1], -m[n][j & 1]);
               y[i][n][j] = x[i][n][j] + ev[i][j >> 1];
-              if (edge) {
+            }
+        if (edge) {  // apart from the sums above, so that it is a branch and not selects in every step
+#pragma unroll
+          for (int i = 0; i < P::GP; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
                 const int key = r + 8 * (j >> 1);
                 if (key >= live[i] || key0 + 16 * i + key >= limit[n][j & 1]) x[i][n][j] = y[i][n][j] = -INFINITY;
               }
-              most = fmaxf(most, y[i][n][j]);
-            }
+        }
+        float most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < P::GP; ++i)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) most = fmaxf(most, y[i][n][j]);
         return most;
       };
       // m = -infinity (no key yet) makes every exponent +infinity

@@ -154,16 +154,25 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
     auto weigh = [&](const float (&s)[NT][4], const float (&kq)[2], const float (&ev)[2], bool edge, auto masked, auto between) {
       float x[NT][4], y[NT][4];  // exponents of l's terms and of the weights
       auto exponents = [&] {
-        float most = -INFINITY;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             x[n][j] = fmaf(s[n][j], kq[j >> 1], -m[n][j & 1]);
             y[n][j] = x[n][j] + ev[j >> 1];
-            if (edge && masked(n, j)) x[n][j] = y[n][j] = -INFINITY;
-            most = fmaxf(most, y[n][j]);
           }
+        if (edge) {  // apart from the sums above, so that it is a branch and not selects in every tile
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (masked(n, j)) x[n][j] = y[n][j] = -INFINITY;
+        }
+        float most = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) most = fmaxf(most, y[n][j]);
         return most;
       };
       // m = -infinity (no key yet) makes every exponent +infinity. Behind this barrier every warp's copies have
