@@ -21,15 +21,16 @@ constexpr int kKeys = 64;
 
 template <int D, int NT>
 struct Wide {
-  static constexpr int kStage = (granule_bytes(D) + 127) / 128 * 128;
+  static constexpr int kHalf = off_v(D);                    // bytes of a granule's K or V part
+  static constexpr int kStage = (kHalf + 127) / 128 * 128;  // V rows start on 128-byte lines
   static constexpr int kRows = 8 * NT;
-  static constexpr int kResident = 3;
-  static constexpr int kRing = 2 * 4 * kStage;  // two tiles of four granules
+  static constexpr int kResident = 2;
+  static constexpr int kRing = 2 * 2 * 4 * kStage;  // two tiles' K, then two tiles' V, of four granules
   static constexpr int kQ = kRows * D * 2;
   static constexpr int kW = 4 * NT * 32 * 8;    // weights: [granule][nt][lane] x 8 bytes
   static constexpr int kMax = kWarps * kRows * 4;
   static constexpr int kSmem = kRing + kQ + kW + kMax + kKeys * 4;
-  static constexpr int kKc = 0, kVc = 8 * D, kKs = 16 * D, kVs = 17 * D, kKe = 18 * D, kVe = 18 * D + 16;
+  static constexpr int kScales = off_k_scale(D), kExps = off_k_exp(D);  // within a stage, after the codes
 };
 
 __device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) {
@@ -56,34 +57,27 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
   const int rows = a.group * a.L;
   const Deal mine = deal<kKeys, P::kRows>(a, 1, box);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may take its place; it waits for our end
-  const uint32_t ring = d3b::smem_u32(smem);
+  const uint32_t k_ring = d3b::smem_u32(smem), v_ring = k_ring + 2 * 4 * P::kStage;
   const int grain_shift = a.page_shift - 4, in_page = (1 << grain_shift) - 1;
-  // a lane copies units lane, lane + 32, ... of 16 bytes of its warp's granule; where each goes in a tile
-  constexpr int kUnits = granule_bytes(D) / 16, kCopies = (kUnits + 31) / 32;
-  uint32_t place[kCopies];
+  // a lane copies units lane, lane + 32, ... of 16 bytes of its warp's granule's K or V; where V's go
+  constexpr int kUnits = P::kHalf / 16, kCopies = (kUnits + 31) / 32;
+  const uint32_t k_to = k_ring + warp * P::kStage + 16 * lane;
+  uint32_t v_to[kCopies];
 #pragma unroll
   for (int i = 0; i < kCopies; ++i) {
-    constexpr int kHalf = off_v(D) / 16, kCodes = 8 * D / 16, kScales = D / 16;
-    const int u = 32 * i + lane;
-    const bool is_v = u >= kHalf;
-    const int x = is_v ? u - kHalf : u;
-    int to;
-    if (x < kCodes) to = is_v ? P::kVc + v_swizzle<D>(16 * x) : P::kKc + 16 * x;
-    else if (x < kCodes + kScales) to = (is_v ? P::kVs : P::kKs) + 16 * (x - kCodes);
-    else to = is_v ? P::kVe : P::kKe;
-    place[i] = ring + warp * P::kStage + to;
-    asm volatile("" : "+r"(place[i]));  // kept, not worked out again at every copy
+    const int at = 16 * (32 * i + lane);
+    v_to[i] = v_ring + warp * P::kStage + (at < 8 * D ? v_swizzle<D>(at) : at);
+    asm volatile("" : "+r"(v_to[i]));  // kept, not worked out again at every copy
   }
-  const uint32_t stage = ring + warp * P::kStage;
-  const uint32_t k_at = stage + P::kKc + r * (D / 2) + c * (D == 256 ? 16 : D / 8);
-  const uint32_t ks_at = stage + P::kKs + r * (D / 16) + (D == 64 ? c : 2 * c);
-  const uint32_t e_at = stage + P::kKe + r;
+  const uint32_t k_at = k_ring + warp * P::kStage + r * (D / 2) + c * (D == 256 ? 16 : D / 8);
+  const uint32_t ks_at = k_ring + warp * P::kStage + P::kScales + r * (D / 16) + (D == 64 ? c : 2 * c);
+  const uint32_t ke_at = k_ring + warp * P::kStage + P::kExps + r, ve_at = v_ring + warp * P::kStage + P::kExps + r;
   // V: channels warp * D/4 + r * D/32 ...; rows 2c, 2c + 1, 2c + 8, 2c + 9 of every granule
   uint32_t v_at[4];
 #pragma unroll
   for (int x = 0; x < 4; ++x)
-    v_at[x] = ring + P::kVc + v_swizzle<D>((2 * c + (x & 1) + 8 * (x >> 1)) * (D / 2) + warp * (D / 8) + r * (D / 64));
-  const uint32_t vs_at = ring + P::kVs + ((warp * (D / 4) + r * kRun) / 16) * 16 + 2 * c;
+    v_at[x] = v_ring + v_swizzle<D>((2 * c + (x & 1) + 8 * (x >> 1)) * (D / 2) + warp * (D / 8) + r * (D / 64));
+  const uint32_t vs_at = v_ring + P::kScales + ((warp * (D / 4) + r * kRun) / 16) * 16 + 2 * c;
 
   int pos = mine.first, b = mine.b, offset = mine.offset;
   while (pos < mine.last) {
@@ -99,32 +93,44 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
     const int last_cached = dead ? piece0 : min(piece1, seq.cached);
     const uint8_t* head_pool = a.pool + kvh * a.head_bytes + 16 * lane;
     const int32_t* table = a.table + b * a.table_stride;
-    int id = 0;  // page of the warp's granule of the tile that is loaded next
+    // page of the warp's granule of a tile; -1 where there is no such granule
     auto look = [&](int p) {
       const int g = 4 * p + warp;
-      if (g < grains) id = __ldg(table + (g >> grain_shift));
+      return p < last_cached && g < grains ? __ldg(table + (g >> grain_shift)) : -1;
     };
-    // copies the warp's granule of tile p to ring half HALF; how many of its tokens are keys
-    auto load = [&](int p, uint32_t half) -> int {
-      const int g = 4 * p + warp;
-      if (g >= grains) return 0;
-      if ((uint32_t)id >= (uint32_t)a.pages) {
-        if (lane == 0) d3b::record_device_error(a.err, kSiteBadPage);
+    auto in_pool = [&](int id) { return (uint32_t)id < (uint32_t)a.pages; };
+    auto source = [&](int p, int id) {
+      return head_pool + id * a.page_bytes + ((4 * p + warp) & in_page) * granule_bytes(D);
+    };
+    // copy the warp's granule of tile p to ring half HALF: K (how many of its tokens are keys), V
+    auto load_k = [&](int p, int id, uint32_t half) -> int {
+      if (!in_pool(id)) {
+        if (lane == 0 && p < last_cached && 4 * p + warp < grains) d3b::record_device_error(a.err, kSiteBadPage);
         return 0;
       }
-      const uint8_t* src = head_pool + id * a.page_bytes + (g & in_page) * granule_bytes(D);
+      const uint8_t* src = source(p, id);
 #pragma unroll
       for (int x = 0; x < kCopies; ++x)
-        if (32 * x + 31 < kUnits || 32 * x + lane < kUnits) cp16(place[x] + half, src + 512 * x);
-      return min(16, len - 16 * g);
+        if (32 * x + 31 < kUnits || 32 * x + lane < kUnits) cp16(k_to + half + 512 * x, src + 512 * x);
+      return min(16, len - 16 * (4 * p + warp));
     };
-    int live_now = 0, live_next = 0;
-    if (piece0 < last_cached) {
-      look(piece0);
-      live_now = load(piece0, 0);
-    }
+    auto load_v = [&](int p, int id, uint32_t half) {
+      if (!in_pool(id)) return;
+      const uint8_t* src = source(p, id) + off_v(D);
+#pragma unroll
+      for (int x = 0; x < kCopies; ++x)
+        if (32 * x + 31 < kUnits || 32 * x + lane < kUnits) cp16(v_to[x] + half, src + 512 * x);
+    };
+    constexpr uint32_t kHalfRing = 4 * P::kStage;
+    // tokens of the warp's granule that are keys: of this tile, the next and the one after; pages of the latter two
+    int live_now = 0, live_next = 0, live_after = 0, id_v = look(piece0), id_k = look(piece0 + 1);
+    live_now = load_k(piece0, id_v, 0);
     cp_commit();
-    if (piece0 + 1 < last_cached) look(piece0 + 1);
+    load_v(piece0, id_v, 0);
+    live_next = load_k(piece0 + 1, id_k, kHalfRing);
+    cp_commit();
+    id_v = id_k;
+    id_k = look(piece0 + 2);
 
     const float q_scale = load_queries<D, NT, BF>(a, b, kvh, row0, rows, qs, tops);
     __syncthreads();
@@ -227,83 +233,92 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
       __syncthreads();
     };
 
-    for (int p = piece0; p < last_cached; ++p) {
-      const uint32_t half = ((p - piece0) & 1) * (4 * P::kStage);
-      cp_wait<0>();
-      __syncwarp();
-      const int key0 = 64 * p + 16 * warp;
-      float s[NT][4];
+    float s[NT][4], kq[2];  // products of keys r and r + 8 of the warp's granule, and the scores' factors
+    auto scores = [&](uint32_t half) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[n][j] = 0.f;
+      uint32_t k0[kKWords], k1[kKWords], s0[kKWords / 2], s1[kKWords / 2];
+      lds_words<D == 256 ? 4 : kKWords>(k_at + half, k0);
+      lds_words<D == 256 ? 4 : kKWords>(k_at + half + 4 * D, k1);
+      if constexpr (D == 256) {
+        lds_words<4>(k_at + half + 64, k0 + 4);
+        lds_words<4>(k_at + half + 4 * D + 64, k1 + 4);
+      }
+      if constexpr (D == 64) {
+        s0[0] = decode_scales(lds_u8(ks_at + half) * 0x101u);
+        s1[0] = decode_scales(lds_u8(ks_at + half + D / 2) * 0x101u);
+      } else {
+#pragma unroll
+        for (int w = 0; w < kKWords / 4; ++w) {
+          const uint32_t x0 = decode_scales(lds_u16(ks_at + half + 8 * w));
+          const uint32_t x1 = decode_scales(lds_u16(ks_at + half + D / 2 + 8 * w));
+          s0[2 * w] = __byte_perm(x0, 0, 0x1010);
+          s0[2 * w + 1] = __byte_perm(x0, 0, 0x3232);
+          s1[2 * w] = __byte_perm(x1, 0, 0x1010);
+          s1[2 * w + 1] = __byte_perm(x1, 0, 0x3232);
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < kKWords; ++w) {
+        uint32_t d0[4], d1[4];
+        decode8(k0[w], d0);
+        decode8(k1[w], d1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          d0[j] = hmul2(d0[j], s0[w / 2]);
+          d1[j] = hmul2(d1[j], s1[w / 2]);
+        }
+        uint4 qv[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) qv[n] = qs[(n * kKWords + w) * 32 + lane];
+        // products into the same sums stand apart
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816(s[n], d0[0], d1[0], d0[1], d1[1], qv[n].x, qv[n].y);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816(s[n], d0[2], d1[2], d0[3], d1[3], qv[n].z, qv[n].w);
+      }
+      // a marked row (255) has codes of zero: its score is 0 * infinity here
+      kq[0] = __uint_as_float(lds_u8(ke_at + half) << 23) * q_scale;
+      kq[1] = __uint_as_float(lds_u8(ke_at + half + 8) << 23) * q_scale;
+    };
+    if (piece0 < last_cached) {
+      cp_wait<1>();
+      __syncwarp();
+      scores(0);
+    }
+    for (int p = piece0; p < last_cached; ++p) {
+      const uint32_t half = ((p - piece0) & 1) * kHalfRing;
+      cp_wait<0>();  // V of this tile and K of the next
+      __syncwarp();
+      const int key0 = 64 * p + 16 * warp;
       if (live_now < 16) {
         // rows that were never written may have scales that are not numbers: their weights are zero,
         // their values have to be finite
         for (int i = lane; i < D / 4; i += 32) {
           const int keep = live_now - 4 * (i & 3);  // bytes of the word that are of keys
-          const uint32_t at = stage + half + P::kVs + 4 * i;
+          const uint32_t at = v_ring + warp * P::kStage + half + P::kScales + 4 * i;
           uint32_t v[1];
           lds_words<1>(at, v);
           sts32(at, keep <= 0 ? 0u : keep >= 4 ? v[0] : v[0] & ((1u << (8 * keep)) - 1u));
         }
       }
-      if (live_now > 0) {
-        uint32_t k0[kKWords], k1[kKWords], s0[kKWords / 2], s1[kKWords / 2];  // keys r and r + 8
-        lds_words<D == 256 ? 4 : kKWords>(k_at + half, k0);
-        lds_words<D == 256 ? 4 : kKWords>(k_at + half + 4 * D, k1);
-        if constexpr (D == 256) {
-          lds_words<4>(k_at + half + 64, k0 + 4);
-          lds_words<4>(k_at + half + 4 * D + 64, k1 + 4);
-        }
-        if constexpr (D == 64) {
-          s0[0] = decode_scales(lds_u8(ks_at + half) * 0x101u);
-          s1[0] = decode_scales(lds_u8(ks_at + half + D / 2) * 0x101u);
-        } else {
-#pragma unroll
-          for (int w = 0; w < kKWords / 4; ++w) {
-            const uint32_t x0 = decode_scales(lds_u16(ks_at + half + 8 * w));
-            const uint32_t x1 = decode_scales(lds_u16(ks_at + half + D / 2 + 8 * w));
-            s0[2 * w] = __byte_perm(x0, 0, 0x1010);
-            s0[2 * w + 1] = __byte_perm(x0, 0, 0x3232);
-            s1[2 * w] = __byte_perm(x1, 0, 0x1010);
-            s1[2 * w + 1] = __byte_perm(x1, 0, 0x3232);
-          }
-        }
-#pragma unroll
-        for (int w = 0; w < kKWords; ++w) {
-          uint32_t d0[4], d1[4];
-          decode8(k0[w], d0);
-          decode8(k1[w], d1);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            d0[j] = hmul2(d0[j], s0[w / 2]);
-            d1[j] = hmul2(d1[j], s1[w / 2]);
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint4 qv = qs[(n * kKWords + w) * 32 + lane];
-            mma16816(s[n], d0[0], d1[0], d0[1], d1[1], qv.x, qv.y);
-            mma16816(s[n], d0[2], d1[2], d0[3], d1[3], qv.z, qv.w);
-          }
-        }
-      }
-      // a marked row (255) has codes of zero: its score is 0 * infinity here
-      const float kq[2] = {__uint_as_float(lds_u8(e_at + half) << 23) * q_scale,
-                           __uint_as_float(lds_u8(e_at + half + 8) << 23) * q_scale};
-      const float ev[2] = {exponent(lds_u8(e_at + half + P::kVe - P::kKe)),
-                           exponent(lds_u8(e_at + half + P::kVe - P::kKe + 8))};
+      const float ev[2] = {exponent(lds_u8(ve_at + half)), exponent(lds_u8(ve_at + half + 8))};
       auto masked = [&](int n, int j) {
         const int key = r + 8 * (j >> 1);
         return key >= live_now || key0 + key >= limit[n][j & 1];
       };
       weigh(s, kq, ev, live_now < 16 || key0 + 16 > first_limit, masked, [&] {
-        if (p + 1 < last_cached) {
-          live_next = load(p + 1, 4 * P::kStage - half);
-          if (p + 2 < last_cached) look(p + 2);
-        }
+        load_v(p + 1, id_v, kHalfRing - half);
+        live_after = load_k(p + 2, id_k, half);
         cp_commit();
+        id_v = id_k;
+        id_k = look(p + 3);
       });
+      // the next tile's scores beside this one's values: they have nothing to do with each other, and behind
+      // the last tile the former are of whatever lies there and not used
+      scores(kHalfRing - half);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t at = half + i * P::kStage;
@@ -343,6 +358,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
         }
       }
       live_now = live_next;
+      live_next = live_after;
     }
     cp_wait<0>();
 
@@ -352,7 +368,6 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
       if (64 * (p - seq.cached) >= seq.own) break;         // a unit without any key has one empty piece
       const uint16_t* k_base = a.k_own + b * a.sk_b + kvh * a.sk_h;
       const uint16_t* v_base = a.v_own + b * a.sv_b + kvh * a.sv_h;
-      float s[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -415,7 +430,8 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
           mma16816(s[n], d[0][2], d[1][2], d[0][3], d[1][3], qv.z, qv.w);
         }
       }
-      const float kq[2] = {power_of(-up_k[0]) * q_scale, power_of(-up_k[1]) * q_scale};
+      kq[0] = power_of(-up_k[0]) * q_scale;
+      kq[1] = power_of(-up_k[1]) * q_scale;
       const float ev[2] = {-(float)up_v[0], -(float)up_v[1]};
       weigh(s, kq, ev, true, [&](int, int j) { return key0 + r + 8 * (j >> 1) >= seq.own; }, [] {});
 #pragma unroll
