@@ -1,9 +1,9 @@
 // The 4-bit cache's writes, reads and page moves (layout: kv4.cuh).
 //
-// append: a row of D values is D/8 lanes x 8 values (one 16-byte load each). The row's power of
-// two comes from the exponent bits of its largest magnitude, a group's scale from the two lanes
-// that hold its 16 channels; all of it is exact fp32 arithmetic but the two roundings to e4m3 and
-// e2m1 that the format is.
+// append: a row of D values is D/8 lanes x 8 values (one 16-byte load each), a lane takes a token's K
+// and its V. The row's power of two comes from the exponent bits of its largest magnitude, a group's
+// scale from the two lanes that hold its 16 channels; all of it is exact but the two roundings to e4m3
+// and e2m1 that the format is.
 // read: a lane turns one 4-byte word of codes into eight 16-bit values (one 16-byte store).
 // move: pages are contiguous, so a move is a copy; a second set of CTAs rewrites the tables in
 // the same launch.
@@ -51,33 +51,18 @@ __device__ __forceinline__ float round17(float x) {
   return __uint_as_float((__float_as_uint(x) + 0x40u) & 0xFFFFFF80u);
 }
 
-// grid: (groups of tokens, kv head, K or V); a row of D values is D/8 lanes
+// One row's codes of a lane's eight values, its group's scale and the row's exponent byte.
+struct Coded {
+  uint32_t codes, scale, exponent;
+};
+
 template <int D, bool BF>
-__global__ void __launch_bounds__(kThreads) append_kernel(uint8_t* __restrict__ pool, int64_t page_bytes, int64_t pages,
-                                                          int page_shift, const uint16_t* __restrict__ k, int64_t sk_t,
-                                                          int64_t sk_h, const uint16_t* __restrict__ v, int64_t sv_t,
-                                                          int64_t sv_h, const int64_t* __restrict__ slots, int64_t n,
-                                                          int* err) {
+__device__ __forceinline__ Coded quantise(const uint4 raw) {
   constexpr int kLanes = D / 8;
-  const int sub = threadIdx.x % kLanes;
-  const int head = blockIdx.y;
-  const bool is_v = blockIdx.z;
-  int64_t tok = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
-  bool live = tok < n;  // every lane stays for the shuffles
-  tok = live ? tok : 0;
-  const uint16_t* src = is_v ? v + tok * sv_t + head * sv_h : k + tok * sk_t + head * sk_h;
-  const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src) + sub);
-  const int64_t slot = __ldg(slots + tok);
-  const int64_t page = slot >> page_shift;
-  live = live && slot >= 0;
-  if (live && page >= pages) {
-    if (sub == 0) d3b::record_device_error(err, kSiteBadSlot);
-    live = false;
-  }
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
   // largest magnitude as bits: ordered like the values, and a NaN or infinity is the largest
-  uint32_t top2 = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu),
-                           __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
+  const uint32_t top2 = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu),
+                                 __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
   uint32_t group = max(top2 & 0xFFFFu, top2 >> 16);
   group = max(group, __shfl_xor_sync(0xffffffffu, group, 1));
   uint32_t most = group;
@@ -88,8 +73,10 @@ __global__ void __launch_bounds__(kThreads) append_kernel(uint8_t* __restrict__ 
   const uint32_t bits = __float_as_uint(widen<BF>(most));
   const int e = max((int)(bits >> 23) - 127 - 11 + ((bits & 0x7FFFFFu) > 0x280000u ? 1 : 0), kExpMin);
   const float down = __uint_as_float((uint32_t)(127 - e) << 23);  // e in [-64, 117]
-  const uint32_t scale_byte = bad ? 0u : to_e4m3(round17(widen<BF>(group) * down * (1.0f / 6.0f)));
-  const float scale = __half2float(__ushort_as_half((unsigned short)(decode_scales(scale_byte) & 0xFFFFu)));
+  Coded c;
+  c.scale = bad ? 0u : to_e4m3(round17(widen<BF>(group) * down * (1.0f / 6.0f)));
+  c.exponent = bad ? 255u : (uint32_t)(e + 127);
+  const float scale = __half2float(__ushort_as_half((unsigned short)(decode_scales(c.scale) & 0xFFFFu)));
   const float by = scale > 0.f ? __frcp_rn(scale) * down : 0.f;
   float x[8];
 #pragma unroll
@@ -97,19 +84,48 @@ __global__ void __launch_bounds__(kThreads) append_kernel(uint8_t* __restrict__ 
     x[2 * i] = round17(widen<BF>(w[i] & 0xFFFFu) * by);
     x[2 * i + 1] = round17(widen<BF>(w[i] >> 16) * by);
   }
-  if (bad) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  c.codes = bad ? 0u : to_e2m1x8(x);  // a NaN times zero is not zero
+  return c;
+}
+
+// grid: (groups of tokens, kv head); D/8 lanes take a token's K row and its V row
+template <int D, bool BF>
+__global__ void __launch_bounds__(kThreads) append_kernel(uint8_t* __restrict__ pool, int64_t page_bytes, int64_t pages,
+                                                          int page_shift, const uint16_t* __restrict__ k, int64_t sk_t,
+                                                          int64_t sk_h, const uint16_t* __restrict__ v, int64_t sv_t,
+                                                          int64_t sv_h, const int64_t* __restrict__ slots, int64_t n,
+                                                          int* err) {
+  constexpr int kLanes = D / 8;
+  const int sub = threadIdx.x % kLanes;
+  const int head = blockIdx.y;
+  int64_t tok = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  bool live = tok < n;  // every lane stays for the shuffles
+  tok = live ? tok : 0;
+  const uint4 k_raw = __ldg(reinterpret_cast<const uint4*>(k + tok * sk_t + head * sk_h) + sub);
+  const uint4 v_raw = __ldg(reinterpret_cast<const uint4*>(v + tok * sv_t + head * sv_h) + sub);
+  const int64_t slot = __ldg(slots + tok);
+  const int64_t page = slot >> page_shift;
+  live = live && slot >= 0;
+  if (live && page >= pages) {
+    if (sub == 0) d3b::record_device_error(err, kSiteBadSlot);
+    live = false;
   }
-  const uint32_t codes = to_e2m1x8(x);
+  const Coded ck = quantise<D, BF>(k_raw), cv = quantise<D, BF>(v_raw);
   if (!live) return;
   const int in_page = (int)slot & ((1 << page_shift) - 1);
-  const int t = in_page & 15;
-  uint8_t* g = pool + page * page_bytes + ((head << (page_shift - 4)) + (in_page >> 4)) * (int64_t)granule_bytes(D) +
-               (is_v ? off_v(D) : 0);
-  reinterpret_cast<uint32_t*>(g + t * (D / 2))[sub] = codes;
-  if (!(sub & 1)) g[off_k_scale(D) + (is_v ? (sub >> 1) * 16 + t : t * (D / 16) + (sub >> 1))] = (uint8_t)scale_byte;
-  if (sub == 0) g[off_k_exp(D) + t] = (uint8_t)(bad ? 255 : e + 127);
+  const int t = in_page & 15, group = sub >> 1;
+  uint8_t* g = pool + page * page_bytes + ((head << (page_shift - 4)) + (in_page >> 4)) * (int64_t)granule_bytes(D);
+  uint8_t* codes = g + t * (D / 2) + 4 * sub;
+  *reinterpret_cast<uint32_t*>(codes) = ck.codes;
+  *reinterpret_cast<uint32_t*>(codes + off_v(D)) = cv.codes;
+  if (!(sub & 1)) {
+    g[off_k_scale(D) + t * (D / 16) + group] = (uint8_t)ck.scale;
+    g[off_v(D) + off_k_scale(D) + group * 16 + t] = (uint8_t)cv.scale;
+  }
+  if (sub == 0) {
+    g[off_k_exp(D) + t] = (uint8_t)ck.exponent;
+    g[off_v(D) + off_k_exp(D) + t] = (uint8_t)cv.exponent;
+  }
 }
 
 // eight values of one word of codes; `power` finite or NaN, `most` the magnitude that may not be passed
@@ -242,7 +258,7 @@ int launch_append(const d3b_kv4_cache* c, int64_t layer, const void* k, const in
                   const int64_t* vs, const int64_t* slots, int64_t n, bool bf, int* err, cudaStream_t s) {
   const int64_t per = kThreads / (D / 8), ctas = (n + per - 1) / per;
   if (ctas > 0x7FFFFFFF) return D3B_EINVAL;
-  const dim3 grid((unsigned)ctas, (unsigned)c->kv_heads, 2);
+  const dim3 grid((unsigned)ctas, (unsigned)c->kv_heads);
   auto* kp = static_cast<const uint16_t*>(k);
   auto* vp = static_cast<const uint16_t*>(v);
   const int shift = log2_of(c->page_tokens);

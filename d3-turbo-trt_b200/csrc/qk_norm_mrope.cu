@@ -68,13 +68,6 @@ __global__ void __launch_bounds__(32 * kWarps) qk_norm_mrope_kernel(
   const int last = min(first + run, passes);
   const uint16_t* q_row = q + r * sq_r + t * sq_t;
   const uint16_t* k_row = k + r * sk_r + t * sk_t;
-  auto fetch = [&](int p) {
-    const bool is_k = p >= q_passes;
-    const int h = (is_k ? p - q_passes : p) * kHeads + lane / kLanes;
-    if (p >= last || h >= (is_k ? k_heads : q_heads)) return make_uint4(0, 0, 0, 0);
-    return __ldg(reinterpret_cast<const uint4*>(is_k ? k_row + h * sk_h : q_row + h * sq_h) + sub);
-  };
-  uint4 next = fetch(first), after = fetch(first + 1);
   for (int i = lane; i < half; i += 32) {
     const double turns =
         (double)__ldg(pos + axis.of[i] * sp_a + r * sp_r + t * sp_t) * (double)__ldg(inv_freq + i) *
@@ -94,53 +87,59 @@ __global__ void __launch_bounds__(32 * kWarps) qk_norm_mrope_kernel(
     cs[i] = x.x;
     sn[i] = low ? -x.y : x.y;
   }
-  float w1[8];
-  int weights = -1;  // whose they are
-  for (int p = first; p < last; ++p) {
-    const bool is_k = p >= q_passes;
-    const uint4 raw = next;
-    next = after;
-    after = fetch(p + 2);
-    if (weights != (int)is_k) {
-      weights = is_k;
-      const uint4 wraw = __ldg(reinterpret_cast<const uint4*>(is_k ? wk : wq) + sub);
-      const uint32_t wr[4] = {wraw.x, wraw.y, wraw.z, wraw.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = widen2<BF>(wr[i]);
-        w1[2 * i] = 1.f + f.x;
-        w1[2 * i + 1] = 1.f + f.y;
-      }
-    }
-    const uint32_t xr[4] = {raw.x, raw.y, raw.z, raw.w};
-    float y[8], ss = 0.f;
+  // passes p0 .. p1 of one tensor's heads
+  auto turn = [&](const uint16_t* row, int64_t s_h, uint16_t* out, int heads, const uint16_t* weight, int p0, int p1) {
+    if (p0 >= p1) return;
+    const int h0 = p0 * kHeads + lane / kLanes;
+    int left = (heads - h0 + kHeads - 1) / kHeads;  // this lane's heads from p0 on
+    left = min(left, p1 - p0);
+    const uint4* src = reinterpret_cast<const uint4*>(row + h0 * s_h) + sub;
+    uint4* dst = reinterpret_cast<uint4*>(out + (int64_t)h0 * D) + sub;
+    const int64_t step = kHeads * s_h / 8;
+    auto fetch = [&](int i) { return i < left ? __ldg(src + i * step) : make_uint4(0, 0, 0, 0); };
+    uint4 next = fetch(0), after = fetch(1);
+    float w1[8];
+    const uint4 wraw = __ldg(reinterpret_cast<const uint4*>(weight) + sub);
+    const uint32_t wr[4] = {wraw.x, wraw.y, wraw.z, wraw.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 f = widen2<BF>(xr[i]);
-      y[2 * i] = f.x;
-      y[2 * i + 1] = f.y;
-      ss = fmaf(f.x, f.x, ss);
-      ss = fmaf(f.y, f.y, ss);
+      const float2 f = widen2<BF>(wr[i]);
+      w1[2 * i] = 1.f + f.x;
+      w1[2 * i + 1] = 1.f + f.y;
     }
+    for (int i = 0; i < p1 - p0; ++i) {
+      const uint4 raw = next;
+      next = after;
+      after = fetch(i + 2);
+      const uint32_t xr[4] = {raw.x, raw.y, raw.z, raw.w};
+      float y[8], ss = 0.f;
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float rs = rsqrtf(ss * (1.0f / D) + eps);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] *= rs * w1[i];
-    if (shift > 0) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float z = __shfl_sync(0xffffffffu, y[i], partner);
-        y[i] = fmaf(y[i], cs[i], z * sn[i]);
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = widen2<BF>(xr[j]);
+        y[2 * j] = f.x;
+        y[2 * j + 1] = f.y;
+        ss = fmaf(f.x, f.x, ss);
+        ss = fmaf(f.y, f.y, ss);
       }
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float rs = rsqrtf(ss * (1.0f / D) + eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] *= rs * w1[j];
+      if (shift > 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float z = __shfl_sync(0xffffffffu, y[j], partner);
+          y[j] = fmaf(y[j], cs[j], z * sn[j]);
+        }
+      }
+      if (i < left)
+        dst[i * (kHeads * D / 8)] = make_uint4(pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3]), pack2<BF>(y[4], y[5]),
+                                               pack2<BF>(y[6], y[7]));
     }
-    const int h = (is_k ? p - q_passes : p) * kHeads + lane / kLanes;
-    if (h < (is_k ? k_heads : q_heads)) {
-      uint16_t* dst = is_k ? k_out + (rt * k_heads + h) * D : q_out + (rt * q_heads + h) * D;
-      reinterpret_cast<uint4*>(dst)[sub] = make_uint4(pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3]),
-                                                      pack2<BF>(y[4], y[5]), pack2<BF>(y[6], y[7]));
-    }
-  }
+  };
+  turn(q_row, sq_h, q_out + rt * q_heads * D, q_heads, wq, min(first, q_passes), min(last, q_passes));
+  turn(k_row, sk_h, k_out + rt * k_heads * D, k_heads, wk, max(first - q_passes, 0), last - q_passes);
 }
 
 }  // namespace

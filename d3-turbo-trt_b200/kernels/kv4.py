@@ -61,6 +61,12 @@ def _index(t: torch.Tensor, dtype: torch.dtype, device: torch.device, what: str)
         raise RuntimeError(f"{what} must be {dtype} on {device}, got {t.dtype} on {t.device}")
 
 
+@functools.lru_cache(maxsize=256)
+def _plans_of(kv_heads: int, head_dim: int, page_tokens: int, device: torch.device) -> dict:
+    """Checked calls on caches of one shape, by what the checks look at: shapes, strides, types, devices."""
+    return {}
+
+
 class Kv4Cache:
     """``pool`` [layers, pages, page_bytes] uint8, allocated here or, with ``over``, the caller's."""
 
@@ -94,7 +100,7 @@ class Kv4Cache:
         self.device = pool.device
         self._c = _lib.Kv4CacheStruct(pool.data_ptr(), self.layers, self.pages, kv_heads, head_dim, page_tokens)
         self._ref = ctypes.byref(self._c)
-        self._plans: dict = {}  # checked calls, by what the checks look at: shapes, strides, types, devices
+        self._plans = _plans_of(kv_heads, head_dim, page_tokens, self.device)
 
     @property
     def nbytes(self) -> int:
@@ -128,8 +134,7 @@ class Kv4Cache:
         ``slots`` [n] int64 on the device; a negative slot leaves its row out. Slots must differ: one
         that is named twice holds a mixture of the rows."""
         self._check_layer(layer)
-        key = (append_key, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, slots.shape,
-               slots.dtype, slots.device)
+        key = (append_key, k.shape, k.dtype, k.device, v.shape, v.dtype, v.device, slots.shape, slots.dtype, slots.device)
         n, code, index, fn = self._plan(key, lambda: self._plan_append(k, v, slots))
         if n == 0:
             return
@@ -360,5 +365,5 @@ def _plan_question(q: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, state_
 
 def _reads_codes(rows: int, heads: int, kv_heads: int, width: int, state_len: int, dim: int) -> bool:
     """Whether a question batch is small enough to read the state's codes in place."""
-    return _ROUTE
-_ROUTE = True
+    tiles = rows * kv_heads * -(-width * (heads // kv_heads) // 32)
+    return tiles * -(-(state_len + width) // 64) < 8000
