@@ -68,25 +68,29 @@ __global__ void __launch_bounds__(32 * kWarps) qk_norm_mrope_kernel(
   const int last = min(first + run, passes);
   const uint16_t* q_row = q + r * sq_r + t * sq_t;
   const uint16_t* k_row = k + r * sk_r + t * sk_t;
-  for (int i = lane; i < half; i += 32) {
-    const double turns =
-        (double)__ldg(pos + axis.of[i] * sp_a + r * sp_r + t * sp_t) * (double)__ldg(inv_freq + i) *
-        0.15915494309189533577;  // 1 / (2 pi)
-    float s, c;
-    sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-    table[warp][i] = make_float2(c, s);
-  }
-  __syncwarp();
   const int shift = half / 8;  // lanes to the rotary partner
   const bool low = sub < shift, turned = sub < 2 * shift;
   const int partner = lane - sub + (turned ? (low ? sub + shift : sub - shift) : sub);
   float cs[8], sn[8];
+  bool ready = false;
+  auto make_table = [&] {
+    for (int i = lane; i < half; i += 32) {
+      const double turns =
+          (double)__ldg(pos + axis.of[i] * sp_a + r * sp_r + t * sp_t) * (double)__ldg(inv_freq + i) *
+          0.15915494309189533577;  // 1 / (2 pi)
+      float s, c;
+      sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+      table[warp][i] = make_float2(c, s);
+    }
+    __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 x = turned ? table[warp][8 * (low ? sub : sub - shift) + i] : make_float2(1.f, 0.f);
-    cs[i] = x.x;
-    sn[i] = low ? -x.y : x.y;
-  }
+    for (int i = 0; i < 8; ++i) {
+      const float2 x = turned ? table[warp][8 * (low ? sub : sub - shift) + i] : make_float2(1.f, 0.f);
+      cs[i] = x.x;
+      sn[i] = low ? -x.y : x.y;
+    }
+    ready = true;
+  };
   // passes p0 .. p1 of one tensor's heads
   auto turn = [&](const uint16_t* row, int64_t s_h, uint16_t* out, int heads, const uint16_t* weight, int p0, int p1) {
     if (p0 >= p1) return;
@@ -98,6 +102,7 @@ __global__ void __launch_bounds__(32 * kWarps) qk_norm_mrope_kernel(
     const int64_t step = kHeads * s_h / 8;
     auto fetch = [&](int i) { return i < left ? __ldg(src + i * step) : make_uint4(0, 0, 0, 0); };
     uint4 next = fetch(0), after = fetch(1);
+    if (!ready) make_table();  // while the first rows are on their way
     float w1[8];
     const uint4 wraw = __ldg(reinterpret_cast<const uint4*>(weight) + sub);
     const uint32_t wr[4] = {wraw.x, wraw.y, wraw.z, wraw.w};
