@@ -1146,6 +1146,10 @@ __global__ void __launch_bounds__(DU_THREADS, 1)
           }
           if (j > 0) m_prev = mref_s[(t - 1) & 1][r];
         }
+        // P[wg] is free once PV(t-2) has completed. Waited for before mdone(t) is published: tile t+1 waits
+        // for PV(t) on this same barrier if it rescales O, and a parity wait holds only where the phase
+        // before it, PV(t-2)'s, is known to have completed.
+        if (!d3b::warp_wait(&bars.p_free[wg], (u & 1) ^ 1, abort_flag, p.err, kSiteDuPFree)) { ok = false; break; }
         // Lazy rescale, decided per warp: tcgen05.ld/st are warp-collective.
         const bool rescale = __any_sync(0xffffffffu, m_tile > m_prev + kRescaleThreshold);
         const float m_new = rescale ? fmaxf(m_prev, m_tile) : m_prev;
@@ -1161,8 +1165,6 @@ __global__ void __launch_bounds__(DU_THREADS, 1)
           d3b::tc_fence_after();
           scale_cols<D>(lane_addr + C::COL_O, d3b::ex2_approx(m_prev - m_new));
         }
-        // P[wg] is free once PV(t-2) has completed
-        if (!d3b::warp_wait(&bars.p_free[wg], (u & 1) ^ 1, abort_flag, p.err, kSiteDuPFree)) { ok = false; break; }
         d3b::tc_fence_after();
         float rowsum = 0.f;
 #pragma unroll
@@ -1643,6 +1645,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DU_THREADS, 1)
           }
           if (j > 0) m_prev = mref_s[(t - 1) & 1][r];
         }
+        // before mdone(t): tile t+1's wait for PV(t) needs PV(t-2)'s phase completed (see the dual kernel)
+        if (!d3b::warp_wait(&bars.p_free[wg], (u & 1) ^ 1, abort_flag, p.err, kSiteDuPFree)) { ok = false; break; }
         const bool rescale = __any_sync(0xffffffffu, m_tile > m_prev + kRescaleThreshold);
         const float m_new = rescale ? fmaxf(m_prev, m_tile) : m_prev;
         mref_s[wg][r] = m_new;
@@ -1656,7 +1660,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DU_THREADS, 1)
           d3b::tc_fence_after();
           scale_cols<D>(lane_addr + C::COL_O, d3b::ex2_approx(m_prev - m_new));
         }
-        if (!d3b::warp_wait(&bars.p_free[wg], (u & 1) ^ 1, abort_flag, p.err, kSiteDuPFree)) { ok = false; break; }
         d3b::tc_fence_after();
         float rowsum = 0.f;
 #pragma unroll
