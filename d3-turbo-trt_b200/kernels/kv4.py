@@ -198,6 +198,8 @@ class Kv4Cache:
     def _move(self, src, dst, tables) -> None:
         if not isinstance(src, torch.Tensor) and not isinstance(dst, torch.Tensor):
             src, dst = [int(p) for p in src], [int(p) for p in dst]
+            if len(src) != len(dst):
+                raise RuntimeError(f"{len(src)} pages to {len(dst)}")
             if len(set(src) | set(dst)) < len(set(src)) + len(dst):
                 raise RuntimeError("a destination is a source or stands twice")
             if tables is not None and any(a >= b for a, b in zip(src, src[1:])):
@@ -363,7 +365,29 @@ def _plan_question(q: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, state_
     return rows, heads, width, _TYPES[q.dtype], cache.device.index, need, lib.d3b_kv4_question
 
 
+# What the two ways of a question batch cost on B200, in us, by head_dim (fitted to 190 measured shapes,
+# 1 to 255 blocks of 3 to 48 tokens over 64 to 16384; off by a quarter at most where the two are near).
+# In place: a start, a piece of 32 rows x 64 keys of a CTA (296 run), the first pieces' share of the
+# merge. Widened: the state's read and a start, a 128-key tile of a unit of 128 rows, and a
+# floor and a slope for few units, whose keys that kernel splits.
+_IN_PLACE = {64: (7.0, 1.1, 1.5), 128: (7.5, 1.47, 3.0), 256: (9.5, 2.13, 5.0)}
+_WIDENED = {64: (9.4, 0.8, 21.0, 0.0), 128: (9.4, 0.87, 24.0, 0.03), 256: (9.4, 1.55, 18.0, 0.33)}
+
+
 def _reads_codes(rows: int, heads: int, kv_heads: int, width: int, state_len: int, dim: int) -> bool:
-    """Whether a question batch is small enough to read the state's codes in place."""
-    tiles = rows * kv_heads * -(-width * (heads // kv_heads) // 32)
-    return tiles * -(-(state_len + width) // 64) < 8000
+    """Whether a question batch is faster reading the state's codes in place than widening the state first
+    and running ``prefix_bidir_attention``'s kernel. For instance 32 query and 4 kv heads of 128 over 4096
+    tokens: one block of 12 tokens 22 against 36 us, 4 blocks of 12 36 against 36, 16 blocks of 12 89
+    against 37."""
+    group = heads // kv_heads
+    pieces = -(-state_len // 64) + -(-width // 64)
+    share = -(-(rows * kv_heads * -(-width * group // 32) * pieces) // 296)
+    start, piece, first = _IN_PLACE[dim]
+    in_place = start + piece * share + first * min(share, 3) + 8 * (share - 1) / pieces
+    units, tiles = rows * kv_heads * -(-width * group // 128), -(-(state_len + width) // 128)
+    start, tile, floor, slope = _WIDENED[dim]
+    if units <= 148:
+        widened = start + max(min(tile * tiles, floor + slope * tiles), 1.2 * tile * tiles * units / 148)
+    else:
+        widened = start + -(-units // 148) * (3.4 + tile * tiles)
+    return in_place < widened

@@ -403,6 +403,69 @@ def test_question(dim, heads, kv_heads, page, dtype, B, L, state):
     assert _lib.device_error() == 0
 
 
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("dim,heads,kv_heads,B,L,state", [(64, 12, 3, 4, 70, 200), (128, 32, 4, 2, 33, 1000), (128, 7, 1, 9, 1, 129),
+                                                          (256, 24, 4, 3, 8, 640), (256, 2, 2, 40, 5, 63)])
+def test_question_both_ways(monkeypatch, in_place, dim, heads, kv_heads, B, L, state):
+    """Either way of reading the state, whatever the sizes would choose: lengths on the device, strided operands,
+    keys of the block behind several tiles of the state, and an output of another layout."""
+    monkeypatch.setattr(kv4, "_reads_codes", lambda *a: in_place)
+    cache, table, kept = filled([state], kv_heads, dim, 32, BF, seed=L)
+    cache._plans.clear()
+    q = rows((B, L, heads, dim), BF, 1, 0.2).transpose(1, 2)
+    both = rows((B, L, 2, kv_heads, dim), BF, 2, 0.2)
+    k, v = both[:, :, 0].transpose(1, 2), both[:, :, 1].transpose(1, 2)
+    dev = both.cuda()
+    lengths = [(L + 5 * b) % (L + 1) for b in range(B)]
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    out = torch.full((B, L, heads, dim), 3.0, dtype=BF, device="cuda").transpose(1, 2)
+    got = kv4.question_attention(q.cuda(), cache, 0, table[0], state, dev[:, :, 0].transpose(1, 2), dev[:, :, 1].transpose(1, 2),
+                                 lens, scale=dim**-0.5, out=out)
+    assert got is out
+    check_question(got, q, kept[0], k, v, lengths, dim**-0.5, BF)
+    assert _lib.device_error() == 0
+    lens[0] = L + 1  # clamped to L and recorded
+    again = kv4.question_attention(q.cuda(), cache, 0, table[0], state, dev[:, :, 0].transpose(1, 2), dev[:, :, 1].transpose(1, 2),
+                                   lens, scale=dim**-0.5)
+    check_question(again, q, kept[0], k, v, [L] + lengths[1:], dim**-0.5, BF)
+    assert _lib.device_error() == 2010
+    cache._plans.clear()
+
+
+def test_question_refuses():
+    cache = new_cache(4, 2, 64, 16)
+    table = torch.arange(4, dtype=torch.int32, device="cuda")
+    q, k = torch.zeros(2, 4, 3, 64, dtype=BF, device="cuda"), torch.zeros(2, 2, 3, 64, dtype=BF, device="cuda")
+    ask = lambda **kw: kv4.question_attention(**(dict(q=q, cache=cache, layer=0, table=table, state_len=60, k_q=k, v_q=k,  # noqa: E731
+                                                      lengths=[3, 2], scale=0.1) | kw))
+    ask()
+    for kw in (dict(state_len=65), dict(state_len=-1), dict(layer=1), dict(lengths=[3]), dict(lengths=[4, 0]), dict(lengths=[-1, 0]),
+               dict(q=q.float()), dict(q=q[:, :3]), dict(q=q[..., :32]), dict(k_q=k.half()), dict(v_q=k[:, :1]), dict(table=table.long()),
+               dict(table=table.cpu()), dict(table=table[None]), dict(out=q.float()), dict(q=q.cpu()), dict(scale=0.0)):
+        with pytest.raises(RuntimeError):
+            ask(**kw)
+    deq = lambda **kw: kv4.decode_attention(**(dict(q=q, cache=cache, layer=0, table=table.view(2, 2),  # noqa: E731
+                                                    lengths=table[:2], scale=0.1) | kw))
+    deq()
+    for kw in (dict(table=table), dict(table=table.view(1, 4)), dict(lengths=table[:1]), dict(lengths=table[:2].long()), dict(layer=-1),
+               dict(q=q[:, :3]), dict(q=q.float()), dict(q=q[..., :32]), dict(scale=-1.0), dict(out=q[:1]), dict(q=q[0, 0])):
+        with pytest.raises(RuntimeError):
+            deq(**kw)
+    app = lambda **kw: cache.append(**(dict(layer=0, k=k[:, :, 0], v=k[:, :, 0], slots=torch.zeros(2, dtype=torch.int64, device="cuda") - 1) | kw))  # noqa: E731
+    app()
+    for kw in (dict(layer=2), dict(k=k[:1, :, 0]), dict(v=k[:, :, 0].half()), dict(slots=torch.zeros(2, dtype=torch.int32, device="cuda")),
+               dict(slots=torch.zeros(3, dtype=torch.int64, device="cuda")), dict(k=k[:, :, 0].cpu())):
+        with pytest.raises(RuntimeError):
+            app(**kw)
+    for bad in (lambda: cache.read(0, table, 65), lambda: cache.read(0, table.long(), 5), lambda: cache.read(0, table, 5, dtype=torch.float32),
+                lambda: cache.copy_pages([0, 1], [1, 2]), lambda: cache.copy_pages([0, 1], [2, 2]), lambda: cache.copy_pages([0], [4]),
+                lambda: cache.copy_pages([0], [2, 3]), lambda: cache.move_pages([1, 0], [2, 3], table), lambda: cache.move_pages([0], [2], table.long()),
+                lambda: cache.slots([0, 1], 30, 3), lambda: kv4.Kv4Cache.over(cache.pool[:, :, 16:], kv_heads=2, head_dim=64, page_tokens=16)):
+        with pytest.raises(RuntimeError):
+            bad()
+    assert _lib.device_error() == 0
+
+
 def check_question(got, q, state, k, v, lengths, scale, dtype):
     got, dim = got.cpu().double(), q.shape[-1]
     for b, n in enumerate(lengths):
