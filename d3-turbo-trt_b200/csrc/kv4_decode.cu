@@ -6,16 +6,15 @@ namespace {
 
 using namespace d3b_kv4;
 
-constexpr int kMergeThreads = 256;
-
 // One CTA a query row: the parts of its unit, added in a fixed order. The parts' factors are worked
 // out first, a thread a part; then groups of D/4 threads add every kGroups-th part, then the groups in
-// turn. Launched before the attention kernel has finished; it waits for it here.
-template <int D, bool BF>
-__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_constant__ AttnArgs a, int tile_rows) {
-  constexpr int kGroups = kMergeThreads / (D / 4);
+// turn. THREADS is 64 where a unit has few parts (64 sequences of 16384 tokens: 2048 rows of 4 parts,
+// 1 us less) and 256 where it has many. Launched before the attention kernel has finished; it waits for it here.
+template <int D, int THREADS, bool BF>
+__global__ void __launch_bounds__(THREADS) merge_kernel(const __grid_constant__ AttnArgs a, int tile_rows) {
+  constexpr int kGroups = THREADS / (D / 4);
   __shared__ float4 part[kGroups][D / 4];
-  __shared__ float factor[kMergeThreads], tops[kMergeThreads / 32], sums[kMergeThreads / 32];
+  __shared__ float factor[THREADS], tops[THREADS / 32], sums[THREADS / 32];
   const int rows = a.group * a.L;
   const int row = blockIdx.x % rows, bk = blockIdx.x / rows;
   const int kvh = bk % a.kv_heads, b = bk / a.kv_heads;
@@ -26,18 +25,18 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
   // the unit's first CTA began it (slot 1), the others went on with it (slot 0)
   auto at = [&](int cta) { return (2 * (int64_t)cta + (cta == range.x)) * tile_rows + row % tile_rows; };
   float top = -INFINITY;
-  for (int c = range.x + t; c <= range.y; c += kMergeThreads) top = fmaxf(top, a.part_st[at(c) * 2]);
+  for (int c = range.x + t; c <= range.y; c += THREADS) top = fmaxf(top, a.part_st[at(c) * 2]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (t % 32 == 0) tops[t / 32] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kMergeThreads / 32; ++w) top = fmaxf(top, tops[w]);
+  for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, tops[w]);
   const float base = finite_or_zero(top);
   float sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c0 = range.x; c0 <= range.y; c0 += kMergeThreads) {
-    const int n = min(kMergeThreads, range.y + 1 - c0);
+  for (int c0 = range.x; c0 <= range.y; c0 += THREADS) {
+    const int n = min(THREADS, range.y + 1 - c0);
     __syncthreads();
     if (t < n) {
       const float2 st = *reinterpret_cast<const float2*>(a.part_st + at(c0 + t) * 2);
@@ -64,7 +63,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const __grid_const
   if (group) return;
   sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < kMergeThreads / 32; ++w) sum += sums[w];
+  for (int w = 0; w < THREADS / 32; ++w) sum += sums[w];
 #pragma unroll
   for (int g = 1; g < kGroups; ++g) {
     const float4 x = part[g][d4];
@@ -109,20 +108,25 @@ size_t plan_bytes(const Plan& p, int D) {
   return (size_t)p.ctas * 2 * 8 * p.nt * (D + 2) * 4 + (size_t)p.units * 8;
 }
 
-template <int D>
+template <int D, int THREADS>
 int launch_merge(const AttnArgs& a, int nt, bool bf, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.kv_heads * a.group * a.L));
-  cfg.blockDim = dim3(kMergeThreads);
+  cfg.blockDim = dim3(THREADS);
   cfg.stream = s;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = bf ? cudaLaunchKernelEx(&cfg, merge_kernel<D, true>, a, 8 * nt)
-                           : cudaLaunchKernelEx(&cfg, merge_kernel<D, false>, a, 8 * nt);
+  const cudaError_t e = bf ? cudaLaunchKernelEx(&cfg, merge_kernel<D, THREADS, true>, a, 8 * nt)
+                           : cudaLaunchKernelEx(&cfg, merge_kernel<D, THREADS, false>, a, 8 * nt);
   return e == cudaSuccess ? d3b_host::check_launch() : D3B_ECUDA;
+}
+
+template <int D>
+int launch_merge(const AttnArgs& a, const Plan& p, bool bf, cudaStream_t s) {
+  return p.ctas <= 6 * p.units ? launch_merge<D, 64>(a, p.nt, bf, s) : launch_merge<D, 256>(a, p.nt, bf, s);
 }
 
 int run(AttnArgs& a, const d3b_kv4_cache* c, const Plan& p, bool bf, void* workspace, cudaStream_t s) {
@@ -135,8 +139,8 @@ int run(AttnArgs& a, const d3b_kv4_cache* c, const Plan& p, bool bf, void* works
   a.ranges = reinterpret_cast<int2*>(a.part_st + (size_t)p.ctas * 2 * 8 * p.nt * 2);
   if (int rc = p.wide ? launch_wide(a, D, p.nt, bf, p.ctas, s) : launch_thin(a, D, p.nt, bf, p.ctas, s)) return rc;
   if (p.ctas == 1) return D3B_OK;  // nothing to merge
-  return D == 64 ? launch_merge<64>(a, p.nt, bf, s) : D == 128 ? launch_merge<128>(a, p.nt, bf, s)
-                                                                   : launch_merge<256>(a, p.nt, bf, s);
+  return D == 64 ? launch_merge<64>(a, p, bf, s) : D == 128 ? launch_merge<128>(a, p, bf, s)
+                                                                   : launch_merge<256>(a, p, bf, s);
 }
 
 int check_shape(const d3b_kv4_cache* c, int B, int H, int L, int64_t width) {
