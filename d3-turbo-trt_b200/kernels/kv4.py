@@ -309,7 +309,9 @@ def question_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torc
     state keys and values are the first ``state_len`` tokens of pages ``table`` [n] int32.
 
     q [B, H, L, D], k_q/v_q [B, H_kv, L, D], ``lengths`` as there. Returns [B, H, L, D], zero rows
-    for padding.
+    for padding. Small batches read the codes in place, larger ones widen the state first. A page outside
+    the pool or a device length outside [0, L] sets the device error word (2102, 2010) either way; in
+    place its tokens are left out or it is clamped, but a widened launch's results are void then.
     """
     cache._check_layer(layer)
     key = (question_attention, q.shape, q.dtype, q.device, k_q.shape, k_q.dtype, k_q.device, v_q.shape, v_q.dtype,
