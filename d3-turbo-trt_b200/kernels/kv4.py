@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 from typing import Sequence
 
 import torch
@@ -240,8 +241,8 @@ def _check_query(q: torch.Tensor, cache: Kv4Cache) -> None:
 
 def _check_out(out: torch.Tensor, q: torch.Tensor) -> None:
     if (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(-1) != 1
-            or out.data_ptr() % 16 or any(s % 8 for s in out.stride()[:-1])):
-        raise RuntimeError("out must be like q, with a contiguous last dimension and 16-byte aligned rows")
+            or out.data_ptr() % 16 or any(s % 8 or (s == 0 and n > 1) for s, n in zip(out.stride()[:-1], out.shape))):
+        raise RuntimeError("out must be like q, with a contiguous last dimension and 16-byte aligned rows of its own")
 
 
 def decode_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torch.Tensor, lengths: torch.Tensor, *,
@@ -251,7 +252,8 @@ def decode_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torch.
     q [B, H, L, D] (any strides, D contiguous) or [B, H, D] for one token each; ``table`` [B, width]
     int32 page numbers (entries behind a sequence's last page are not read); ``lengths`` [B] int32
     tokens in the cache, the L newest among them already appended. Every token sees all ``lengths[b]``
-    tokens, or with ``causal`` those up to itself. Rows without a key are zero. Returns a tensor like q.
+    tokens, or with ``causal`` those up to itself. Rows without a key are zero. ``scale`` must
+    be positive. Returns a tensor like q.
     """
     if q.dim() == 3:
         out = None if out is None else out.unsqueeze(2)
@@ -260,6 +262,8 @@ def decode_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torch.
            lengths.shape, lengths.stride(), lengths.dtype, lengths.device)
     rows, heads, width, code, index, need, fn = cache._plan(key, lambda: _plan_decode(q, cache, table, lengths))
     cache._check_layer(layer)
+    if not 0 < scale < math.inf:
+        raise RuntimeError(f"scale must be positive and finite, got {scale}")
     q = _lib.rows16(q)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -314,6 +318,8 @@ def question_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torc
     place its tokens are left out or it is clamped, but a widened launch's results are void then.
     """
     cache._check_layer(layer)
+    if not 0 < scale < math.inf:
+        raise RuntimeError(f"scale must be positive and finite, got {scale}")
     key = (question_attention, q.shape, q.dtype, q.device, k_q.shape, k_q.dtype, k_q.device, v_q.shape, v_q.dtype,
            v_q.device, table.shape, table.dtype, table.device, state_len)
     rows, heads, width, code, index, need, fn = cache._plan(key, lambda: _plan_question(q, cache, table, state_len, k_q, v_q))

@@ -163,6 +163,8 @@ class Kv4States:
         self._rows = list(range(max_states))
         self._held: dict[int, list[int]] = {}  # the pages of the states, by row; the snapshots share the lists
         self._lock = threading.RLock()
+        self._moving = False
+        self._dropped: list[int] = []  # rows whose snapshot went while the pages moved
 
     @staticmethod
     def pages_for(tokens: int, page_tokens: int = 64) -> int:
@@ -175,6 +177,9 @@ class Kv4States:
 
     def _drop(self, row: int) -> None:
         with self._lock:
+            if self._moving:  # a finaliser that ran inside compact(): this thread holds the lock already
+                self._dropped.append(row)
+                return
             self.pool.release(self._held.pop(row))
             heapq.heappush(self._rows, row)
 
@@ -215,11 +220,11 @@ class Kv4States:
             if pages is None:
                 return None
             snap = self._snapshot(snapshot, pages, tokens, 0)
-        if tokens:
-            slots = self.cache.slots(snap_table(snap), 0, tokens)
-            for layer, e in enumerate(entries):
-                self.cache.append(layer, e.keys[0].transpose(0, 1), e.values[0].transpose(0, 1), slots)
-        return snap
+            if tokens:
+                slots = self.cache.slots(snap_table(snap), 0, tokens)
+                for layer, e in enumerate(entries):
+                    self.cache.append(layer, e.keys[0].transpose(0, 1), e.values[0].transpose(0, 1), slots)
+            return snap
 
     def fork(self, snap: Kv4Snapshot) -> Kv4Snapshot | None:
         """A snapshot of the same state that can be extended by itself: its full pages are shared, a partly
@@ -238,7 +243,8 @@ class Kv4States:
     def extend(self, snap: Kv4Snapshot, count: int) -> torch.Tensor | None:
         """int64 slots of ``count`` new tokens of ``snap``, to append K/V to in every layer; its entries then
         have them. Only for a snapshot whose last page is its own (a stored one that was not forked since,
-        or a fork). None where no pages are free."""
+        or a fork). None where no pages are free. The slots are places in the pool: append before the next
+        ``compact``."""
         with self._lock:
             page = self.cache.page_tokens
             need = self.pages_for(snap.tokens + count, page)
@@ -263,12 +269,18 @@ class Kv4States:
         """Move the used pages to the front of the pool, in every layer and table, in one launch; how many
         moved."""
         with self._lock:
-            src, dst = self.pool.compact()
-            if src:
-                self.cache.move_pages(src, dst, self.tables)
-                to = dict(zip(src, dst))
-                for pages in self._held.values():
-                    pages[:] = [to.get(p, p) for p in pages]
+            self._moving = True
+            try:
+                src, dst = self.pool.compact()
+                if src:
+                    self.cache.move_pages(src, dst, self.tables)
+                    to = dict(zip(src, dst))
+                    for pages in self._held.values():
+                        pages[:] = [to.get(p, p) for p in pages]
+            finally:
+                self._moving = False
+                while self._dropped:
+                    self._drop(self._dropped.pop())
             return len(src)
 
 

@@ -295,6 +295,44 @@ def test_decode_strides_out_and_single():
     assert torch.allclose(one.float(), again.float(), atol=0.02, rtol=0.02)
 
 
+def test_attention_refuses_shared_output_rows_and_scales():
+    cache, table, _ = filled([20, 9], 1, 64, 16, BF, seed=3)
+    lens = torch.tensor([20, 9], dtype=torch.int32, device="cuda")
+    q = torch.zeros(2, 2, 1, 64, dtype=BF, device="cuda")
+    k = torch.zeros(2, 1, 1, 64, dtype=BF, device="cuda")
+    one = torch.zeros(1, 2, 1, 64, dtype=BF, device="cuda")
+    for kw in (dict(out=one.expand(2, 2, 1, 64)), dict(out=one[:, :1].expand(2, 2, 1, 64)), dict(scale=float("inf")),
+               dict(scale=float("nan")), dict(scale=0.0)):
+        kw = dict(scale=0.1) | kw
+        with pytest.raises(RuntimeError):
+            kv4.decode_attention(q, cache, 0, table, lens, **kw)
+        with pytest.raises(RuntimeError):
+            kv4.question_attention(q, cache, 0, table[0], 20, k, k, [1, 1], **kw)
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("L", [1, 18])  # both kernels
+def test_decode_many_short_sequences(L):
+    # 40000 sequences of 0 to 2 granules over 2 pages: thousands to a CTA, most of them without keys
+    dim, B = 64, 40000
+    cache, table, kept = filled([16, 16], 1, dim, 16, BF, seed=5)
+    pages = torch.tensor([int(table[0, 0]), int(table[1, 0])], dtype=torch.int32, device="cuda")
+    lens = (torch.arange(B, dtype=torch.int32, device="cuda") * 7919 % 131 - 98).clamp_(0, 32)
+    q = rows((1, L, 1, dim), BF, 6).transpose(1, 2)
+    out = kv4.decode_attention(q.cuda().expand(B, 1, L, dim), cache, 0, pages[None].expand(B, 2), lens, scale=0.1)
+    both = [torch.cat([kept[0][i], kept[1][i]], 1) for i in range(2)]
+    for n in range(33):
+        got = out[lens == n].cpu().double()
+        assert got.shape[0] > 100
+        if n == 0:
+            assert bool((got == 0).all())
+            continue
+        want, mass, top = ref.attention(q[0], both[0][:, :n], both[1][:, :n], 0.1)
+        bound = decode_bound(want, mass, top, n, float(both[1].abs().max()), dim, BF)
+        assert bool(((got - want).abs() <= bound).all()), n
+    assert _lib.device_error() == 0
+
+
 def test_decode_not_finite_rows_reach_only_their_readers():
     dim, n = 128, 40
     cache, table, kept = filled([n, n], 1, dim, 16, BF, seed=10)

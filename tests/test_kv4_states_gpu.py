@@ -95,6 +95,31 @@ def test_store_fork_extend_compact_question():
     assert _lib.device_error() == 0
 
 
+def test_a_snapshot_dropped_while_pages_move(monkeypatch):
+    # a finaliser may run inside compact() on the same thread: its pages must be those it has after the move
+    states = Kv4States(1, 8, kv_heads=1, head_dim=64, page_tokens=16, max_tokens=64, max_states=4)
+    snap, kept = make_snapshot(1, 1, 30, 64, 3)
+    held = [states.store(snap) for _ in range(3)]
+    held.pop(0)
+    gc.collect()
+    move = states.cache.move_pages
+
+    def moves(src, dst, tables):
+        held.pop()  # the one whose pages lie last
+        gc.collect()
+        move(src, dst, tables)
+
+    monkeypatch.setattr(states.cache, "move_pages", moves)
+    assert states.compact() == 2
+    assert states.pool.used == 2 and states.stats()["states"] == 1
+    monkeypatch.undo()
+    check_decode_entry(held[0][0], kept[0], rows((1, 2, 1, 64), BF, 9, 0.2), 0.1)
+    states.compact()
+    assert sorted(held[0].pages) == [0, 1]
+    check_decode_entry(held[0][0], kept[0], rows((1, 2, 1, 64), BF, 9, 0.2), 0.1)
+    assert states.store(snap) is not None and _lib.device_error() == 0
+
+
 def test_no_room_and_shared_last_page():
     # five pages: three of the state, one copied by its fork, one that the fork grows into
     states = Kv4States(1, 5, kv_heads=1, head_dim=64, page_tokens=16, max_tokens=64, max_states=2)
