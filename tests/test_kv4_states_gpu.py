@@ -15,6 +15,7 @@ from test_kv4_gpu import check_question, decode_bound, rows
 
 from d3_turbo_trt_b200 import _lib
 from d3_turbo_trt_b200.kernels import kv4
+from d3_turbo_trt_b200.model import fused
 from d3_turbo_trt_b200.model.backbone import BackboneConfig, D3Backbone
 from d3_turbo_trt_b200.model.cache import StateCache
 from d3_turbo_trt_b200.model.pages import Kv4Entry, Kv4States
@@ -118,6 +119,79 @@ def test_a_snapshot_dropped_while_pages_move(monkeypatch):
     assert sorted(held[0].pages) == [0, 1]
     check_decode_entry(held[0][0], kept[0], rows((1, 2, 1, 64), BF, 9, 0.2), 0.1)
     assert states.store(snap) is not None and _lib.device_error() == 0
+
+
+def test_a_captured_step_replayed():
+    # rotation, append and attention of one token of two sequences in a graph, run for four tokens, against eager calls
+    B, heads, kv_heads, dim, page, steps = 2, 6, 2, 128, 16, 4
+    table = torch.arange(8, dtype=torch.int32, device="cuda").flip(0).view(B, 4)
+    start = [14, 30]  # the second token of both begins a page
+    inv = (10000.0 ** (-torch.arange(32) / 32)).float().cuda()
+    axes = fused.rotary_axes([12, 10, 10])
+    w = rows((2, dim), BF, 3, 0.1).cuda()
+    qs, ks, vs = (rows((steps, B, 1, n, dim), BF, 4 + n, 0.5).cuda() for n in (heads, kv_heads, kv_heads))
+    q, k, v = (x[0].clone() for x in (qs, ks, vs))
+    lengths = torch.tensor(start, dtype=torch.int32, device="cuda")
+
+    def run(cache):
+        at = lengths.to(torch.int64)
+        positions = torch.stack([at, at // 2, at // 3]).view(3, B, 1)
+        slots = table.gather(1, (at // page)[:, None]).view(B).to(torch.int64) * page + at % page
+        rq, rk = fused.qk_norm_mrope(q, k, w[0], w[1], positions, inv, axes, 1e-6)
+        cache.append(0, rk[:, 0], v[:, 0], slots)
+        return kv4.decode_attention(rq.transpose(1, 2), cache, 0, table, lengths + 1, scale=dim**-0.5)
+
+    def fresh():
+        cache = kv4.Kv4Cache(1, 8, kv_heads=kv_heads, head_dim=dim, page_tokens=page)
+        for b, n in enumerate(start):
+            old = rows((n, kv_heads, dim), BF, 20 + b).cuda()
+            cache.append(0, old, old, cache.slots(table[b], 0, n))
+        lengths.copy_(torch.tensor(start, dtype=torch.int32))
+        return cache
+
+    cache, want = fresh(), []
+    for i in range(steps):
+        q.copy_(qs[i]), k.copy_(ks[i]), v.copy_(vs[i])
+        want.append(run(cache))
+        lengths.add_(1)
+    cache = fresh()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(cache)
+    for i in range(steps):
+        q.copy_(qs[i]), k.copy_(ks[i]), v.copy_(vs[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i]), i
+        lengths.add_(1)
+    assert not torch.equal(want[0], want[1]) and _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_a_captured_question_batch(monkeypatch, in_place):
+    monkeypatch.setattr(kv4, "_reads_codes", lambda *a: in_place)
+    kv4._plans_of.cache_clear()
+    cache = kv4.Kv4Cache(1, 6, kv_heads=2, head_dim=128, page_tokens=32)
+    table, lens = torch.arange(6, dtype=torch.int32, device="cuda"), torch.tensor([5, 0, 9], dtype=torch.int32, device="cuda")
+    old = rows((150, 2, 128), BF, 1, 0.5)
+    cache.append(0, old.cuda(), old.cuda(), cache.slots(table, 0, 150))
+    kept = ref.stored(old).transpose(0, 1)
+    q, k, v = (rows((3, 9, n, 128), BF, n + s, 0.5).transpose(1, 2) for n, s in ((8, 1), (2, 2), (2, 3)))
+    on = [x.cuda() for x in (q, k, v)]
+    ask = lambda: kv4.question_attention(on[0], cache, 0, table, 150, on[1], on[2], lens, scale=128**-0.5)  # noqa: E731
+    check_question(ask(), q, (kept, kept), k, v, [5, 0, 9], 128**-0.5, BF)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ask()
+    for lengths in ([5, 0, 9], [9, 1, 3]):
+        lens.copy_(torch.tensor(lengths, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        check_question(out, q, (kept, kept), k, v, lengths, 128**-0.5, BF)
+    kv4._plans_of.cache_clear()
+    assert _lib.device_error() == 0
 
 
 def test_no_room_and_shared_last_page():
