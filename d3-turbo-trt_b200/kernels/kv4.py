@@ -351,7 +351,8 @@ def question_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torc
             k, v = cache.read(layer, table, state_len, dtype=q.dtype)
             if k_q.stride() != v_q.stride():
                 k_q, v_q = (x.clone(memory_format=torch.contiguous_format) for x in (k_q, v_q))
-            _prefix_bidir(q, k, v, k_q, v_q, lens, scale, out)
+            # graphs may be replayed in any order and side by side: each call in one has its own workspace
+            _prefix_bidir(q, k, v, k_q, v_q, lens, scale, out, torch.cuda.is_current_stream_capturing())
     return out
 
 

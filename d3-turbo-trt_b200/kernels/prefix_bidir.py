@@ -126,6 +126,7 @@ def _launch(
     lens: torch.Tensor,
     scale: float,
     out: torch.Tensor,
+    own_workspace: bool = False,
 ) -> None:
     rows, heads, width, dim = q.shape
     kv_heads = k_q.shape[1]
@@ -141,7 +142,8 @@ def _launch(
     if k_q.stride() != v_q.stride():
         raise RuntimeError("k_q and v_q must share strides")
     lib = _lib.lib()
-    ws = _workspace(q.device, int(lib.d3b_prefix_bidir_workspace_size(rows, heads, kv_heads, state, width, dim)))
+    need = int(lib.d3b_prefix_bidir_workspace_size(rows, heads, kv_heads, state, width, dim))
+    ws = q.new_zeros(need, dtype=torch.uint8) if own_workspace and need else _workspace(q.device, need)
     status = lib.d3b_prefix_bidir_ws(
         _lib.ptr(q), st_q, _lib.ptr(k_state), _lib.ptr(v_state), st_kv, _lib.ptr(k_q), _lib.ptr(v_q), st_kq,
         _lib.ptr(lens), rows, heads, kv_heads, state, width, dim, _lib.dtype_code(q.dtype), float(scale),

@@ -11,7 +11,7 @@ import torch
 
 import e2e_model as em
 from conftest import ROOT  # noqa: F401
-from test_kv4_gpu import check_question, decode_bound, rows
+from test_kv4_gpu import check_question, decode_bound, half_step, rows
 
 from d3_turbo_trt_b200 import _lib
 from d3_turbo_trt_b200.kernels import kv4
@@ -190,6 +190,38 @@ def test_a_captured_question_batch(monkeypatch, in_place):
         graph.replay()
         torch.cuda.synchronize()
         check_question(out, q, (kept, kept), k, v, lengths, 128**-0.5, BF)
+    kv4._plans_of.cache_clear()
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_two_question_graphs_side_by_side(monkeypatch, in_place):
+    # captured on one stream, the later one replayed first, then both at once on two streams
+    monkeypatch.setattr(kv4, "_reads_codes", lambda *a: in_place)
+    kv4._plans_of.cache_clear()
+    tokens, B, L = 4096, 2, 40
+    cache = kv4.Kv4Cache(1, 32, kv_heads=4, head_dim=256, page_tokens=128)
+    table, lens = torch.arange(32, dtype=torch.int32, device="cuda"), torch.full((B,), L, dtype=torch.int32, device="cuda")
+    assert _lib.lib().d3b_prefix_bidir_workspace_size(B, 24, 4, tokens, L, 256) > 0
+    old = rows((tokens, 4, 256), BF, 1, 0.5).cuda()
+    cache.append(0, old, old, cache.slots(table, 0, tokens))
+    args = [[rows((B, L, n, 256), BF, 10 * g + n, 0.5).cuda().transpose(1, 2) for n in (24, 4, 4)] for g in range(2)]
+    ask = lambda g: kv4.question_attention(args[g][0], cache, 0, table, tokens, args[g][1], args[g][2], lens, scale=0.1)  # noqa: E731
+    want, graphs, outs, streams = [ask(g) for g in range(2)], [], [], [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    cap = torch.cuda.Stream()
+    for g in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[g], stream=cap):
+            outs.append(ask(g))
+    for order in ((1,), (0,), *((1, 0), (0, 1)) * 10):
+        for g in order:
+            with torch.cuda.stream(streams[g]):
+                outs[g].fill_(1)
+                graphs[g].replay()
+        torch.cuda.synchronize()
+        for g in order:  # a unit's parts are added in the order in which they end: within their rounding of each other
+            assert float((outs[g].float() - want[g].float()).abs().max()) <= 2 * half_step(BF) * float(want[g].abs().max())
     kv4._plans_of.cache_clear()
     assert _lib.device_error() == 0
 
