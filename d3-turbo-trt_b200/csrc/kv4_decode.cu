@@ -6,64 +6,95 @@ namespace {
 
 using namespace d3b_kv4;
 
-// One CTA a query row: the parts of its unit, added in a fixed order. The parts' factors are worked
-// out first, a thread a part; then groups of D/4 threads add every kGroups-th part, then the groups in
-// turn. THREADS is 64 where a unit has few parts (64 sequences of 16384 tokens: 2048 rows of 4 parts,
-// 1 us less) and 256 where it has many. Launched before the attention kernel has finished; it waits for it here.
+// One CTA a query row: the parts of its unit, added in a fixed order by groups of D/4 threads, every
+// kGroups-th part a group, then the groups in turn. Bound: latency. Behind the attention kernel stand one
+// load of the unit's range, one of its parts and their factors side by side, and one barrier: with up to 32
+// parts every warp works out all factors by itself. THREADS is 64 where a unit has few parts (64 sequences
+// of 16384 tokens: 2048 rows of 4 parts) and 256 where it has many. Launched before the attention kernel has
+// finished; it waits for it here.
 template <int D, int THREADS, bool BF>
 __global__ void __launch_bounds__(THREADS) merge_kernel(const __grid_constant__ AttnArgs a, int tile_rows) {
   constexpr int kGroups = THREADS / (D / 4);
+  constexpr int kAhead = 32 / kGroups < 8 ? 32 / kGroups : 8;  // parts a thread loads at once
   __shared__ float4 part[kGroups][D / 4];
   __shared__ float factor[THREADS], tops[THREADS / 32], sums[THREADS / 32];
   const int rows = a.group * a.L;
   const int row = blockIdx.x % rows, bk = blockIdx.x / rows;
   const int kvh = bk % a.kv_heads, b = bk / a.kv_heads;
   const int t = threadIdx.x, d4 = t % (D / 4), group = t / (D / 4);
+  int tokens = a.L;
+  if (a.own_lengths) tokens = min(max(__ldg(a.own_lengths + b), 0), a.L);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int2 range = a.ranges[(int64_t)bk * a.row_tiles + row / tile_rows];
   if (range.x == range.y) return;  // finished where it was computed
   // the unit's first CTA began it (slot 1), the others went on with it (slot 0)
   auto at = [&](int cta) { return (2 * (int64_t)cta + (cta == range.x)) * tile_rows + row % tile_rows; };
-  float top = -INFINITY;
-  for (int c = range.x + t; c <= range.y; c += THREADS) top = fmaxf(top, a.part_st[at(c) * 2]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (t % 32 == 0) tops[t / 32] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, tops[w]);
-  const float base = finite_or_zero(top);
+  auto load_st = [&](int cta) { return *reinterpret_cast<const float2*>(a.part_st + at(cta) * 2); };
+  auto load_o = [&](int cta) { return *reinterpret_cast<const float4*>(a.part_o + at(cta) * D + 4 * d4); };
   float sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c0 = range.x; c0 <= range.y; c0 += THREADS) {
-    const int n = min(THREADS, range.y + 1 - c0);
-    __syncthreads();
-    if (t < n) {
-      const float2 st = *reinterpret_cast<const float2*>(a.part_st + at(c0 + t) * 2);
-      const float f = ex2(st.x - base);
-      factor[t] = f;
-      sum = fmaf(st.y, f, sum);
+  auto add = [&](const float4& x, float f) {
+    acc.x = fmaf(x.x, f, acc.x);
+    acc.y = fmaf(x.y, f, acc.y);
+    acc.z = fmaf(x.z, f, acc.z);
+    acc.w = fmaf(x.w, f, acc.w);
+  };
+  const int count = range.y + 1 - range.x, lane = t % 32;
+  if (count <= 32) {
+    const float2 st = lane < count ? load_st(range.x + lane) : make_float2(-INFINITY, 0.f);
+    float4 x[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      x[i] = group + i * kGroups < count ? load_o(range.x + group + i * kGroups) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = st.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float f = lane < count ? ex2(st.x - finite_or_zero(top)) : 0.f;
+    sum = st.y * f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) add(x[i], __shfl_sync(0xffffffffu, f, (group + i * kGroups) & 31));
+    for (int i = kAhead; i * kGroups < count; ++i) {  // the same number of times in every lane
+      const int p = group + i * kGroups;
+      const float g = __shfl_sync(0xffffffffu, f, p & 31);
+      if (p < count) add(load_o(range.x + p), g);
     }
+  } else {
+    float top = -INFINITY;
+    for (int c = range.x + t; c <= range.y; c += THREADS) top = fmaxf(top, a.part_st[at(c) * 2]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) tops[t / 32] = top;
     __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, tops[w]);
+    const float base = finite_or_zero(top);
+    for (int c0 = range.x; c0 <= range.y; c0 += THREADS) {
+      const int n = min(THREADS, range.y + 1 - c0);
+      __syncthreads();
+      if (t < n) {
+        const float2 st = load_st(c0 + t);
+        const float f = ex2(st.x - base);
+        factor[t] = f;
+        sum = fmaf(st.y, f, sum);
+      }
+      __syncthreads();
 #pragma unroll 8
-    for (int i = group; i < n; i += kGroups) {
-      const float4 x = *reinterpret_cast<const float4*>(a.part_o + at(c0 + i) * D + 4 * d4);
-      const float f = factor[i];
-      acc.x = fmaf(x.x, f, acc.x);
-      acc.y = fmaf(x.y, f, acc.y);
-      acc.z = fmaf(x.z, f, acc.z);
-      acc.w = fmaf(x.w, f, acc.w);
+      for (int i = group; i < n; i += kGroups) add(load_o(c0 + i), factor[i]);
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sums[t / 32] = sum;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (t % 32 == 0) sums[t / 32] = sum;
-  part[group][d4] = acc;
-  __syncthreads();
+  if constexpr (kGroups > 1) part[group][d4] = acc;
+  if (kGroups > 1 || count > 32) __syncthreads();
   if (group) return;
-  sum = 0.f;
+  if (count > 32) {
+    sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) sum += sums[w];
+    for (int w = 0; w < THREADS / 32; ++w) sum += sums[w];
+  }
 #pragma unroll
   for (int g = 1; g < kGroups; ++g) {
     const float4 x = part[g][d4];
@@ -72,8 +103,6 @@ __global__ void __launch_bounds__(THREADS) merge_kernel(const __grid_constant__ 
     acc.z += x.z;
     acc.w += x.w;
   }
-  int tokens = a.L;
-  if (a.own_lengths) tokens = min(max(__ldg(a.own_lengths + b), 0), a.L);
   store_row<BF>(a, b, kvh, row, tokens, 4 * d4, acc, sum);
 }
 
