@@ -25,7 +25,9 @@
 // Work is dealt out evenly whatever the lengths are: all units (sequence, kv head, tile of rows)
 // are cut into pieces of keys, laid end to end, and every CTA takes the same number of pieces. A
 // unit that lies in one CTA is finished there; the others leave partial results, at most two a
-// CTA, which a second kernel adds in order.
+// CTA, which a second kernel adds in order. A CTA that goes from one unit to the next starts its loads anew,
+// which takes as long as two or three tiles; with few sequences every unit begins with a CTA where that makes
+// no share much longer.
 #pragma once
 
 #include "kv4.cuh"
@@ -200,7 +202,19 @@ struct Sequence {
   int len, own, tokens;  // cached keys, own keys, tokens of the block that are real
   int cached, pieces;    // pieces of cached keys; of all keys, at least one
   int live;              // row tiles with real tokens; each other tile is one piece that writes zeros
-  int per_head, total;   // pieces of a kv head and of the sequence
+  int step, dead;        // places of a live tile, of all other tiles: their pieces, filled up to `round`
+  int per_head, total;   // places of a kv head and of the sequence
+
+  __device__ __forceinline__ void lay(const AttnArgs& a, int round) {
+    step = pieces;
+    dead = a.row_tiles - live;
+    if (round > 1) {
+      step = (int)((uint32_t)(step + round - 1) / (uint32_t)round) * round;
+      if (dead) dead = (int)((uint32_t)(dead + round - 1) / (uint32_t)round) * round;
+    }
+    per_head = live * step + dead;
+    total = a.kv_heads * per_head;
+  }
 };
 
 template <int KEYS, int ROWS>
@@ -227,24 +241,43 @@ __device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b, bool repo
   s.cached = (s.len + KEYS - 1) / KEYS;
   s.pieces = max(1, s.cached + (s.own + KEYS - 1) / KEYS);
   s.live = (s.tokens * a.group + ROWS - 1) / ROWS;
-  s.per_head = s.live * s.pieces + a.row_tiles - s.live;
-  s.total = a.kv_heads * s.per_head;
+  s.lay(a, 1);
   return s;
 }
 
 // where a CTA's pieces begin
 struct Deal {
-  int first, last;  // its pieces
-  int share;
+  int first, last;  // its places
+  int share, round;  // round: 1, or the share where every unit begins with a CTA
   int b, offset;  // the sequence of the first, and how far into it
 };
 
-// Sums the sequences' pieces and finds the CTA's share; all threads, `box` in shared memory.
-template <int KEYS, int ROWS>
+// Sums the sequences' pieces and finds the CTA's share; all threads, `box` in shared memory. STEP: what a share
+// grows by so that units can begin with a CTA, twice at most.
+template <int KEYS, int ROWS, int STEP>
 __device__ __forceinline__ Deal deal(const AttnArgs& a, int at_least, int* box) {
   const int t = threadIdx.x, warp = t / 32, lane = t % 32;
   if (a.B <= 32) {  // a lane a sequence, every warp for itself: no barrier
-    const int mine = lane < a.B ? sequence<KEYS, ROWS>(a, lane, t < 32 && blockIdx.x == 0).total : 0;
+    Sequence s = {};
+    if (lane < a.B) s = sequence<KEYS, ROWS>(a, lane, t < 32 && blockIdx.x == 0);
+    Deal d;
+    const int places = (int)__reduce_add_sync(0xffffffffu, (uint32_t)s.total);
+    d.share = max(at_least, (places + (int)gridDim.x - 1) / (int)gridDim.x);
+    d.round = 1;
+    // one place each needs nothing; with no more units than CTAs, filled up they have at most twice the places: below 2^31 here
+    if (d.share > 1 && places < (1 << 28) && (int64_t)a.B * a.kv_heads * a.row_tiles <= (int64_t)gridDim.x) {
+#pragma unroll 1
+      for (int i = 0; i < 3 && d.round == 1; ++i) {
+        const int share = (d.share + STEP - 1) / STEP * STEP + i * STEP;
+        if (lane < a.B) s.lay(a, share);
+        if ((int)__reduce_add_sync(0xffffffffu, (uint32_t)s.total / (uint32_t)share) <= (int)gridDim.x) d.round = share;
+      }
+      if (d.round > 1)
+        d.share = d.round;
+      else if (lane < a.B)
+        s.lay(a, 1);
+    }
+    const int mine = s.total;
     int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -252,8 +285,6 @@ __device__ __forceinline__ Deal deal(const AttnArgs& a, int at_least, int* box) 
       if (lane >= o) upto += x;
     }
     const int total = __shfl_sync(0xffffffffu, upto, 31);
-    Deal d;
-    d.share = max(at_least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
     d.first = (int)min((int64_t)blockIdx.x * d.share, (int64_t)total);
     d.last = min(d.first + d.share, total);
     d.b = min(__popc(__ballot_sync(0xffffffffu, upto <= d.first)), 31);
@@ -281,6 +312,7 @@ __device__ __forceinline__ Deal deal(const AttnArgs& a, int at_least, int* box) 
   before += upto - mine;
   Deal d;
   d.share = max(at_least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+  d.round = 1;
   d.first = (int)min((int64_t)blockIdx.x * d.share, (int64_t)total);
   d.last = min(d.first + d.share, total);  // shares are far below 2^31 when first is not the total
   if (d.first >= before && d.first < before + mine) {

@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
   uint4* qs = reinterpret_cast<uint4*>(smem + (P::kRing > P::kMerge ? P::kRing : P::kMerge));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
   const int rows = a.group * a.L;
-  const Deal mine = deal<P::kKeys, P::kRows>(a, kLeast, box);
+  const Deal mine = deal<P::kKeys, P::kRows, kWarps>(a, kLeast, box);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may take its place; it waits for our end
   const uint32_t ring = d3b::smem_u32(smem) + warp * P::kWarpRing;
   const int grain_shift = a.page_shift - 4, in_page = (1 << grain_shift) - 1;
@@ -63,9 +63,11 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
 
   int pos = mine.first, b = mine.b, offset = mine.offset;
   while (pos < mine.last) {
-    const Sequence seq = sequence<P::kKeys, P::kRows>(a, b, false);
-    const int kvh = offset / seq.per_head, tile = (offset - kvh * seq.per_head) / seq.pieces;  // every tile is live
-    const int piece0 = offset - kvh * seq.per_head - tile * seq.pieces, piece1 = min(seq.pieces, piece0 + mine.last - pos);
+    Sequence seq = sequence<P::kKeys, P::kRows>(a, b, false);
+    seq.lay(a, mine.round);
+    const int kvh = offset / seq.per_head, tile = (offset - kvh * seq.per_head) / seq.step;  // every tile is live
+    const int piece0 = offset - kvh * seq.per_head - tile * seq.step, taken = min(seq.step - piece0, mine.last - pos);
+    const int piece1 = min(seq.pieces, piece0 + taken);
     const int row0 = tile * P::kRows, len = seq.len, grains = (len + 15) / 16;
     // the warp's steps: granules my_first + step * kStride ...
     constexpr int kStride = P::GP * kWarps;
@@ -392,8 +394,8 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
       a.ranges[((int64_t)b * a.kv_heads + kvh) * a.row_tiles + tile] =
           make_int2(pos / mine.share, (pos + seq.pieces - 1) / mine.share);
     __syncthreads();  // the rings and the queries are free again
-    pos += piece1 - piece0;
-    offset += piece1 - piece0;
+    pos += taken;
+    offset += taken;
     if (offset == seq.total) {
       offset = 0;
       ++b;

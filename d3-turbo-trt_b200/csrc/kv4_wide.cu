@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
   float* own_scale = maxima + kWarps * P::kRows;  // [key]: what an own V row is multiplied by
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
   const int rows = a.group * a.L;
-  const Deal mine = deal<kKeys, P::kRows>(a, 1, box);
+  const Deal mine = deal<kKeys, P::kRows, 1>(a, 1, box);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may take its place; it waits for our end
   const uint32_t k_ring = d3b::smem_u32(smem), v_ring = k_ring + 2 * 4 * P::kStage;
   const int grain_shift = a.page_shift - 4, in_page = (1 << grain_shift) - 1;
@@ -81,14 +81,17 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
 
   int pos = mine.first, b = mine.b, offset = mine.offset;
   while (pos < mine.last) {
-    const Sequence seq = sequence<kKeys, P::kRows>(a, b, false);
+    Sequence seq = sequence<kKeys, P::kRows>(a, b, false);
+    seq.lay(a, mine.round);
     const int kvh = offset / seq.per_head;
     const int in_head = offset - kvh * seq.per_head;
-    // live tiles have seq.pieces pieces each, the others one
-    const bool dead = in_head >= seq.live * seq.pieces;
-    const int tile = dead ? seq.live + in_head - seq.live * seq.pieces : in_head / seq.pieces;
-    const int pieces = dead ? 1 : seq.pieces;
-    const int piece0 = dead ? 0 : in_head - tile * seq.pieces, piece1 = min(pieces, piece0 + mine.last - pos);
+    // live tiles have seq.step places each, the others one, the last of them also what fills up
+    const int none = in_head - seq.live * seq.step;
+    const bool dead = none >= 0;
+    const int tile = dead ? seq.live + none : in_head / seq.step;
+    const int pieces = dead ? 1 : seq.pieces, piece0 = dead ? 0 : in_head - tile * seq.step;
+    const int left = !dead ? seq.step - piece0 : tile + 1 < a.row_tiles ? 1 : seq.dead - none;
+    const int taken = min(left, mine.last - pos), piece1 = min(pieces, piece0 + taken);
     const int row0 = tile * P::kRows, len = seq.len, grains = (len + 15) / 16;
     const int last_cached = dead ? piece0 : min(piece1, seq.cached);
     const uint8_t* head_pool = a.pool + kvh * a.head_bytes + 16 * lane;
@@ -517,8 +520,8 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
       a.ranges[((int64_t)b * a.kv_heads + kvh) * a.row_tiles + tile] =
           make_int2(pos / mine.share, (pos + pieces - 1) / mine.share);
     __syncthreads();  // ring, queries and sums are free again
-    pos += piece1 - piece0;
-    offset += piece1 - piece0;
+    pos += taken;
+    offset += taken;
     if (offset == seq.total) {
       offset = 0;
       ++b;
