@@ -14,6 +14,10 @@ cfg4 (readout 255 x 5120 x 255; snapshot: the 64-layer state snapshot at a
 255 blocks x 48 tokens x 48 value heads; gdn_state: one GDN layer's state pass,
 4096 tokens x 48 value heads with a final state; gated_norm_fp8, causal_conv,
 qk_norm_rope: the backbone's glue kernels at the question pass's 255 x 48 tokens).
+Kernels over the 4-bit cache have shapes of their own: kv4_append (16384 tokens), kv4_decode
+(64 sequences of 16384 tokens, 32/4 heads x 128), kv4_verify (3 sequences of 98765, five new
+tokens each, 24/4 heads x 256), kv4_question (one block of 11 tokens over 4096); qk_norm_mrope
+is 255 x 48 tokens of 32/4 heads x 128.
 Inputs are seeded synthetic tensors.
 """
 
@@ -199,7 +203,51 @@ def _glue(kernel: str, dev: torch.device, rows: int = 255, T: int = 48):
     return (lambda: fused.qk_norm_rope(qg[..., :128], w, cos, sin, 1e-6)), {"bytes": M * 32 * 128 * 4}
 
 
+def _kv4(kernel: str, dev: torch.device):
+    from .kernels import kv4
+
+    B, n, L, H, Hkv, D = {"kv4_append": (1, 16384, 1, 4, 4, 128), "kv4_decode": (64, 16384, 1, 32, 4, 128),
+                          "kv4_verify": (3, 98765, 5, 24, 4, 256), "kv4_question": (1, 4096, 11, 32, 4, 128)}[kernel]
+    g = torch.Generator(device=dev).manual_seed(7)
+    page = 64
+    need = -(-n // page)
+    cache = kv4.Kv4Cache(1, B * need, kv_heads=Hkv, head_dim=D, page_tokens=page, device=dev)
+    table = torch.randperm(B * need, generator=g, device=dev).to(torch.int32).view(B, need)
+    for b in range(B):
+        k, v = (torch.randn(n, Hkv, D, generator=g, device=dev).to(torch.bfloat16) for _ in range(2))
+        slots = cache.slots(table[b], 0, n)
+        cache.append(0, k, v, slots)
+    row = 2 * D * 2  # bytes of a token's K and V in 16 bits, per kv head
+    codes = (18 * D + 32) / 16
+    if kernel == "kv4_append":
+        return (lambda: cache.append(0, k, v, slots)), {"bytes": n * Hkv * (row + codes)}
+    q = torch.randn(B, H, L, D, generator=g, device=dev).to(torch.bfloat16)
+    work = {"bytes": B * n * Hkv * codes, "flops": 4.0 * B * H * L * n * D}
+    if kernel == "kv4_question":
+        own = k[:L].transpose(0, 1)[None]
+        return (lambda: kv4.question_attention(q, cache, 0, table[0], n, own, own, [L], scale=D ** -0.5)), work
+    lengths = torch.full((B,), n, dtype=torch.int32, device=dev)
+    return (lambda: kv4.decode_attention(q, cache, 0, table, lengths, scale=D ** -0.5, causal=True)), work
+
+
+def _mrope(dev: torch.device, rows: int = 255, T: int = 48):
+    from .model import fused
+
+    g = torch.Generator(device=dev).manual_seed(8)
+    q = torch.randn(rows, T, 32, 128, generator=g, device=dev).to(torch.bfloat16)
+    k = torch.randn(rows, T, 4, 128, generator=g, device=dev).to(torch.bfloat16)
+    w = (torch.randn(128, generator=g, device=dev) * 0.1).to(torch.bfloat16)
+    positions = torch.randint(0, 200000, (3, rows, T), generator=g, device=dev)
+    inv = 1.0 / 1e7 ** (torch.arange(16, device=dev).float() / 16)
+    axes = fused.rotary_axes([6, 5, 5])
+    return (lambda: fused.qk_norm_mrope(q, k, w, w, positions, inv, axes, 1e-6)), {"bytes": 2 * 2 * (q.numel() + k.numel())}
+
+
 def build(kernel: str, config: str, dev: torch.device):
+    if kernel.startswith("kv4_"):
+        return _kv4(kernel, dev)
+    if kernel == "qk_norm_mrope":
+        return _mrope(dev)
     if kernel in ("gated_norm_fp8", "causal_conv", "qk_norm_rope"):
         return _glue(kernel, dev)
     if kernel == "attention":
@@ -230,7 +278,7 @@ def main() -> None:
     ap.add_argument("--kernel", required=True,
                     choices=["attention", "gemm_fp8", "gemm_int8", "act_quant_fp8", "act_quant_int8", "readout",
                              "snapshot", "gdn", "gdn_recurrent", "gdn_state", "gated_norm_fp8", "causal_conv",
-                             "qk_norm_rope"])
+                             "qk_norm_rope", "qk_norm_mrope", "kv4_append", "kv4_decode", "kv4_verify", "kv4_question"])
     ap.add_argument("--config", default="cfg3a", choices=[*ATTN, "state4k", "cfg2", "cfg4"])
     ap.add_argument("--launches", type=int, default=3)
     ap.add_argument("--warmup", type=int, default=1)
