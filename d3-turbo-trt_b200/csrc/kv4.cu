@@ -42,14 +42,12 @@ __device__ __forceinline__ uint32_t to_e2m1x8(const float (&x)[8]) {
   return r;
 }
 
-// Rounded to 17 significant bits (half up). A quotient x / s is formed as x * (1 / s), which is off by
-// 2^-22 of it; x has at most 11 significant bits and s 4, so a quotient that is not a border of two
-// codes (at most 3 bits; for the scales' borders, 5 bits times 6) is 2^-12 of itself away from it, and
-// one that is a border becomes exactly that border here. The conversions below then round as the
-// quotient itself would.
-__device__ __forceinline__ float round17(float x) {
-  return __uint_as_float((__float_as_uint(x) + 0x40u) & 0xFFFFFF80u);
-}
+// Quotients x / s are formed as x * (1 / s), and must round to codes as themselves would. x has at most 11
+// significant bits and s 4, so a quotient that is not a border of two codes is 2^-12 of itself away from one,
+// far more than the product is off by. One that is a border is b = 1, 3, 5 or 7 (times a power of two) and
+// x = b * s; for every s the reciprocal's nearest float lies above 1 / s, by so little that the product with
+// b * s, rounded towards zero, is b (all 32 cases tried). Scales: x = 6 b with b of 5 bits, and
+// 6 b * float(1 / 6) rounds to b (all tried).
 
 // One row's codes of a lane's eight values, its group's scale and the row's exponent byte.
 struct Coded {
@@ -74,15 +72,15 @@ __device__ __forceinline__ Coded quantise(const uint4 raw) {
   const int e = max((int)(bits >> 23) - 127 - 11 + ((bits & 0x7FFFFFu) > 0x280000u ? 1 : 0), kExpMin);
   const float down = __uint_as_float((uint32_t)(127 - e) << 23);  // e in [-64, 117]
   Coded c;
-  c.scale = bad ? 0u : to_e4m3(round17(widen<BF>(group) * down * (1.0f / 6.0f)));
+  c.scale = bad ? 0u : to_e4m3(__fmul_rn(widen<BF>(group) * down, 1.0f / 6.0f));
   c.exponent = bad ? 255u : (uint32_t)(e + 127);
   const float scale = __half2float(__ushort_as_half((unsigned short)(decode_scales(c.scale) & 0xFFFFu)));
   const float by = scale > 0.f ? __frcp_rn(scale) * down : 0.f;
   float x[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    x[2 * i] = round17(widen<BF>(w[i] & 0xFFFFu) * by);
-    x[2 * i + 1] = round17(widen<BF>(w[i] >> 16) * by);
+    x[2 * i] = __fmul_rz(widen<BF>(w[i] & 0xFFFFu), by);
+    x[2 * i + 1] = __fmul_rz(widen<BF>(w[i] >> 16), by);
   }
   c.codes = bad ? 0u : to_e2m1x8(x);  // a NaN times zero is not zero
   return c;

@@ -118,6 +118,32 @@ def test_append_borders_zeros_and_range(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
+def test_append_every_scale_and_border(dtype):
+    """x = border * scale for every significand of a scale and every border of two codes, both signs: products with a
+    rounded reciprocal must not fall off the border; and 6 * border of two scales for every border."""
+    x = []
+    for m in range(8, 16):
+        for power in (-10, -3, 0, 5):
+            s = m * 2.0**power
+            b = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0]) * s
+            x.append(torch.cat([b, -b, 448 * 6 * 2.0**power * torch.ones(1), torch.zeros(47)]))
+    for m in range(16, 32):  # borders have 5 bits
+        for power in (-9, -4, 0, 3):
+            x.append(torch.cat([torch.full((16,), 6 * m * 2.0**power), torch.full((1,), 2688.0), torch.zeros(47)]))
+    x = torch.stack(x).to(dtype)[:, None]
+    n = len(x)
+    cache = new_cache(8, 1, 64, 16)
+    table = torch.tensor([7, 2, 0, 1, 5, 6], dtype=torch.int32, device="cuda")
+    cache.append(0, x.cuda(), x.flip(-1).contiguous().cuda(), cache.slots(table, 0, n))
+    k, v = cache.read(0, table, n, dtype=dtype)
+    # 2688 * 2^5 is infinite in fp16: those rows read back as NaN
+    whole = lambda t: torch.nan_to_num(t.cpu().double(), nan=7e300)  # noqa: E731
+    assert torch.equal(whole(k[0]), whole(ref.stored(x)[:, 0]))
+    assert torch.equal(whole(v[0]), whole(ref.stored(x.flip(-1))[:, 0]))
+    assert bool((k[0].isfinite().all(-1).cpu() == x[:, 0].isfinite().all(-1)).all()) and _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
 def test_read_saturates(dtype):
     """A row whose maximum rounds up beyond the type's largest value reads as that value."""
     top = torch.finfo(dtype).max
