@@ -17,7 +17,8 @@
 // as many warps as there are heads, many tokens share the table's cost.
 //
 // Bound: bytes, each value read and written once, with instructions close behind (about 90 for
-// the 256 values a warp holds, where memory leaves room for 170).
+// the 256 values a warp holds, where memory leaves room for 170). Measured (B200): 255 x 47 tokens of 32 + 4
+// heads x 128 49 us (4.5 TB/s, 0.69 of a plain copy's rate, issue slots 62 % busy); one token 6 us.
 #include "common.cuh"
 
 namespace {

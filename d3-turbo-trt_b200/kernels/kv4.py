@@ -386,8 +386,8 @@ _WIDENED = {64: (9.4, 0.8, 21.0, 0.0), 128: (9.4, 0.87, 24.0, 0.03), 256: (9.4, 
 def _reads_codes(rows: int, heads: int, kv_heads: int, width: int, state_len: int, dim: int) -> bool:
     """Whether a question batch is faster reading the state's codes in place than widening the state first
     and running ``prefix_bidir_attention``'s kernel. For instance 32 query and 4 kv heads of 128 over 4096
-    tokens: one block of 12 tokens 22 against 36 us, 4 blocks of 12 36 against 36, 16 blocks of 12 89
-    against 37."""
+    tokens: one block of 12 tokens 17 against 37 us, 4 blocks of 12 29 against 37, 16 blocks of 12 82
+    against 38."""
     group = heads // kv_heads
     pieces = -(-state_len // 64) + -(-width // 64)
     share = -(-(rows * kv_heads * -(-width * group // 32) * pieces) // 296)
