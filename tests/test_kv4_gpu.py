@@ -453,7 +453,33 @@ def test_decode_pool_beyond_4_gib():
     assert torch.equal(cache.pool[1, pages - 1], cache.pool[1, pages - 2])
 
 
+
+@pytest.mark.parametrize("dim,group,L", [(64, 8, 1), (128, 5, 3), (256, 6, 1), (256, 6, 5), (64, 3, 11)])
+@pytest.mark.parametrize("lengths", [[5000, 0, 17, 3100, 1], [2900], [700] * 32, [64, 4096, 4095, 4097]])
+def test_decode_shares_of_ragged_sequences(dim, group, L, lengths):
+    """Shares of several tiles: units that begin with a CTA, filled up at their ends, and those that do not."""
+    cache, table, kept = filled(lengths, 2, dim, 64, BF, seed=group)
+    q = rows((len(lengths), 2 * group, L, dim), BF, seed=L)
+    check_decode(q, cache, table, lengths, kept, dim**-0.5, True, BF)
+
+
 # --------------------------------------------------------------------------- question attention
+@pytest.mark.parametrize("lengths", [[40, 3, 0, 17], [0, 0, 40], [1] * 9])
+def test_question_shares_with_tiles_of_padding(monkeypatch, lengths):
+    # in place, with shares of several tiles and whole tiles of rows behind their block's length
+    monkeypatch.setattr(kv4, "_reads_codes", lambda *a: True)
+    state, L, dim = 2100, 40, 64
+    cache, table, kept = filled([state], 2, dim, 32, BF, seed=3)
+    cache._plans.clear()
+    q = rows((len(lengths), L, 16, dim), BF, 1, 0.2).transpose(1, 2)
+    k, v = (rows((len(lengths), 2, L, dim), BF, s, 0.2) for s in (2, 3))
+    out = torch.full((len(lengths), 16, L, dim), 3.0, dtype=BF, device="cuda")
+    got = kv4.question_attention(q.cuda(), cache, 0, table[0], state, k.cuda(), v.cuda(), lengths, scale=dim**-0.5, out=out)
+    check_question(got, q, kept[0], k, v, lengths, dim**-0.5, BF)
+    cache._plans.clear()
+    assert _lib.device_error() == 0
+
+
 @pytest.mark.parametrize("dim,heads,kv_heads,page", [(64, 8, 2, 16), (128, 8, 1, 64), (256, 6, 1, 32)])
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("B,L,state", [(1, 1, 1), (2, 11, 77), (5, 20, 300), (3, 7, 0)])
