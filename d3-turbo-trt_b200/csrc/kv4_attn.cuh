@@ -27,7 +27,7 @@
 // unit that lies in one CTA is finished there; the others leave partial results, at most two a
 // CTA, which a second kernel adds in order. A CTA that goes from one unit to the next starts its loads anew,
 // which takes as long as two or three tiles; with few sequences every unit begins with a CTA where that makes
-// no share much longer.
+// no share much longer, else a unit counts as some pieces more than it has.
 #pragma once
 
 #include "kv4.cuh"
@@ -202,14 +202,14 @@ struct Sequence {
   int len, own, tokens;  // cached keys, own keys, tokens of the block that are real
   int cached, pieces;    // pieces of cached keys; of all keys, at least one
   int live;              // row tiles with real tokens; each other tile is one piece that writes zeros
-  int step, dead;        // places of a live tile, of all other tiles: their pieces, filled up to `round`
+  int step, dead;        // places of a live tile, of all other tiles: their pieces, filled up to `round` or with `start`
   int per_head, total;   // places of a kv head and of the sequence
 
-  __device__ __forceinline__ void lay(const AttnArgs& a, int round) {
-    step = pieces;
+  __device__ __forceinline__ void lay(const AttnArgs& a, int round, int start) {
+    step = pieces + start;
     dead = a.row_tiles - live;
     if (round > 1) {
-      step = (int)((uint32_t)(step + round - 1) / (uint32_t)round) * round;
+      step = (int)((uint32_t)(pieces + round - 1) / (uint32_t)round) * round;
       if (dead) dead = (int)((uint32_t)(dead + round - 1) / (uint32_t)round) * round;
     }
     per_head = live * step + dead;
@@ -217,7 +217,7 @@ struct Sequence {
   }
 };
 
-template <int KEYS, int ROWS>
+template <int KEYS, int ROWS, int START>
 __device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b, bool report) {
   Sequence s;
   s.len = a.most;
@@ -241,7 +241,7 @@ __device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b, bool repo
   s.cached = (s.len + KEYS - 1) / KEYS;
   s.pieces = max(1, s.cached + (s.own + KEYS - 1) / KEYS);
   s.live = (s.tokens * a.group + ROWS - 1) / ROWS;
-  s.lay(a, 1);
+  s.lay(a, 1, START);
   return s;
 }
 
@@ -249,33 +249,39 @@ __device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b, bool repo
 struct Deal {
   int first, last;  // its places
   int share, round;  // round: 1, or the share where every unit begins with a CTA
+  int start;         // else: places a unit has behind its pieces, for the time that starting it takes
   int b, offset;  // the sequence of the first, and how far into it
 };
 
 // Sums the sequences' pieces and finds the CTA's share; all threads, `box` in shared memory. STEP: what a share
 // grows by so that units can begin with a CTA, twice at most.
-template <int KEYS, int ROWS, int STEP>
+template <int KEYS, int ROWS, int STEP, int START>
 __device__ __forceinline__ Deal deal(const AttnArgs& a, int at_least, int* box) {
   const int t = threadIdx.x, warp = t / 32, lane = t % 32;
   if (a.B <= 32) {  // a lane a sequence, every warp for itself: no barrier
     Sequence s = {};
-    if (lane < a.B) s = sequence<KEYS, ROWS>(a, lane, t < 32 && blockIdx.x == 0);
+    if (lane < a.B) s = sequence<KEYS, ROWS, 0>(a, lane, t < 32 && blockIdx.x == 0);
     Deal d;
     const int places = (int)__reduce_add_sync(0xffffffffu, (uint32_t)s.total);
     d.share = max(at_least, (places + (int)gridDim.x - 1) / (int)gridDim.x);
     d.round = 1;
+    d.start = 0;
     // one place each needs nothing; with no more units than CTAs, filled up they have at most twice the places: below 2^31 here
     if (d.share > 1 && places < (1 << 28) && (int64_t)a.B * a.kv_heads * a.row_tiles <= (int64_t)gridDim.x) {
 #pragma unroll 1
       for (int i = 0; i < 3 && d.round == 1; ++i) {
         const int share = (d.share + STEP - 1) / STEP * STEP + i * STEP;
-        if (lane < a.B) s.lay(a, share);
+        if (lane < a.B) s.lay(a, share, 0);
         if ((int)__reduce_add_sync(0xffffffffu, (uint32_t)s.total / (uint32_t)share) <= (int)gridDim.x) d.round = share;
       }
-      if (d.round > 1)
-        d.share = d.round;
-      else if (lane < a.B)
-        s.lay(a, 1);
+    }
+    if (d.round > 1) {
+      d.share = d.round;
+    } else if (d.share > 1) {
+      d.start = START;
+      if (lane < a.B) s.lay(a, 1, START);
+      const int more = (int)__reduce_add_sync(0xffffffffu, (uint32_t)s.total);
+      d.share = max(at_least, (more + (int)gridDim.x - 1) / (int)gridDim.x);
     }
     const int mine = s.total;
     int upto = mine;
@@ -294,7 +300,7 @@ __device__ __forceinline__ Deal deal(const AttnArgs& a, int at_least, int* box) 
   const int per = (a.B + kThreads - 1) / kThreads;
   const int b0 = min(t * per, a.B), b1 = min(b0 + per, a.B);
   int mine = 0;
-  for (int b = b0; b < b1; ++b) mine += sequence<KEYS, ROWS>(a, b, blockIdx.x == 0).total;
+  for (int b = b0; b < b1; ++b) mine += sequence<KEYS, ROWS, START>(a, b, blockIdx.x == 0).total;
   int upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -313,12 +319,13 @@ __device__ __forceinline__ Deal deal(const AttnArgs& a, int at_least, int* box) 
   Deal d;
   d.share = max(at_least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
   d.round = 1;
+  d.start = START;
   d.first = (int)min((int64_t)blockIdx.x * d.share, (int64_t)total);
   d.last = min(d.first + d.share, total);  // shares are far below 2^31 when first is not the total
   if (d.first >= before && d.first < before + mine) {
     int b = b0, at = before;
     for (;; ++b) {
-      const int n = sequence<KEYS, ROWS>(a, b, false).total;
+      const int n = sequence<KEYS, ROWS, START>(a, b, false).total;
       if (d.first < at + n) break;
       at += n;
     }
@@ -329,6 +336,24 @@ __device__ __forceinline__ Deal deal(const AttnArgs& a, int at_least, int* box) 
   d.b = box[kWarps];
   d.offset = box[kWarps + 1];
   return d;
+}
+
+// A CTA whose first place lies behind a unit's pieces begins with the next unit. (Only the first can: a unit that
+// was worked on is left with all its places.)
+template <int KEYS, int ROWS>
+__device__ __forceinline__ void past_filling(const AttnArgs& a, Deal& d) {
+  if (!d.start || d.first >= d.last) return;
+  Sequence s = sequence<KEYS, ROWS, 0>(a, d.b, false);
+  s.lay(a, 1, d.start);
+  const int in_head = d.offset % s.per_head, place = in_head % s.step;
+  if (in_head >= s.live * s.step || place < s.pieces) return;
+  const int skip = min(s.step - place, d.last - d.first);
+  d.first += skip;
+  d.offset += skip;
+  if (d.offset == s.total) {
+    d.offset = 0;
+    ++d.b;
+  }
 }
 
 // Queries to shared memory in operand order, as fp16 under one power of two for the tile's rows:

@@ -126,7 +126,7 @@ bool make_plan(const d3b_kv4_cache* c, int B, int H, int L, int64_t keys, bool o
   const int64_t piece = p->wide ? 64 : D == 256 ? 16 : 32, least = p->wide ? 1 : 4;
   // own keys add at most L / 64 pieces, which `keys` holds
   const int64_t most = p->units * (keys / piece + 3);
-  if (p->units > (1 << 28) || most > (1 << 30)) return false;
+  if (p->units > (1 << 28) || most + 20 * p->units > (1 << 30)) return false;  // a unit counts as up to 20 pieces more
   p->row_tiles = (int)tiles;
   int64_t ctas = (int64_t)d3b_host::num_sms(d3b_host::current_device()) *
                  (p->wide ? resident_wide(D, p->nt) : resident_thin(D, p->nt));

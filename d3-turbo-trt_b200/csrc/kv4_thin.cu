@@ -22,6 +22,9 @@ template <int D, int NT>
 struct Thin {
   static constexpr int GP = D == 256 ? 1 : 2;                          // granules a step
   static constexpr int kKeys = 16 * GP;                                // keys of a piece
+  // pieces that starting a unit costs: 64 ragged sequences up to 4000 with 0, 8, 12, 16 and 24 of them 54, 31, 30,
+  // 31 and 32 us at D = 128; 68, 58, 52, 47 and 47 at D = 256
+  static constexpr int kStart = D == 256 ? 20 : 12;
   static constexpr int kStage = (granule_bytes(D) + 127) / 128 * 128;  // V rows start on 128-byte lines
   static constexpr int kRows = 8 * NT;
   static constexpr int kResident = NT == 1 ? (D == 64 ? 5 : 3) : 2;    // CTAs an SM
@@ -44,7 +47,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
   uint4* qs = reinterpret_cast<uint4*>(smem + (P::kRing > P::kMerge ? P::kRing : P::kMerge));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
   const int rows = a.group * a.L;
-  const Deal mine = deal<P::kKeys, P::kRows, kWarps>(a, kLeast, box);
+  Deal mine = deal<P::kKeys, P::kRows, kWarps, P::kStart>(a, kLeast, box);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may take its place; it waits for our end
   const uint32_t ring = d3b::smem_u32(smem) + warp * P::kWarpRing;
   const int grain_shift = a.page_shift - 4, in_page = (1 << grain_shift) - 1;
@@ -65,10 +68,11 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
     asm volatile("" : "+r"(place[i]));  // kept, not worked out again at every copy
   }
 
+  past_filling<P::kKeys, P::kRows>(a, mine);
   int pos = mine.first, b = mine.b, offset = mine.offset;
   while (pos < mine.last) {
-    Sequence seq = sequence<P::kKeys, P::kRows>(a, b, false);
-    seq.lay(a, mine.round);
+    Sequence seq = sequence<P::kKeys, P::kRows, 0>(a, b, false);
+    seq.lay(a, mine.round, mine.start);
     const int kvh = offset / seq.per_head, tile = (offset - kvh * seq.per_head) / seq.step;  // every tile is live
     const int piece0 = offset - kvh * seq.per_head - tile * seq.step, taken = min(seq.step - piece0, mine.last - pos);
     const int piece1 = min(seq.pieces, piece0 + taken);

@@ -29,6 +29,9 @@ struct Wide {
   static constexpr int kStage = (kHalf + 127) / 128 * 128;  // V rows start on 128-byte lines
   static constexpr int kRows = 8 * NT;
   static constexpr int kResident = 2;
+  // pieces that starting a unit costs: 200 ragged sequences up to 800, 30 rows x 256, with 0, 2, 4, 6 and 8 of them
+  // 151, 120, 107, 100 and 101 us
+  static constexpr int kStart = 6;
   static constexpr int kRing = 2 * 2 * 4 * kStage;  // two tiles' K, then two tiles' V, of four granules
   static constexpr int kQ = kRows * D * 2;
   static constexpr int kW = 4 * NT * 32 * 8;    // weights: [granule][nt][lane] x 8 bytes
@@ -45,6 +48,11 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// What a unit's end needs to know, kept in shared memory while its tiles use the registers.
+struct Unit {
+  int b, kvh, tile, tokens, own, cached, pieces, piece0, piece1, taken, pos, offset, total;
+};
+
 template <int D, int NT, bool BF>
 __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(const __grid_constant__ AttnArgs a) {
   using P = Wide<D, NT>;
@@ -53,13 +61,14 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int box[kWarps + 2];
   __shared__ float tops[kWarps];
+  __shared__ Unit kept;
   uint4* qs = reinterpret_cast<uint4*>(smem + P::kRing);
   uint2* ws = reinterpret_cast<uint2*>(smem + P::kRing + P::kQ);
   float* maxima = reinterpret_cast<float*>(smem + P::kRing + P::kQ + P::kW);  // [warp][row]
   float* own_scale = maxima + kWarps * P::kRows;  // [key]: what an own V row is multiplied by
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
   const int rows = a.group * a.L;
-  const Deal mine = deal<kKeys, P::kRows, 1>(a, 1, box);
+  Deal mine = deal<kKeys, P::kRows, 1, P::kStart>(a, 1, box);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may take its place; it waits for our end
   const uint32_t k_ring = d3b::smem_u32(smem), v_ring = k_ring + 2 * 4 * P::kStage;
   const int grain_shift = a.page_shift - 4, in_page = (1 << grain_shift) - 1;
@@ -83,10 +92,11 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
     v_at[x] = v_ring + v_swizzle<D>((2 * c + (x & 1) + 8 * (x >> 1)) * (D / 2) + warp * (D / 8) + r * (D / 64));
   const uint32_t vs_at = v_ring + P::kScales + ((warp * (D / 4) + r * kRun) / 16) * 16 + 2 * c;
 
+  past_filling<kKeys, P::kRows>(a, mine);
   int pos = mine.first, b = mine.b, offset = mine.offset;
   while (pos < mine.last) {
-    Sequence seq = sequence<kKeys, P::kRows>(a, b, false);
-    seq.lay(a, mine.round);
+    Sequence seq = sequence<kKeys, P::kRows, 0>(a, b, false);
+    seq.lay(a, mine.round, mine.start);
     const int kvh = offset / seq.per_head;
     const int in_head = offset - kvh * seq.per_head;
     // live tiles have seq.step places each, the others one, the last of them also what fills up
@@ -139,6 +149,8 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
     id_v = id_k;
     id_k = look(piece0 + 2);
 
+    if (threadIdx.x == 0)  // a dead tile has no own keys either
+      kept = {b, kvh, tile, seq.tokens, seq.own, dead ? 1 : seq.cached, pieces, piece0, piece1, taken, pos, offset, seq.total};
     const float q_scale = load_queries<D, NT, BF>(a, b, kvh, row0, rows, qs, tops);
     __syncthreads();
 
@@ -369,12 +381,14 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
     }
     cp_wait<0>();
 
+    const volatile Unit& u = kept;  // read where it is needed, not held
+
     // the block's own keys
-    for (int p = dead ? piece1 : max(piece0, seq.cached); p < piece1 && a.k_own; ++p) {
-      const int key0 = 64 * (p - seq.cached) + 16 * warp;  // the warp's 16 keys
-      if (64 * (p - seq.cached) >= seq.own) break;         // a unit without any key has one empty piece
-      const uint16_t* k_base = a.k_own + b * a.sk_b + kvh * a.sk_h;
-      const uint16_t* v_base = a.v_own + b * a.sv_b + kvh * a.sv_h;
+    for (int p = max(u.piece0, u.cached); p < u.piece1 && a.k_own; ++p) {
+      const int key0 = 64 * (p - u.cached) + 16 * warp;  // the warp's 16 keys
+      if (64 * (p - u.cached) >= u.own) break;         // a unit without any key has one empty piece
+      const uint16_t* k_base = a.k_own + u.b * a.sk_b + u.kvh * a.sk_h;
+      const uint16_t* v_base = a.v_own + u.b * a.sv_b + u.kvh * a.sv_h;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -383,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
       auto channel = [&](int w) { return D == 256 ? 128 * (w / 4) + 32 * c + 8 * (w % 4) : c * (D / 4) + 8 * w; };
       auto fetch = [&](const uint16_t* base, int64_t stride, int i, int w) {
         const int key = key0 + r + 8 * i;
-        return key < seq.own ? __ldg(reinterpret_cast<const uint4*>(base + key * stride + channel(w))) : make_uint4(0, 0, 0, 0);
+        return key < u.own ? __ldg(reinterpret_cast<const uint4*>(base + key * stride + channel(w))) : make_uint4(0, 0, 0, 0);
       };
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -440,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
       kq[0] = power_of(-up_k[0]) * q_scale;
       kq[1] = power_of(-up_k[1]) * q_scale;
       const float ev[2] = {-(float)up_v[0], -(float)up_v[1]};
-      weigh(s, kq, ev, true, [&](int, int j) { return key0 + r + 8 * (j >> 1) >= seq.own; }, [] {});
+      weigh(s, kq, ev, true, [&](int, int j) { return key0 + r + 8 * (j >> 1) >= u.own; }, [] {});
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint2 wf[NT];
@@ -449,11 +463,11 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
         uint32_t h[4][kRun / 2];  // channels of keys 2c, 2c + 1, 2c + 8, 2c + 9, as fp16
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const int in_tile = 16 * i + 2 * c + (x & 1) + 8 * (x >> 1), key = 64 * (p - seq.cached) + in_tile;
+          const int in_tile = 16 * i + 2 * c + (x & 1) + 8 * (x >> 1), key = 64 * (p - u.cached) + in_tile;
           const uint32_t* src = reinterpret_cast<const uint32_t*>(v_base + key * a.sv_l + warp * (D / 4) + r * kRun);
 #pragma unroll
           for (int j = 0; j < kRun / 2; ++j) {
-            const uint32_t w = key < seq.own ? __ldg(src + j) : 0u;
+            const uint32_t w = key < u.own ? __ldg(src + j) : 0u;
             if constexpr (BF) {
               const float2 f = widen2<BF>(w);
               h[x][j] = pack_half2(f.x * own_scale[in_tile], f.y * own_scale[in_tile]);
@@ -492,23 +506,24 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
         for (int j = 0; j < 2; ++j) maxima[warp * P::kRows + n * 8 + 2 * c + j] = l[n][j];
     }
     __syncthreads();
-    const bool whole = piece0 == 0 && piece1 == pieces;
-    const int64_t part = 2 * (int64_t)blockIdx.x + (piece0 == 0);
+    const int first_piece = u.piece0, first_row = u.tile * P::kRows;
+    const bool whole = first_piece == 0 && u.piece1 == u.pieces;
+    const int64_t part = 2 * (int64_t)blockIdx.x + (first_piece == 0);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int row = n * 8 + 2 * c + j;
-        if (row0 + row >= rows) continue;
+        if (first_row + row >= rows) continue;
         float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) sum += maxima[w * P::kRows + row];
         const int d = warp * (D / 4) + r * kRun;
         if (whole) {
-          const int li = (row0 + row) / a.group, h = kvh * a.group + (row0 + row) % a.group;
-          const bool real = sum != 0.f && li < seq.tokens;
+          const int li = (first_row + row) / a.group, h = u.kvh * a.group + (first_row + row) % a.group;
+          const bool real = sum != 0.f && li < u.tokens;
           const float f = real ? 1.f / sum : 0.f;
-          uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + b * a.so_b + h * a.so_h + li * a.so_l + d);
+          uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + u.b * a.so_b + h * a.so_h + li * a.so_l + d);
 #pragma unroll
           for (int x = 0; x < kTiles; ++x)
             dst[x] = real ? narrow<BF>(o[n][x][j] * f) | ((uint32_t)narrow<BF>(o[n][x][j + 2] * f) << 16) : 0u;
@@ -520,16 +535,17 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
             *reinterpret_cast<float2*>(a.part_st + (part * P::kRows + row) * 2) = make_float2(m[n][j], sum);
         }
       }
-    if (piece0 == 0 && threadIdx.x == 0)
-      a.ranges[((int64_t)b * a.kv_heads + kvh) * a.row_tiles + tile] =
-          make_int2(pos / mine.share, (pos + pieces - 1) / mine.share);
-    __syncthreads();  // ring, queries and sums are free again
-    pos += taken;
-    offset += taken;
-    if (offset == seq.total) {
+    if (first_piece == 0 && threadIdx.x == 0)
+      a.ranges[((int64_t)u.b * a.kv_heads + u.kvh) * a.row_tiles + u.tile] =
+          make_int2(u.pos / mine.share, (u.pos + u.pieces - 1) / mine.share);
+    pos = u.pos + u.taken;
+    offset = u.offset + u.taken;
+    b = u.b;
+    if (offset == u.total) {
       offset = 0;
       ++b;
     }
+    __syncthreads();  // ring, queries, sums and the unit's data are free again
   }
 }
 
