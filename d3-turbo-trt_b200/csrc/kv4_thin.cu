@@ -1,7 +1,7 @@
 // Attention over the 4-bit cache for few query rows a kv head (up to 16): decoding.
 //
 // A warp takes GP granules (32 keys, 16 at D = 256) a step by itself, from its own cp.async ring of
-// three steps and without barriers, and keeps all of O for its rows; a unit's warps are merged at the
+// two steps and without barriers, and keeps all of O for its rows; a unit's warps are merged at the
 // end of the CTA's share. One m16n8k16 serves 8 rows, so a group of up to 8 heads costs one product.
 //
 // Bound: the cache's bytes, 18 D + 32 for 16 tokens and kv head, with the ALU close behind: a code
@@ -16,7 +16,8 @@ namespace d3b_kv4 {
 namespace {
 
 constexpr int kLeast = kWarps;  // pieces a CTA takes at least: one a warp
-constexpr int kDepth = 3;       // steps in a warp's ring
+// Steps in a warp's ring. Three are 1 to 8 % slower: what they hold is not needed with 12 warps an SM and more.
+constexpr int kDepth = 2;
 
 template <int D, int NT>
 struct Thin {
@@ -27,7 +28,9 @@ struct Thin {
   static constexpr int kStart = D == 256 ? 20 : 12;
   static constexpr int kStage = (granule_bytes(D) + 127) / 128 * 128;  // V rows start on 128-byte lines
   static constexpr int kRows = 8 * NT;
-  static constexpr int kResident = NT == 1 ? (D == 64 ? 5 : 3) : 2;    // CTAs an SM
+  // CTAs an SM. 8 rows x 64 with 4 of them, 64 x 16000 keys, 49 us, with 5 (registers spilled) and 3 51; 16 x 64 with 3
+  // 64 us, with 2 70; 16 x 128 with 3 175 against 181, but one sequence of 16000 19 against 17 us
+  static constexpr int kResident = NT == 1 ? (D == 64 ? 4 : 3) : (D == 64 ? 3 : 2);
   static constexpr int kWarpRing = kDepth * GP * kStage;
   static constexpr int kRing = kWarps * kWarpRing;
   static constexpr int kMerge = kWarps * kRows * (D + 2) * 4;
@@ -122,14 +125,11 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
       }
       return bad;
     };
-    uint32_t bad_now = 0, bad_next = 0, bad_after = 0;
+    uint32_t bad_now = 0, bad_next = 0;
     look(0);
     bad_now = load(0, Int<0>{});
     cp_commit();
     look(1);
-    bad_next = load(1, Int<1>{});
-    cp_commit();
-    look(2);
 
     const float q_scale = load_queries<D, NT, BF>(a, b, kvh, row0, rows, qs, tops);
     __syncthreads();
@@ -172,9 +172,9 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
     auto step = [&](int now, auto slot) {
       constexpr int kSlot = decltype(slot)::value, kAt = kSlot * P::GP * P::kStage;
       __syncwarp();  // every lane is done with the slot that is loaded next
-      bad_after = load(now + 2, Int<(kSlot + 2) % kDepth>{});
+      bad_next = load(now + 1, Int<1 - kSlot>{});
       cp_commit();
-      look(now + 3);
+      look(now + 2);
       cp_wait<kDepth - 1>();
       __syncwarp();
 
@@ -345,12 +345,10 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
         }
       }
       bad_now = bad_next;
-      bad_next = bad_after;
     };
     for (int now = 0; now < steps; now += kDepth) {
       step(now, Int<0>{});
       if (now + 1 < steps) step(now + 1, Int<1>{});
-      if (now + 2 < steps) step(now + 2, Int<2>{});
     }
     cp_wait<0>();
 
@@ -434,8 +432,8 @@ int launch_thin(const AttnArgs& a, int D, int nt, bool bf, int ctas, cudaStream_
 }
 
 int resident_thin(int D, int nt) {
-  return nt == 1 ? (D == 64 ? Thin<64, 1>::kResident : D == 128 ? Thin<128, 1>::kResident : Thin<256, 1>::kResident)
-                 : Thin<128, 2>::kResident;
+  if (nt == 2) return D == 64 ? Thin<64, 2>::kResident : Thin<128, 2>::kResident;
+  return D == 64 ? Thin<64, 1>::kResident : D == 128 ? Thin<128, 1>::kResident : Thin<256, 1>::kResident;
 }
 
 }  // namespace d3b_kv4
