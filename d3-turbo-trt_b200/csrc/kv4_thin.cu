@@ -6,10 +6,10 @@
 //
 // Bound: the cache's bytes, 18 D + 32 for 16 tokens and kv head, with the ALU close behind: a code
 // pair costs a conversion (64 lanes a clock and SM) and a product with its scale. Measured (B200, 4 kv heads,
-// up to 8 rows): 64 sequences of 16000 tokens D = 128 131 us (4.6 TB/s, 0.70 of a plain copy's rate), D = 256
-// 222 us (5.3 TB/s, 0.81); D = 64, 2 heads, 54 us (2.8 TB/s: the instructions for a key do not halve with D). At 64
-// ragged sequences up to 16384 the loads alone take 91 us, the arithmetic alone 99 and the kernel 104. One token
-// of one sequence of 1000 11 us.
+// up to 8 rows): 64 sequences of 16000 tokens D = 128 128 us (4.7 TB/s, 0.71 of a plain copy's rate), D = 256
+// 221 us (5.4 TB/s, 0.82); D = 64, 2 heads, 49 us (3.1 TB/s: the instructions for a key do not halve with D). At 64
+// ragged sequences up to 16384 the loads alone took 91 us, the arithmetic alone 99, both 104 to 109. One token
+// of one sequence of 1000 10 us.
 #include "kv4_attn.cuh"
 
 namespace d3b_kv4 {
