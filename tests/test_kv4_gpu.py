@@ -455,7 +455,7 @@ def test_decode_pool_beyond_4_gib():
 
 
 @pytest.mark.parametrize("dim,group,L", [(64, 8, 1), (128, 5, 3), (256, 6, 1), (256, 6, 5), (64, 3, 11)])
-@pytest.mark.parametrize("lengths", [[5000, 0, 17, 3100, 1], [2900], [700] * 32, [64, 4096, 4095, 4097]])
+@pytest.mark.parametrize("lengths", [[5000, 0, 17, 3100, 1], [2900], [700] * 32, [64, 4096, 4095, 4097], [900, 0, 31, 350] * 10])
 def test_decode_shares_of_ragged_sequences(dim, group, L, lengths):
     """Shares of several tiles: units that begin with a CTA, filled up at their ends, and those that do not."""
     cache, table, kept = filled(lengths, 2, dim, 64, BF, seed=group)
@@ -464,7 +464,7 @@ def test_decode_shares_of_ragged_sequences(dim, group, L, lengths):
 
 
 # --------------------------------------------------------------------------- question attention
-@pytest.mark.parametrize("lengths", [[40, 3, 0, 17], [0, 0, 40], [1] * 9])
+@pytest.mark.parametrize("lengths", [[40, 3, 0, 17], [0, 0, 40], [1] * 9, [40, 1, 0, 17] * 9])
 def test_question_shares_with_tiles_of_padding(monkeypatch, lengths):
     # in place, with shares of several tiles and whole tiles of rows behind their block's length
     monkeypatch.setattr(kv4, "_reads_codes", lambda *a: True)
