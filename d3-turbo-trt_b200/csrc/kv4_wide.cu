@@ -385,8 +385,9 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
 
     // the block's own keys
     for (int p = max(u.piece0, u.cached); p < u.piece1 && a.k_own; ++p) {
-      const int key0 = 64 * (p - u.cached) + 16 * warp;  // the warp's 16 keys
-      if (64 * (p - u.cached) >= u.own) break;         // a unit without any key has one empty piece
+      const int own = u.own, cached = u.cached;
+      const int key0 = 64 * (p - cached) + 16 * warp;  // the warp's 16 keys
+      if (64 * (p - cached) >= own) break;         // a unit without any key has one empty piece
       const uint16_t* k_base = a.k_own + u.b * a.sk_b + u.kvh * a.sk_h;
       const uint16_t* v_base = a.v_own + u.b * a.sv_b + u.kvh * a.sv_h;
 #pragma unroll
@@ -397,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
       auto channel = [&](int w) { return D == 256 ? 128 * (w / 4) + 32 * c + 8 * (w % 4) : c * (D / 4) + 8 * w; };
       auto fetch = [&](const uint16_t* base, int64_t stride, int i, int w) {
         const int key = key0 + r + 8 * i;
-        return key < u.own ? __ldg(reinterpret_cast<const uint4*>(base + key * stride + channel(w))) : make_uint4(0, 0, 0, 0);
+        return key < own ? __ldg(reinterpret_cast<const uint4*>(base + key * stride + channel(w))) : make_uint4(0, 0, 0, 0);
       };
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -454,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
       kq[0] = power_of(-up_k[0]) * q_scale;
       kq[1] = power_of(-up_k[1]) * q_scale;
       const float ev[2] = {-(float)up_v[0], -(float)up_v[1]};
-      weigh(s, kq, ev, true, [&](int, int j) { return key0 + r + 8 * (j >> 1) >= u.own; }, [] {});
+      weigh(s, kq, ev, true, [&](int, int j) { return key0 + r + 8 * (j >> 1) >= own; }, [] {});
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint2 wf[NT];
@@ -463,11 +464,11 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
         uint32_t h[4][kRun / 2];  // channels of keys 2c, 2c + 1, 2c + 8, 2c + 9, as fp16
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const int in_tile = 16 * i + 2 * c + (x & 1) + 8 * (x >> 1), key = 64 * (p - u.cached) + in_tile;
+          const int in_tile = 16 * i + 2 * c + (x & 1) + 8 * (x >> 1), key = 64 * (p - cached) + in_tile;
           const uint32_t* src = reinterpret_cast<const uint32_t*>(v_base + key * a.sv_l + warp * (D / 4) + r * kRun);
 #pragma unroll
           for (int j = 0; j < kRun / 2; ++j) {
-            const uint32_t w = key < u.own ? __ldg(src + j) : 0u;
+            const uint32_t w = key < own ? __ldg(src + j) : 0u;
             if constexpr (BF) {
               const float2 f = widen2<BF>(w);
               h[x][j] = pack_half2(f.x * own_scale[in_tile], f.y * own_scale[in_tile]);
