@@ -356,17 +356,29 @@ __device__ __forceinline__ void past_filling(const AttnArgs& a, Deal& d) {
   }
 }
 
-// Queries to shared memory in operand order, as fp16 under one power of two for the tile's rows:
-// [nt][word][lane] x 16 bytes, lane = 4 * row + quarter. Returns scale * log2(e) * 2^power. The largest
-// magnitude goes to 2^14 or above; what is 2^-29 of it or less loses bits, scores by 2^-40 of the
-// largest row's. All threads, with a barrier; `box` kWarps floats.
+// the largest of a row's lanes; x is not negative
+template <int LANES>
+__device__ __forceinline__ float max_of_lanes(float x) {
+  if constexpr (LANES == 32) {
+    return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x)));  // ordered as bits
+  } else {
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+  }
+}
+
+// Queries to shared memory in operand order, as fp16, each row under its own power of two:
+// [nt][word][lane] x 16 bytes, lane = 4 * row + quarter. factors[row]: scale * log2(e) * 2^power, what a product is
+// multiplied by. The row's largest finite magnitude goes to 2^14 or above; what is 2^-29 of it or less loses bits,
+// scores by 2^-40 of the row's largest term. All threads; a barrier has to follow.
 template <int D, int NT, bool BF>
-__device__ __forceinline__ float load_queries(const AttnArgs& a, int b, int kvh, int row0, int rows, uint4* qs, float* box) {
+__device__ __forceinline__ void load_queries(const AttnArgs& a, int b, int kvh, int row0, int rows, uint4* qs,
+                                             float* factors) {
   constexpr int kLanes = D / 8;  // a lane takes 8 channels
   constexpr int kWords = D / 32;
   constexpr int kItems = (8 * NT * kLanes + kThreads - 1) / kThreads;
   uint4 raw[kItems];
-  float top = 0.f;
 #pragma unroll
   for (int x = 0; x < kItems; ++x) {
     const int i = x * kThreads + threadIdx.x, row = i / kLanes, sub = i % kLanes;
@@ -375,25 +387,22 @@ __device__ __forceinline__ float load_queries(const AttnArgs& a, int b, int kvh,
       const int l = (row0 + row) / a.group, g = (row0 + row) % a.group;
       raw[x] = __ldg(reinterpret_cast<const uint4*>(a.q + b * a.sq_b + (int64_t)(kvh * a.group + g) * a.sq_h + l * a.sq_l) + sub);
     }
+  }
+#pragma unroll
+  for (int x = 0; x < kItems; ++x) {
+    const int i = x * kThreads + threadIdx.x, row = i / kLanes, sub = i % kLanes;
     const uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+    float top = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 f = widen2<BF>(w[j]);
       top = fabsf(f.x) < INFINITY ? fmaxf(top, fabsf(f.x)) : top;
       top = fabsf(f.y) < INFINITY ? fmaxf(top, fabsf(f.y)) : top;
     }
-  }
-  const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));  // not negative: ordered as bits
-  if (threadIdx.x % 32 == 0) box[threadIdx.x / 32] = __uint_as_float(most);
-  __syncthreads();
-  top = fmaxf(fmaxf(box[0], box[1]), fmaxf(box[2], box[3]));
-  const int up = row_up(top);
-  const float by = power_of(up);
-#pragma unroll
-  for (int x = 0; x < kItems; ++x) {
-    const int i = x * kThreads + threadIdx.x, row = i / kLanes, sub = i % kLanes;
-    if (row >= 8 * NT) continue;
-    const uint32_t w[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+    const int up = row_up(max_of_lanes<kLanes>(top));
+    if (row >= 8 * NT) continue;  // whole warps, or lanes of rows that do not exist
+    if (sub == 0) factors[row] = a.scale_log2 * power_of(-up);
+    const float by = power_of(up);
     uint32_t h[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -407,7 +416,6 @@ __device__ __forceinline__ float load_queries(const AttnArgs& a, int b, int kvh,
     const int quarter = in / per, word = half * 4 + in % per;
     qs[((row / 8) * kWords + word) * 32 + (row % 8) * 4 + quarter] = make_uint4(h[0], h[1], h[2], h[3]);
   }
-  return a.scale_log2 * power_of(-up);
 }
 
 // lets `kernel` have `bytes` of dynamic shared memory, once a device (`ready` by device; twice is harmless)

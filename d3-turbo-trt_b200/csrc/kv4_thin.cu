@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
   constexpr int kKWords = D / 32, kVWords = D / 64, kTiles = D / 16;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int box[kWarps + 2];
-  __shared__ float tops[kWarps];
+  __shared__ float factors[P::kRows];  // of the query rows' products
   uint4* qs = reinterpret_cast<uint4*>(smem + (P::kRing > P::kMerge ? P::kRing : P::kMerge));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
   const int rows = a.group * a.L;
@@ -131,11 +131,11 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
     cp_commit();
     look(1);
 
-    const float q_scale = load_queries<D, NT, BF>(a, b, kvh, row0, rows, qs, tops);
+    load_queries<D, NT, BF>(a, b, kvh, row0, rows, qs, factors);
     __syncthreads();
 
     float o[NT][kTiles][4];
-    float m[NT][2], l[NT][2];
+    float m[NT][2], l[NT][2], qf[NT][2];
     int limit[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
         const int row = n * 8 + 2 * c + j;
         m[n][j] = -INFINITY;
         l[n][j] = 0.f;
+        qf[n][j] = factors[row];
         limit[n][j] = a.causal ? len - (a.L - 1 - (row0 + row) / a.group) : len;
       }
     }
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
 
       const int key0 = 16 * (my_first + now * kStride);
       const bool edge = key0 + P::kKeys > first_limit || bad_now;  // some key is masked for some row
-      float s[P::GP][NT][4], kq[P::GP][2], ev[P::GP][2];  // of keys r and r + 8: products, factor of the score, V's power
+      float s[P::GP][NT][4], kq[P::GP][2], ev[P::GP][2];  // of keys r and r + 8: products, K's power, V's
       int live[P::GP];  // tokens of the granule that are keys at all
 #pragma unroll
       for (int i = 0; i < P::GP; ++i)
@@ -233,8 +234,8 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
           }
         }
         // a marked row (255) has codes of zero: its score is 0 * infinity here
-        kq[i][0] = __uint_as_float(lds_u8(e_at + at) << 23) * q_scale;
-        kq[i][1] = __uint_as_float(lds_u8(e_at + at + 8) << 23) * q_scale;
+        kq[i][0] = __uint_as_float(lds_u8(e_at + at) << 23);
+        kq[i][1] = __uint_as_float(lds_u8(e_at + at + 8) << 23);
         ev[i][0] = exponent(lds_u8(e_at + at + P::kVe - P::kKe));
         ev[i][1] = exponent(lds_u8(e_at + at + P::kVe - P::kKe + 8));
       }
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              x[i][n][j] = fmaf(s[i][n][j], kq[i][j >> 1], -m[n][j & 1]);
+              x[i][n][j] = fmaf(s[i][n][j], kq[i][j >> 1] * qf[n][j & 1], -m[n][j & 1]);
               y[i][n][j] = x[i][n][j] + ev[i][j >> 1];
             }
         if (edge) {  // apart from the sums above, so that it is a branch and not selects in every step
@@ -285,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
               for (int h = 0; h < 2; ++h) {
                 const int key = r + 8 * h;
                 const bool in = !edge || (key < live[i] && key0 + 16 * i + key < limit[n][j]);
-                if (in) top = fmaxf(top, fmaf(s[i][n][j + 2 * h], kq[i][h], ev[i][h]));
+                if (in) top = fmaxf(top, fmaf(s[i][n][j + 2 * h], kq[i][h] * qf[n][j], ev[i][h]));
               }
             const float now = fmaxf(old, max_over_rows(top));
             const float keep = ex2(old - finite_or_zero(now));

@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
   constexpr int kRun = D / 32;                      // channels of V a lane has
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int box[kWarps + 2];
-  __shared__ float tops[kWarps];
+  __shared__ float factors[P::kRows];  // of the query rows' products
   __shared__ Unit kept;
   uint4* qs = reinterpret_cast<uint4*>(smem + P::kRing);
   uint2* ws = reinterpret_cast<uint2*>(smem + P::kRing + P::kQ);
@@ -151,11 +151,11 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
 
     if (threadIdx.x == 0)  // a dead tile has no own keys either
       kept = {b, kvh, tile, seq.tokens, seq.own, dead ? 1 : seq.cached, pieces, piece0, piece1, taken, pos, offset, seq.total};
-    const float q_scale = load_queries<D, NT, BF>(a, b, kvh, row0, rows, qs, tops);
+    load_queries<D, NT, BF>(a, b, kvh, row0, rows, qs, factors);
     __syncthreads();
 
     float o[NT][kTiles][4];
-    float m[NT][2], l[NT][2];
+    float m[NT][2], l[NT][2], qf[NT][2];
     int limit[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -168,13 +168,14 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
         const int row = n * 8 + 2 * c + j;
         m[n][j] = -INFINITY;
         l[n][j] = 0.f;
+        qf[n][j] = factors[row];
         limit[n][j] = a.causal ? len - (a.L - 1 - (row0 + row) / a.group) : len;
       }
     }
     const int first_limit = a.causal ? len - (a.L - 1) : len;
 
     // Products in s, of keys r and r + 8 of the warp's 16, to weights in shared memory; l and m follow.
-    // kq: factors of the scores; ev: powers of the V rows; masked(j, n): key r + 8 * (j >> 1) is none for
+    // kq: powers of the K rows; ev: powers of the V rows; masked(j, n): key r + 8 * (j >> 1) is none for
     // row n * 8 + 2 * c + (j & 1). `between` runs behind the first barrier.
     auto weigh = [&](const float (&s)[NT][4], const float (&kq)[2], const float (&ev)[2], bool edge, auto masked, auto between) {
       float x[NT][4], y[NT][4];  // exponents of l's terms and of the weights
@@ -183,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            x[n][j] = fmaf(s[n][j], kq[j >> 1], -m[n][j & 1]);
+            x[n][j] = fmaf(s[n][j], kq[j >> 1] * qf[n][j & 1], -m[n][j & 1]);
             y[n][j] = x[n][j] + ev[j >> 1];
           }
         if (edge) {  // apart from the sums above, so that it is a branch and not selects in every tile
@@ -212,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
             float top = -INFINITY;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              if (!edge || !masked(n, j + 2 * h)) top = fmaxf(top, fmaf(s[n][j + 2 * h], kq[h], ev[h]));
+              if (!edge || !masked(n, j + 2 * h)) top = fmaxf(top, fmaf(s[n][j + 2 * h], kq[h] * qf[n][j], ev[h]));
             top = max_over_rows(top);
             if (r == 0) maxima[warp * P::kRows + n * 8 + 2 * c + j] = top;
           }
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
       __syncthreads();
     };
 
-    float s[NT][4], kq[2];  // products of keys r and r + 8 of the warp's granule, and the scores' factors
+    float s[NT][4], kq[2];  // products of keys r and r + 8 of the warp's granule, and the K rows' powers
     auto scores = [&](uint32_t half) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -299,8 +300,8 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
         for (int n = 0; n < NT; ++n) mma16816(s[n], d0[2], d1[2], d0[3], d1[3], qv[n].z, qv[n].w);
       }
       // a marked row (255) has codes of zero: its score is 0 * infinity here
-      kq[0] = __uint_as_float(lds_u8(ke_at + half) << 23) * q_scale;
-      kq[1] = __uint_as_float(lds_u8(ke_at + half + 8) << 23) * q_scale;
+      kq[0] = __uint_as_float(lds_u8(ke_at + half) << 23);
+      kq[1] = __uint_as_float(lds_u8(ke_at + half + 8) << 23);
     };
     if (piece0 < last_cached) {
       cp_wait<1>();
@@ -452,8 +453,8 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
           mma16816(s[n], d[0][2], d[1][2], d[0][3], d[1][3], qv.z, qv.w);
         }
       }
-      kq[0] = power_of(-up_k[0]) * q_scale;
-      kq[1] = power_of(-up_k[1]) * q_scale;
+      kq[0] = power_of(-up_k[0]);
+      kq[1] = power_of(-up_k[1]);
       const float ev[2] = {-(float)up_v[0], -(float)up_v[1]};
       weigh(s, kq, ev, true, [&](int, int j) { return key0 + r + 8 * (j >> 1) >= own; }, [] {});
 #pragma unroll

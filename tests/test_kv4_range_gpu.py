@@ -1,0 +1,104 @@
+"""The 4-bit cache's attention where magnitudes lie far apart: query rows of one tile, in place and over a widened
+state. The bounds go by channel."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from conftest import ROOT  # noqa: F401  (puts the repository on sys.path)
+from test_kv4_gpu import BF, HF, half_step, new_cache, rows
+
+from d3_turbo_trt_b200 import _lib
+from d3_turbo_trt_b200.kernels import kv4
+from oracle import kv4 as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def channel_bound(out, mass, spread, top, keys, dim, dtype, widened=False):
+    """How far a kernel output may be from ``out``, channel by channel (all float64).
+
+    * the output's rounding: half a step of it, and of the subnormals' spacing;
+    * scores: a product is exact, its fp32 sum of dim terms is off by at most dim * 2^-24 of the sum of magnitudes
+      (``top`` bounds that), three fp32 factors by 2^-22 more; a score off by d changes a weight by a factor e^(2 d);
+    * weights: 2^-11 of each and 2^-25 of the largest one in fp16, so 2^-25 of |V| in this channel at most
+      (``spread`` sums it over the keys); ex2 is off by 2^-22, sums of ``keys`` terms by keys * 2^-24;
+    * over a widened state, or over its own keys, a weight has the inputs' type: half a step of it, twice.
+    """
+    weight = 2.0**-11 + 2 * top * (dim + 6) * 2.0**-24 + 2.0**-20 + keys * 2.0**-23
+    if widened:
+        weight += 2 * half_step(dtype)
+    tiny = float(torch.finfo(dtype).smallest_normal) * torch.finfo(dtype).eps
+    return out.abs() * half_step(dtype) * (1 + 2.0**-10) + mass * weight + spread * 2.0**-25 + tiny
+
+
+def check_rows(got, q, k, v, scale, widened=False):
+    """got, q [H, n, D]; k, v [Hkv, m, D]: each output row against float64."""
+    out, mass, top = ref.attention(q, k, v, scale)
+    spread = v.double().abs().sum(1, keepdim=True).repeat_interleave(q.shape[0] // v.shape[0], 0)
+    bound = channel_bound(out, mass, spread, top, k.shape[1], q.shape[-1], got.dtype, widened)
+    off = (got.cpu().double() - out).abs()
+    assert bool((off <= bound).all()), (float((off / bound).max()), float(off.max()))
+
+
+def cache_of(k, v, page, layers_seed=0):
+    """(cache, table [pages], K, V as stored [Hkv, n, D]) of rows k, v [n, Hkv, D]."""
+    n, kv_heads, dim = k.shape
+    pages = max(1, -(-n // page))
+    cache = new_cache(pages + 2, kv_heads, dim, page, seed=layers_seed)
+    table = torch.randperm(pages + 2, generator=torch.Generator().manual_seed(n))[:pages].to(torch.int32).cuda()
+    cache.append(0, k.cuda(), v.cuda(), cache.slots(table, 0, n))
+    return cache, table, ref.stored(k).transpose(0, 1), ref.stored(v).transpose(0, 1)
+
+
+def decode(q, cache, table, n, scale, causal=False):
+    return kv4.decode_attention(q.cuda(), cache, 0, table[None], torch.tensor([n], dtype=torch.int32, device="cuda"),
+                                scale=scale, causal=causal)
+
+
+# --------------------------------------------------------------------------- query rows of one tile
+@pytest.mark.parametrize("dim,group,L", [(64, 8, 1), (128, 4, 4), (256, 8, 1), (128, 8, 4), (256, 5, 5)])
+@pytest.mark.parametrize("dtype,loud,quiet", [(BF, 1e30, 1.0), (BF, -(2.0**36), 1.0), (HF, 60000.0, 2.0**-13)])
+def test_quiet_queries_beside_a_loud_one(dim, group, L, dtype, loud, quiet):
+    """One row of a tile is ``loud`` in a channel that no key has; the others keep their scores of order 1."""
+    n = 150
+    k, v = rows((n, 1, dim), dtype, 1, 0.2), rows((n, 1, dim), dtype, 2, 0.2)
+    k[..., 1] = 0
+    q = (rows((1, group, L, dim), dtype, 3, 0.2).double() * quiet).to(dtype)
+    q[0, group // 2, L // 2] = 0
+    q[0, group // 2, L // 2, 1] = loud
+    scale = dim**-0.5 / quiet
+    cache, table, ks, vs = cache_of(k, v, 32)
+    got = decode(q, cache, table, n, scale)
+    for g in range(group):
+        for i in range(L):
+            check_rows(got[0, g:g + 1, i:i + 1], q[0, g:g + 1, i:i + 1], ks, vs, scale)
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("dim,heads,L", [(64, 4, 9), (128, 8, 12), (256, 6, 20)])
+def test_padding_queries_of_any_size(monkeypatch, in_place, dim, heads, L):
+    """What stands in the query rows behind a block's length reaches no real row."""
+    monkeypatch.setattr(kv4, "_reads_codes", lambda *a: in_place)
+    kv4._plans_of.cache_clear()
+    state, lengths = 100, [L - 4, 3, 1, 0]
+    k, v = rows((state, 1, dim), BF, 1, 0.2), rows((state, 1, dim), BF, 2, 0.2)
+    cache, table, ks, vs = cache_of(k, v, 32)
+    q = rows((4, heads, L, dim), BF, 3, 0.2)
+    kq, vq = rows((4, 1, L, dim), BF, 4, 0.2), rows((4, 1, L, dim), BF, 5, 0.2)
+    pads = [1e30, -3e38] + ([math.nan, math.inf] if in_place else [])
+    for pad in pads:
+        for b, m in enumerate(lengths):
+            q[b, :, m:] = pad
+        got = kv4.question_attention(q.cuda(), cache, 0, table, state, kq.cuda(), vq.cuda(), lengths, scale=dim**-0.5)
+        for b, m in enumerate(lengths):
+            assert bool((got[b, :, m:] == 0).all())
+            if m:
+                check_rows(got[b, :, :m], q[b, :, :m], torch.cat([ks, kq[b, :, :m].double()], 1),
+                           torch.cat([vs, vq[b, :, :m].double()], 1), dim**-0.5, True)
+    kv4._plans_of.cache_clear()
+    assert _lib.device_error() == 0
