@@ -9,17 +9,25 @@
 //
 // Every thread decodes its own operand from the bytes it needs (a K row's quarter is 16 bytes at
 // D = 128), so nothing is widened in shared memory. code * scale is exact in fp16 and queries are
-// brought under a power of two a row, so S has no rounding but its fp32 sums. A V row's power of
-// two cannot be applied after the sum over keys; it goes into the weight's exponent instead:
+// brought under a power of two a row, so S has no rounding but its fp32 sums. With s_j in base 2:
 //
-//   s_j in base 2, t_j = s_j + e_j, m = max t:
-//   O = sum_j 2^(t_j - m) (code * scale)_j,  l = sum_j 2^(s_j - m),  out = O / l
+//   w_j = 2^(s_j - m),  l = sum_j w_j,  O = sum_j w_j (code * scale * 2^(e_j - E))_j,  out = O 2^E / l
 //
-// m follows the maximum only when it has to: while no t passes m by more than kRoom, weights up to
-// 2^kRoom are as exact as others (fp16 holds 2^15), and nothing is reduced over keys, rescaled or,
-// where warps share rows, exchanged. Whatever the rows' powers are, weights keep fp16's 11 bits. The terms
-// of l are fp32 numbers up to 2^64 (e >= -64); with V values beyond 2^100 the least of them fall
-// below fp32's range, keys whose weight is under 2^-9 of the largest at the very end of bf16.
+// e_j, a V row's power, goes into its scale: code * scale * 2^d is exact in fp16 for d from -14 to 4
+// (a multiple of 2^-24, at most 43008). E is one power for all of a unit's rows that a warp (thin) or a CTA
+// (wide) sees: kFirst, for rows whose largest value is 2^-10 to 2^7, or, where the first rows that are not zeros go
+// beyond that, kAbove over their largest. A step with powers outside E - 14 .. E + 4 is banded: its V rows go
+// through the products once for every band of 19 powers that has rows, each with weights under their own
+// maxima, and the fp32 sums go to O under the band's power. So a row keeps its weight whatever the others'
+// magnitudes are; what it costs is another pass over the step's codes a band, with sums of its own (64 sequences of
+// 16000 tokens, 8 rows x 128, with every 37th V row 2^30 times the others: 510 us instead of 129). Rows at the
+// least power (all values under 2^-52; rows of zeros) count as zeros where E is more than 14 above it, as it is
+// at first.
+//
+// m follows the maximum only when it has to: weights lie under 2^kHead where m has moved and may grow to
+// 2^kRoom (fp16 holds 2^15) before it moves again; until then nothing is reduced over keys, rescaled or,
+// where warps share rows, exchanged. A weight keeps fp16's 11 bits down to 2^-22 of the largest; below, it
+// is off by 2^-33 of the largest at most.
 // The weights change from accumulator to operand layout by movmatrix.
 //
 // Work is dealt out evenly whatever the lengths are: all units (sequence, kv head, tile of rows)
@@ -36,7 +44,13 @@ namespace d3b_kv4 {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr float kRoom = 12.f;
+constexpr float kHead = 8.f, kRoom = 15.f;
+// Powers of V rows are kept as their bytes (biased by 127).
+constexpr int kLeastPower = kExpMin + 127;  // of rows of zeros
+constexpr int kFirst = 119, kAbove = 3;
+constexpr int kFar = 64;           // a row that far over E moves it all the same: O stays in fp32's range
+constexpr int kMostPower = 40 + 127;  // E's largest, and the power of the partial results
+constexpr int kDown = 14, kBand = 19;  // a band: from E - kDown + kBand * k, kBand powers
 constexpr int kSiteOwnLength = 2010;  // a question block's length outside [0, L]
 
 struct AttnArgs {
@@ -92,6 +106,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void mma16816_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -132,6 +153,14 @@ __device__ __forceinline__ uint32_t lds_u16(uint32_t addr) {
   return v;
 }
 
+// a word of four rows' bytes in shared memory, of which the first `keep` stay and the others become `byte`
+__device__ __forceinline__ void keep_rows(uint32_t addr, int keep, int byte) {
+  const uint32_t mask = keep <= 0 ? 0u : keep >= 4 ? 0xFFFFFFFFu : (1u << (8 * keep)) - 1u;
+  uint32_t w[1];
+  lds_words<1>(addr, w);
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"((w[0] & mask) | ((uint32_t)byte * 0x01010101u & ~mask)) : "memory");
+}
+
 // the low half of every byte from a, the high half from b
 __device__ __forceinline__ uint32_t low_nibbles(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -161,10 +190,51 @@ struct Int {
   static constexpr int value = N;
 };
 
-// byte - 127 as a float, NaN for 255
-__device__ __forceinline__ float exponent(uint32_t byte) {
-  return byte == 255u ? __int_as_float(0x7FC00000) : __uint_as_float(0x4B000000u | byte) - 8388735.f;
+// two bytes of w to halves
+__device__ __forceinline__ uint32_t two_bytes(uint32_t w) { return __byte_perm(w, 0, 0x4140); }
+
+// two powers (halves) relative to E - kDown: those of E's band are 0 .. kBand - 1. A negative one borrows from the
+// high half and is itself out of range.
+__device__ __forceinline__ uint32_t relative(uint32_t two, int E) { return two + (uint32_t)((kDown - E) * 0x10001); }
+__device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
+__device__ __forceinline__ bool in_band(uint32_t rel) {
+  constexpr uint32_t kTop = (uint32_t)(kBand - 1) * 0x10001u;
+  return max_halves(rel, kTop) == kTop;
+}
+// fp16 factors 2^(e - E) of two powers of E's band
+__device__ __forceinline__ uint32_t band_factors(uint32_t rel) { return (rel << 10) + (uint32_t)(15 - kDown) * 0x04000400u; }
+// the factors of two powers in band k; 0 for a row of another one
+__device__ __forceinline__ uint32_t band_factors(uint32_t two, int E, int k) {
+  const int base = kDown - E - kBand * k;
+  const int lo = (int)(two & 0xFFFFu) + base, hi = (int)(two >> 16) + base;
+  return (lo >= 0 && lo < kBand ? (uint32_t)(lo + 15 - kDown) << 10 : 0u) |
+         (hi >= 0 && hi < kBand ? (uint32_t)(hi + 15 - kDown) << 26 : 0u);
+}
+__device__ __forceinline__ int band_of(int e, int E) { return (e - E + kDown + kBand * 16) / kBand - 16; }
+
+// E after rows of power `top` at most; first: no row but those of zeros came before
+__device__ __forceinline__ int next_power(int E, int top, bool first) {
+  return top > kLeastPower && (first || top > E + kFar) ? min(top + kAbove, kMostPower) : E;
+}
+
+// What a step's rows span, marked rows and those at the least power apart: the largest power (0: no row) and the
+// smallest (255).
+struct Span {
+  int most, least;
+  __device__ __forceinline__ void add(uint32_t two) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int e = (two >> (16 * h)) & 0xFF;
+      if (e == 255 || e == kLeastPower) continue;
+      most = max(most, e);
+      least = min(least, e);
+    }
+  }
+};
 
 // the power of two that brings a row's largest magnitude to [2^14, 2^15), as far as 2^126 goes; rows
 // that are not finite stay
@@ -183,14 +253,14 @@ __device__ __forceinline__ void add_part(float4& acc, float& sum, const float4 o
   acc.w = fmaf(o.w, f, acc.w);
 }
 
-// four channels of a finished row; zeros where there was no key or the token is behind its block's length
+// four channels of a finished row, sums under 2^(kMostPower - 127); zeros where there was no key or the token is behind its block's length
 template <bool BF>
 __device__ __forceinline__ void store_row(const AttnArgs& a, int b, int kvh, int row, int tokens, int d, const float4 acc,
                                           float sum) {
   const int l = row / a.group, h = kvh * a.group + row % a.group;
   uint32_t lo = 0, hi = 0;
   if (sum != 0.f && l < tokens) {
-    const float f = 1.f / sum;
+    const float f = __uint_as_float((uint32_t)kMostPower << 23) / sum;
     lo = narrow<BF>(acc.x * f) | ((uint32_t)narrow<BF>(acc.y * f) << 16);
     hi = narrow<BF>(acc.z * f) | ((uint32_t)narrow<BF>(acc.w * f) << 16);
   }

@@ -47,6 +47,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int box[kWarps + 2];
   __shared__ float factors[P::kRows];  // of the query rows' products
+  __shared__ int zero_steps[kWarps];   // steps from a warp's first on without a V row that counts
   uint4* qs = reinterpret_cast<uint4*>(smem + (P::kRing > P::kMerge ? P::kRing : P::kMerge));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
   const int rows = a.group * a.L;
@@ -161,9 +162,12 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
         for (int w = 0; w < kKWords; ++w) qr[n][w] = qs[(n * kKWords + w) * 32 + lane];
     }
     const int first_limit = a.causal ? len - (a.L - 1) : len;
+    int E = kFirst;  // the sums' power
+    if (lane == 0) zero_steps[warp] = 0;
+    __syncwarp();
     const uint32_t k_at = ring + P::kKc + r * (D / 2) + c * (D == 256 ? 16 : D / 8);
     const uint32_t ks_at = ring + P::kKs + r * (D / 16) + (D == 64 ? c : 2 * c);
-    const uint32_t e_at = ring + P::kKe + r;
+    const uint32_t e_at = ring + P::kKe + r, ve_at = ring + P::kVe + 2 * c;
     const uint32_t vs_at = ring + P::kVs + (D == 64 ? r / 2 : D == 128 ? r : 2 * r) * 16 + 2 * c;
     uint32_t v_at[4];  // V rows 2c, 2c + 1, 2c + 8, 2c + 9
 #pragma unroll
@@ -181,11 +185,21 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
 
       const int key0 = 16 * (my_first + now * kStride);
       const bool edge = key0 + P::kKeys > first_limit || bad_now;  // some key is masked for some row
-      float s[P::GP][NT][4], kq[P::GP][2], ev[P::GP][2];  // of keys r and r + 8: products, K's power, V's
+      float s[P::GP][NT][4], kq[P::GP][2];  // of keys r and r + 8: products, K's power
       int live[P::GP];  // tokens of the granule that are keys at all
 #pragma unroll
       for (int i = 0; i < P::GP; ++i)
         live[i] = edge ? ((bad_now >> i) & 1 ? 0 : min(16, len - key0 - 16 * i)) : 16;
+      if (edge) {
+        // V rows that are no keys may never have been written: their scales, which can be NaN, become zero and
+        // their powers E
+#pragma unroll
+        for (int i = 0; i < P::GP; ++i)
+          for (int at = lane; at < D / 4 + 4 && live[i] < 16; at += 32)
+            keep_rows(ring + kAt + i * P::kStage + (at < D / 4 ? P::kVs + 4 * at : P::kVe + 4 * (at - D / 4)),
+                      live[i] - 4 * (at & 3), at < D / 4 ? 0 : E);
+        __syncwarp();
+      }
 #pragma unroll
       for (int i = 0; i < P::GP; ++i) {
         const int at = kAt + i * P::kStage;
@@ -236,12 +250,23 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
         // a marked row (255) has codes of zero: its score is 0 * infinity here
         kq[i][0] = __uint_as_float(lds_u8(e_at + at) << 23);
         kq[i][1] = __uint_as_float(lds_u8(e_at + at + 8) << 23);
-        ev[i][0] = exponent(lds_u8(e_at + at + P::kVe - P::kKe));
-        ev[i][1] = exponent(lds_u8(e_at + at + P::kVe - P::kKe + 8));
       }
 
-      // exponents of l's terms and of the weights, masked keys at -infinity
-      float x[P::GP][NT][4], y[P::GP][NT][4];
+      // powers of V rows 2c, 2c + 1 and 2c + 8, 2c + 9
+      auto powers = [&](int i, int h) { return two_bytes(lds_u16(ve_at + kAt + i * P::kStage + 8 * h)); };
+      uint32_t vf[P::GP][2], worst = 0;  // their factors
+#pragma unroll
+      for (int i = 0; i < P::GP; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t rel = relative(powers(i, h), E);
+          worst = max_halves(worst, rel);
+          vf[i][h] = band_factors(rel);
+        }
+      const bool odd = !in_band(worst);
+
+      // exponents of the weights, masked keys at -infinity
+      float x[P::GP][NT][4];
       auto exponents = [&] {
 #pragma unroll
         for (int i = 0; i < P::GP; ++i)
@@ -250,7 +275,6 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               x[i][n][j] = fmaf(s[i][n][j], kq[i][j >> 1] * qf[n][j & 1], -m[n][j & 1]);
-              y[i][n][j] = x[i][n][j] + ev[i][j >> 1];
             }
         if (edge) {  // apart from the sums above, so that it is a branch and not selects in every step
 #pragma unroll
@@ -260,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const int key = r + 8 * (j >> 1);
-                if (key >= live[i] || key0 + 16 * i + key >= limit[n][j & 1]) x[i][n][j] = y[i][n][j] = -INFINITY;
+                if (key >= live[i] || key0 + 16 * i + key >= limit[n][j & 1]) x[i][n][j] = -INFINITY;
               }
         }
         float most = -INFINITY;
@@ -269,11 +293,72 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) most = fmaxf(most, y[i][n][j]);
+            for (int j = 0; j < 4; ++j) most = fmaxf(most, x[i][n][j]);
         return most;
       };
+      // V's rows under factors `f` as operands: use(granule, 16-channel tile, a0 .. a3)
+      auto values = [&](const uint32_t (&f)[P::GP][2], auto use) {
+#pragma unroll
+        for (int i = 0; i < P::GP; ++i) {
+          const int at = kAt + i * P::kStage;
+          uint32_t v[4][kVWords];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) lds_words<kVWords>(v_at[x] + at, v[x]);
+          uint32_t sc01 = 0, sc89 = 0;
+#pragma unroll
+          for (int w = 0; w < kVWords; ++w) {
+            if (w == 0 || (D == 256 && w == 2)) {
+              sc01 = hmul2(decode_scales(lds_u16(vs_at + at + 8 * w)), f[i][0]);
+              sc89 = hmul2(decode_scales(lds_u16(vs_at + at + 8 * w + 8)), f[i][1]);
+            }
+            uint32_t x0[4], x1[4], y0[4], y1[4];
+            decode8(low_nibbles(v[0][w], v[1][w] << 4), x0);
+            decode8(low_nibbles(v[0][w] >> 4, v[1][w]), x1);
+            decode8(low_nibbles(v[2][w], v[3][w] << 4), y0);
+            decode8(low_nibbles(v[2][w] >> 4, v[3][w]), y1);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              use(i, 4 * w + x, hmul2(x0[x], sc01), hmul2(x1[x], sc01), hmul2(y0[x], sc89), hmul2(y1[x], sc89));
+          }
+        }
+      };
+      uint32_t wf[P::GP][NT][2];
       // m = -infinity (no key yet) makes every exponent +infinity
-      if (__any_sync(0xffffffffu, exponents() > kRoom)) {
+      if (__any_sync(0xffffffffu, exponents() > kRoom || odd)) {
+        int band0 = 0, band1 = 0;  // the step's bands; the common products below are those of band 0
+        if (__any_sync(0xffffffffu, odd)) {
+          Span span = {0, 255};
+#pragma unroll
+          for (int i = 0; i < P::GP; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (lds_u8(e_at + kAt + i * P::kStage + P::kVe - P::kKe + 8 * h) == 255u) kq[i][h] = __int_as_float(0x7FC00000);
+              span.add(powers(i, h));
+            }
+          span.most = (int)__reduce_max_sync(0xffffffffu, (uint32_t)span.most);
+          span.least = (int)__reduce_min_sync(0xffffffffu, (uint32_t)span.least);
+          const int zeros = zero_steps[warp], to = next_power(E, span.most, zeros == now);
+          __syncwarp();
+          if (lane == 0 && span.most == 0) zero_steps[warp] = zeros + 1;
+          __syncwarp();
+          if (to != E) {
+            const float by = power_of(E - to);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int z = 0; z < kTiles; ++z)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[n][z][j] *= by;
+          }
+          // what is no key has the old E: a row of zeros
+#pragma unroll
+          for (int i = 0; i < P::GP; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) vf[i][h] = band_factors(powers(i, h), to, 0);
+          E = to;
+          band0 = min(band_of(span.least, E), 0);
+          band1 = max(band_of(span.most, E), 0);
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -286,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
               for (int h = 0; h < 2; ++h) {
                 const int key = r + 8 * h;
                 const bool in = !edge || (key < live[i] && key0 + 16 * i + key < limit[n][j]);
-                if (in) top = fmaxf(top, fmaf(s[i][n][j + 2 * h], kq[i][h] * qf[n][j], ev[i][h]));
+                if (in) top = fmaxf(top, fmaf(s[i][n][j + 2 * h], kq[i][h] * qf[n][j], -kHead));
               }
             const float now = fmaxf(old, max_over_rows(top));
             const float keep = ex2(old - finite_or_zero(now));
@@ -299,52 +384,90 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
             }
           }
         exponents();
+        if (band0 != band1) {
+#pragma unroll 1
+          for (int k = band0; k <= band1; ++k) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int i = 0; i < P::GP; ++i)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) any |= vf[i][h] = band_factors(powers(i, h), E, k);
+            if (k == 0 || !__any_sync(0xffffffffu, any)) continue;
+            // the weights of the band's rows under their own largest one, and what brings a sum of theirs to O
+            bool mine[P::GP][2];
+#pragma unroll
+            for (int i = 0; i < P::GP; ++i)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int e = (int)lds_u8(e_at + kAt + i * P::kStage + P::kVe - P::kKe + 8 * h);
+                mine[i][h] = r + 8 * h < live[i] && band_of(e, E) == k;
+              }
+            float to[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              float under[2];
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < P::GP; ++i)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h)
+                    if (mine[i][h]) top = fmaxf(top, x[i][n][j + 2 * h]);
+                under[j] = finite_or_zero(max_over_rows(top));
+                to[n][j] = ex2(under[j] + (float)(kBand * k));
+              }
+#pragma unroll
+              for (int i = 0; i < P::GP; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  float w0 = 0.f, w1 = 0.f;
+                  if (mine[i][h]) {
+                    float &x0 = x[i][n][2 * h], &x1 = x[i][n][2 * h + 1];
+                    l[n][0] += ex2(x0);
+                    l[n][1] += ex2(x1);
+                    w0 = ex2(x0 - under[0]);
+                    w1 = ex2(x1 - under[1]);
+                    x0 = x1 = -INFINITY;  // done
+                  }
+                  const __half2 w = __floats2half2_rn(w0, w1);
+                  wf[i][n][h] = transpose8x8(*reinterpret_cast<const uint32_t*>(&w));
+                }
+            }
+            values(vf, [&](int i, int tile, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                mma16816(part, a0, a1, a2, a3, wf[i][n][0], wf[i][n][1]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[n][tile][j] = fmaf(part[j], to[n][j & 1], o[n][tile][j]);
+              }
+            });
+          }
+#pragma unroll
+          for (int i = 0; i < P::GP; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) vf[i][h] = band_factors(powers(i, h), E, 0);
+        }
       }
-      uint32_t wf[P::GP][NT][2];
 #pragma unroll
       for (int i = 0; i < P::GP; ++i)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+          float w[4];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) l[n][j] += ex2(x[i][n][j]) + ex2(x[i][n][j + 2]);
+          for (int j = 0; j < 4; ++j) w[j] = ex2(x[i][n][j]);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const __half2 h = __floats2half2_rn(ex2(y[i][n][2 * j]), ex2(y[i][n][2 * j + 1]));
+            l[n][j] += w[j] + w[j + 2];
+            const __half2 h = __floats2half2_rn(w[2 * j], w[2 * j + 1]);
             wf[i][n][j] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h));
           }
         }
-
+      values(vf, [&](int i, int tile, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
-      for (int i = 0; i < P::GP; ++i) {
-        const int at = kAt + i * P::kStage;
-        uint32_t v[4][kVWords];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) lds_words<kVWords>(v_at[x] + at, v[x]);
-        uint32_t sc01 = 0, sc89 = 0;
-#pragma unroll
-        for (int w = 0; w < kVWords; ++w) {
-          if (w == 0 || (D == 256 && w == 2)) {
-            uint32_t b01 = lds_u16(vs_at + at + 8 * w), b89 = lds_u16(vs_at + at + 8 * w + 8);
-            if (edge) {  // a granule's last rows may never have been written: their scales can be NaN
-              b01 &= (2 * c < live[i] ? 0xFFu : 0u) | (2 * c + 1 < live[i] ? 0xFF00u : 0u);
-              b89 &= (2 * c + 8 < live[i] ? 0xFFu : 0u) | (2 * c + 9 < live[i] ? 0xFF00u : 0u);
-            }
-            sc01 = decode_scales(b01);
-            sc89 = decode_scales(b89);
-          }
-          uint32_t x0[4], x1[4], y0[4], y1[4];
-          decode8(low_nibbles(v[0][w], v[1][w] << 4), x0);
-          decode8(low_nibbles(v[0][w] >> 4, v[1][w]), x1);
-          decode8(low_nibbles(v[2][w], v[3][w] << 4), y0);
-          decode8(low_nibbles(v[2][w] >> 4, v[3][w]), y1);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const uint32_t a0 = hmul2(x0[x], sc01), a1 = hmul2(x1[x], sc01), a2 = hmul2(y0[x], sc89), a3 = hmul2(y1[x], sc89);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816(o[n][4 * w + x], a0, a1, a2, a3, wf[i][n][0], wf[i][n][1]);
-          }
-        }
-      }
+        for (int n = 0; n < NT; ++n) mma16816(o[n][tile], a0, a1, a2, a3, wf[i][n][0], wf[i][n][1]);
+      });
       bad_now = bad_next;
     };
     for (int now = 0; now < steps; now += kDepth) {
@@ -357,6 +480,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
     __syncthreads();
     float* mo = reinterpret_cast<float*>(smem);   // [warp][row][D]
     float* ms = mo + kWarps * P::kRows * D;       // [warp][row][2]
+    const float to_part = power_of(E - kMostPower);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -371,7 +495,8 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
 #pragma unroll
         for (int x = 0; x < kTiles; x += 2)
           *reinterpret_cast<float4*>(dst + 2 * x) =
-              make_float4(o[n][x][j], o[n][x][j + 2], o[n][x + 1][j], o[n][x + 1][j + 2]);
+              make_float4(o[n][x][j] * to_part, o[n][x][j + 2] * to_part, o[n][x + 1][j] * to_part,
+                          o[n][x + 1][j + 2] * to_part);
       }
     __syncthreads();
     const bool whole = piece0 == 0 && piece1 == seq.pieces;

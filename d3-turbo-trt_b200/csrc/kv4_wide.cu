@@ -7,8 +7,8 @@
 // decoded once too and O is 1/4 of the rows' channels in a warp's registers. Two barriers a tile:
 // maxima, weights.
 //
-// A block's own keys are tiles of the same kind whose operands come from the 16-bit rows: brought
-// under a power of two a row, so that bf16 values fit fp16 without rounding.
+// A block's own keys are tiles of the same kind whose operands come from the 16-bit rows: K brought under a
+// power of two a row, so that bf16 values fit fp16 without rounding, V as it is.
 //
 // Bound: products. 32 rows x 64 keys are 2 D m16n8k16, 8 clocks each on one of four tensor pipes; at D = 256 they
 // take 1.3 times as long as the cache's bytes, and the chain conversion, product with the scale, matrix
@@ -36,13 +36,11 @@ struct Wide {
   static constexpr int kQ = kRows * D * 2;
   static constexpr int kW = 4 * NT * 32 * 8;    // weights: [granule][nt][lane] x 8 bytes
   static constexpr int kMax = kWarps * kRows * 4;
-  static constexpr int kSmem = kRing + kQ + kW + kMax + kKeys * 4;
+  static constexpr int kFactors = kKeys * 2;  // of the V rows: [granule][pair of rows] x 4 bytes
+  static constexpr int kSmem = kRing + kQ + kW + kMax + kFactors;
   static constexpr int kScales = off_k_scale(D), kExps = off_k_exp(D);  // within a stage, after the codes
 };
 
-__device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -61,11 +59,12 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int box[kWarps + 2];
   __shared__ float factors[P::kRows];  // of the query rows' products
+  __shared__ Span spans[kWarps];
   __shared__ Unit kept;
   uint4* qs = reinterpret_cast<uint4*>(smem + P::kRing);
   uint2* ws = reinterpret_cast<uint2*>(smem + P::kRing + P::kQ);
   float* maxima = reinterpret_cast<float*>(smem + P::kRing + P::kQ + P::kW);  // [warp][row]
-  float* own_scale = maxima + kWarps * P::kRows;  // [key]: what an own V row is multiplied by
+  uint32_t* vfs = reinterpret_cast<uint32_t*>(maxima + kWarps * P::kRows);  // [granule][pair of V rows]: their factors
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
   const int rows = a.group * a.L;
   Deal mine = deal<kKeys, P::kRows, 1, P::kStart>(a, 1, box);
@@ -84,7 +83,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
   }
   const uint32_t k_at = k_ring + warp * P::kStage + r * (D / 2) + c * (D == 256 ? 16 : D / 8);
   const uint32_t ks_at = k_ring + warp * P::kStage + P::kScales + r * (D / 16) + (D == 64 ? c : 2 * c);
-  const uint32_t ke_at = k_ring + warp * P::kStage + P::kExps + r, ve_at = v_ring + warp * P::kStage + P::kExps + r;
+  const uint32_t ke_at = k_ring + warp * P::kStage + P::kExps + r, ve_at = v_ring + P::kExps;
   // V: channels warp * D/4 + r * D/32 ...; rows 2c, 2c + 1, 2c + 8, 2c + 9 of every granule
   uint32_t v_at[4];
 #pragma unroll
@@ -174,86 +173,76 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
     }
     const int first_limit = a.causal ? len - (a.L - 1) : len;
 
-    // Products in s, of keys r and r + 8 of the warp's 16, to weights in shared memory; l and m follow.
-    // kq: powers of the K rows; ev: powers of the V rows; masked(j, n): key r + 8 * (j >> 1) is none for
-    // row n * 8 + 2 * c + (j & 1). `between` runs behind the first barrier.
-    auto weigh = [&](const float (&s)[NT][4], const float (&kq)[2], const float (&ev)[2], bool edge, auto masked, auto between) {
-      float x[NT][4], y[NT][4];  // exponents of l's terms and of the weights
-      auto exponents = [&] {
+    int E = kFirst, zero_tiles = 0;  // the sums' power, the same in every warp; tiles from the first on without a row that counts
+    float s[NT][4], kq[2];  // products of keys r and r + 8 of the warp's granule, and the K rows' powers
+    float x[NT][4];         // the weights' exponents
+    // masked(n, j): key r + 8 * (j >> 1) is none for row n * 8 + 2 * c + (j & 1)
+    auto exponents = [&](bool edge, auto masked) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[n][j] = fmaf(s[n][j], kq[j >> 1] * qf[n][j & 1], -m[n][j & 1]);
+      if (edge) {  // apart from the sums above, so that it is a branch and not selects in every tile
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[n][j] = fmaf(s[n][j], kq[j >> 1] * qf[n][j & 1], -m[n][j & 1]);
-            y[n][j] = x[n][j] + ev[j >> 1];
-          }
-        if (edge) {  // apart from the sums above, so that it is a branch and not selects in every tile
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (masked(n, j)) x[n][j] = y[n][j] = -INFINITY;
-        }
-        float most = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) most = fmaxf(most, y[n][j]);
-        return most;
-      };
-      // m = -infinity (no key yet) makes every exponent +infinity. Behind this barrier every warp's copies have
-      // landed and its work on the other half is done.
-      const bool move = __syncthreads_or(exponents() > kRoom);
-      between();
-      if (move) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float top = -INFINITY;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              if (!edge || !masked(n, j + 2 * h)) top = fmaxf(top, fmaf(s[n][j + 2 * h], kq[h] * qf[n][j], ev[h]));
-            top = max_over_rows(top);
-            if (r == 0) maxima[warp * P::kRows + n * 8 + 2 * c + j] = top;
-          }
-        __syncthreads();
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float2 top = make_float2(m[n][0], m[n][1]);
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            const float2 z = *reinterpret_cast<const float2*>(maxima + w * P::kRows + n * 8 + 2 * c);
-            top.x = fmaxf(top.x, z.x);
-            top.y = fmaxf(top.y, z.y);
-          }
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float now = j ? top.y : top.x, keep = ex2(m[n][j] - finite_or_zero(now));
-            m[n][j] = now;
-            l[n][j] *= keep;
-#pragma unroll
-            for (int z = 0; z < kTiles; ++z) {
-              o[n][z][j] *= keep;
-              o[n][z][j + 2] *= keep;
-            }
-          }
-        }
-        exponents();
+          for (int j = 0; j < 4; ++j)
+            if (masked(n, j)) x[n][j] = -INFINITY;
       }
+      float most = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) most = fmaxf(most, x[n][j]);
+      return most;
+    };
+    // the warp's maxima for `settle`, behind a barrier
+    auto offer = [&](bool edge, auto masked) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (!edge || !masked(n, j + 2 * h)) top = fmaxf(top, fmaf(s[n][j + 2 * h], kq[h] * qf[n][j], -kHead));
+          top = max_over_rows(top);
+          if (r == 0) maxima[warp * P::kRows + n * 8 + 2 * c + j] = top;
+        }
+    };
+    // m moved to the warps' maxima
+    auto settle = [&] {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        float2 top = make_float2(m[n][0], m[n][1]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) l[n][j] += ex2(x[n][j]) + ex2(x[n][j + 2]);
-        uint2 w;
-        w.x = transpose8x8(pack_half2(ex2(y[n][0]), ex2(y[n][1])));
-        w.y = transpose8x8(pack_half2(ex2(y[n][2]), ex2(y[n][3])));
-        ws[(warp * NT + n) * 32 + lane] = w;
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 z = *reinterpret_cast<const float2*>(maxima + w * P::kRows + n * 8 + 2 * c);
+          top.x = fmaxf(top.x, z.x);
+          top.y = fmaxf(top.y, z.y);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float now = j ? top.y : top.x, keep = ex2(m[n][j] - finite_or_zero(now));
+          m[n][j] = now;
+          l[n][j] *= keep;
+#pragma unroll
+          for (int z = 0; z < kTiles; ++z) {
+            o[n][z][j] *= keep;
+            o[n][z][j + 2] *= keep;
+          }
+        }
       }
-      __syncthreads();
+    };
+    auto rescale = [&](float by) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int z = 0; z < kTiles; ++z)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[n][z][j] *= by;
     };
 
-    float s[NT][4], kq[2];  // products of keys r and r + 8 of the warp's granule, and the K rows' powers
     auto scores = [&](uint32_t half) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -313,54 +302,49 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
       cp_wait<0>();  // V of this tile and K of the next
       __syncwarp();
       const int key0 = 64 * p + 16 * warp;
+      const uint32_t mine = ve_at + warp * P::kStage + half;  // the powers of the warp's own V rows
       if (live_now < 16) {
         // rows that were never written may have scales that are not numbers: their weights are zero,
-        // their values have to be finite
-        for (int i = lane; i < D / 4; i += 32) {
-          const int keep = live_now - 4 * (i & 3);  // bytes of the word that are of keys
-          const uint32_t at = v_ring + warp * P::kStage + half + P::kScales + 4 * i;
-          uint32_t v[1];
-          lds_words<1>(at, v);
-          sts32(at, keep <= 0 ? 0u : keep >= 4 ? v[0] : v[0] & ((1u << (8 * keep)) - 1u));
-        }
+        // their values have to be finite; their powers are set to E
+        for (int i = lane; i < D / 4 + 4; i += 32)
+          keep_rows(v_ring + warp * P::kStage + half + P::kScales + 4 * i, live_now - 4 * (i & 3), i < D / 4 ? 0 : E);
+        __syncwarp();
       }
-      const float ev[2] = {exponent(lds_u8(ve_at + half)), exponent(lds_u8(ve_at + half + 8))};
       auto masked = [&](int n, int j) {
         const int key = r + 8 * (j >> 1);
         return key >= live_now || key0 + key >= limit[n][j & 1];
       };
-      weigh(s, kq, ev, live_now < 16 || key0 + 16 > first_limit, masked, [&] {
-        load_v(p + 1, id_v, kHalfRing - half);
-        live_after = load_k(p + 2, id_k, half);
-        cp_commit();
-        id_v = id_k;
-        id_k = look(p + 3);
-      });
-      // the next tile's scores beside this one's values: they have nothing to do with each other, and behind
-      // the last tile the former are of whatever lies there and not used
-      scores(kHalfRing - half);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      const bool edge = live_now < 16 || key0 + 16 > first_limit;
+      // rows 2 (lane % 8) and the one behind it
+      const uint32_t rel = relative(two_bytes(lds_u16(mine + 2 * (lane & 7))), E);
+      const bool odd = !in_band(rel);
+      // Behind this barrier every warp's copies have landed and its work on the other half is done. m = -infinity (no key
+      // yet) makes every exponent +infinity.
+      const bool move = __syncthreads_or(exponents(edge, masked) > kRoom || odd);
+      if (lane < 8) vfs[8 * warp + lane] = band_factors(rel);
+      load_v(p + 1, id_v, kHalfRing - half);
+      live_after = load_k(p + 2, id_k, half);
+      cp_commit();
+      id_v = id_k;
+      id_k = look(p + 3);
+      // V's rows of granule i under factors of its pairs as operands: use(16-channel tile, a0 .. a3)
+      auto values = [&](int i, uint32_t f01, uint32_t f89, auto use) {
         const uint32_t at = half + i * P::kStage;
-        const uint32_t sc01 = decode_scales(lds_u16(vs_at + at)), sc89 = decode_scales(lds_u16(vs_at + at + 8));
-        uint2 wf[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) wf[n] = ws[(i * NT + n) * 32 + lane];
-        auto add = [&](int x, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-          a0 = hmul2(a0, sc01), a1 = hmul2(a1, sc01), a2 = hmul2(a2, sc89), a3 = hmul2(a3, sc89);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816(o[n][x], a0, a1, a2, a3, wf[n].x, wf[n].y);
+        const uint32_t sc01 = hmul2(decode_scales(lds_u16(vs_at + at)), f01);
+        const uint32_t sc89 = hmul2(decode_scales(lds_u16(vs_at + at + 8)), f89);
+        auto add = [&](int t, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+          use(t, hmul2(a0, sc01), hmul2(a1, sc01), hmul2(a2, sc89), hmul2(a3, sc89));
         };
         if constexpr (D == 256) {  // 8 channels a lane: one word of each row
           uint32_t v[4], x0[4], x1[4], y0[4], y1[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) lds_words<1>(v_at[x] + at, v + x);
+          for (int z = 0; z < 4; ++z) lds_words<1>(v_at[z] + at, v + z);
           decode8(low_nibbles(v[0], v[1] << 4), x0);
           decode8(low_nibbles(v[0] >> 4, v[1]), x1);
           decode8(low_nibbles(v[2], v[3] << 4), y0);
           decode8(low_nibbles(v[2] >> 4, v[3]), y1);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) add(x, x0[x], x1[x], y0[x], y1[x]);
+          for (int z = 0; z < 4; ++z) add(z, x0[z], x1[z], y0[z], y1[z]);
         } else if constexpr (D == 128) {  // 4 channels: two bytes of each row, two rows a word
           const uint32_t u = lds_u16(v_at[0] + at) | (lds_u16(v_at[2] + at) << 16);
           const uint32_t w = lds_u16(v_at[1] + at) | (lds_u16(v_at[3] + at) << 16);
@@ -376,6 +360,112 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
           decode8((low_nibbles(u, w << 4) & 0xFFFFu) | (low_nibbles(u >> 4, w) << 16), x0);
           add(0, x0[0], x0[2], x0[1], x0[3]);
         }
+      };
+      if (move) {
+        Span span = {0, 255};
+        span.add(two_bytes(lds_u16(mine + 2 * (lane & 7))));
+        span.most = (int)__reduce_max_sync(0xffffffffu, (uint32_t)span.most);
+        span.least = (int)__reduce_min_sync(0xffffffffu, (uint32_t)span.least);
+        if (lane == 0) spans[warp] = span;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (lds_u8(mine + r + 8 * h) == 255u) kq[h] = __int_as_float(0x7FC00000);
+        offer(edge, masked);
+        __syncthreads();
+        settle();
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          span.most = max(span.most, spans[w].most);
+          span.least = min(span.least, spans[w].least);
+        }
+        const int to = next_power(E, span.most, zero_tiles == p - piece0);
+        zero_tiles += span.most == 0;
+        if (to != E) rescale(power_of(E - to));
+        E = to;
+        const int band0 = min(band_of(span.least, E), 0);
+        const int band1 = max(band_of(span.most, E), 0);
+        if (lane < 8) vfs[8 * warp + lane] = band_factors(two_bytes(lds_u16(mine + 2 * lane)), E, 0);
+        exponents(edge, masked);
+        if (band0 != band1) {  // the common products below are those of band 0
+#pragma unroll 1
+          for (int k = band0; k <= band1; ++k) {
+            // weights of the granule's rows in the band under their own largest one, and what brings their sums to O
+            bool in[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              in[h] = k != 0 && r + 8 * h < live_now && band_of((int)lds_u8(mine + r + 8 * h), E) == k;
+            if (!__syncthreads_or(in[0] || in[1])) continue;  // and the weights and factors are free
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              float under[2];
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  if (in[h]) top = fmaxf(top, x[n][j + 2 * h]);
+                under[j] = finite_or_zero(max_over_rows(top));
+                if (r == 0) maxima[warp * P::kRows + n * 8 + 2 * c + j] = ex2(under[j] + (float)(kBand * k));
+              }
+              uint32_t w[2];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                float w0 = 0.f, w1 = 0.f;
+                if (in[h]) {
+                  float &x0 = x[n][2 * h], &x1 = x[n][2 * h + 1];
+                  l[n][0] += ex2(x0);
+                  l[n][1] += ex2(x1);
+                  w0 = ex2(x0 - under[0]);
+                  w1 = ex2(x1 - under[1]);
+                  x0 = x1 = -INFINITY;  // done
+                }
+                w[h] = transpose8x8(pack_half2(w0, w1));
+              }
+              ws[(warp * NT + n) * 32 + lane] = make_uint2(w[0], w[1]);
+            }
+            if (lane < 8) vfs[8 * warp + lane] = band_factors(two_bytes(lds_u16(mine + 2 * lane)), E, k);
+            __syncthreads();
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i)
+              values(i, vfs[8 * i + c], vfs[8 * i + 4 + c], [&](int t, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  const uint2 w = ws[(i * NT + n) * 32 + lane];
+                  const float2 to = *reinterpret_cast<const float2*>(maxima + i * P::kRows + n * 8 + 2 * c);
+                  float part[4] = {0.f, 0.f, 0.f, 0.f};
+                  mma16816(part, a0, a1, a2, a3, w.x, w.y);
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) o[n][t][j] = fmaf(part[j], j & 1 ? to.y : to.x, o[n][t][j]);
+                }
+              });
+          }
+          __syncthreads();  // the weights and factors are free
+          if (lane < 8) vfs[8 * warp + lane] = band_factors(two_bytes(lds_u16(mine + 2 * lane)), E, 0);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = ex2(x[n][j]);
+        l[n][0] += w[0] + w[2];
+        l[n][1] += w[1] + w[3];
+        ws[(warp * NT + n) * 32 + lane] =
+            make_uint2(transpose8x8(pack_half2(w[0], w[1])), transpose8x8(pack_half2(w[2], w[3])));
+      }
+      __syncthreads();
+      // the next tile's scores beside this one's values: they have nothing to do with each other, and behind
+      // the last tile the former are of whatever lies there and not used
+      scores(kHalfRing - half);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint2 wf[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) wf[n] = ws[(i * NT + n) * 32 + lane];
+        values(i, vfs[8 * i + c], vfs[8 * i + 4 + c], [&](int t, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816(o[n][t], a0, a1, a2, a3, wf[n].x, wf[n].y);
+        });
       }
       live_now = live_next;
       live_next = live_after;
@@ -384,48 +474,48 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
 
     const volatile Unit& u = kept;  // read where it is needed, not held
 
-    // the block's own keys
+    // The block's own keys. V's rows are operands as they are, in the inputs' type, so O goes under the power of the
+    // partial results and takes each product's fp32 sums times 2^(127 - kMostPower). In bf16 a weight is the sum of two
+    // bf16 numbers, both above zero (an infinity times either is one), under 2^-kSmall so that no product of
+    // finite numbers leaves fp32; rows of V below 2^-90 count as zeros.
+    constexpr int kSmall = BF ? 20 : 0;
+    uint2* ws_low = reinterpret_cast<uint2*>(smem);  // the smaller numbers, where the ring was
     for (int p = max(u.piece0, u.cached); p < u.piece1 && a.k_own; ++p) {
       const int own = u.own, cached = u.cached;
       const int key0 = 64 * (p - cached) + 16 * warp;  // the warp's 16 keys
       if (64 * (p - cached) >= own) break;         // a unit without any key has one empty piece
       const uint16_t* k_base = a.k_own + u.b * a.sk_b + u.kvh * a.sk_h;
       const uint16_t* v_base = a.v_own + u.b * a.sv_b + u.kvh * a.sv_h;
+      if (E != kMostPower) {
+        rescale(power_of(E - kMostPower));
+        E = kMostPower;
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[n][j] = 0.f;
-      int up_k[2] = {0, 0}, up_v[2] = {0, 0};  // of keys r and r + 8
+      int up_k[2] = {0, 0};  // of keys r and r + 8
       auto channel = [&](int w) { return D == 256 ? 128 * (w / 4) + 32 * c + 8 * (w % 4) : c * (D / 4) + 8 * w; };
-      auto fetch = [&](const uint16_t* base, int64_t stride, int i, int w) {
+      auto fetch = [&](int i, int w) {
         const int key = key0 + r + 8 * i;
-        return key < own ? __ldg(reinterpret_cast<const uint4*>(base + key * stride + channel(w))) : make_uint4(0, 0, 0, 0);
+        return key < own ? __ldg(reinterpret_cast<const uint4*>(k_base + key * a.sk_l + channel(w))) : make_uint4(0, 0, 0, 0);
       };
+      if constexpr (BF) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float top_k = 0.f, top_v = 0.f;
-        if constexpr (BF) {
+        for (int i = 0; i < 2; ++i) {
+          float top = 0.f;
 #pragma unroll
           for (int w = 0; w < kKWords; ++w) {
-            const uint4 k4 = fetch(k_base, a.sk_l, i, w), v4 = fetch(v_base, a.sv_l, i, w);
-            const uint32_t kw[4] = {k4.x, k4.y, k4.z, k4.w}, vw[4] = {v4.x, v4.y, v4.z, v4.w};
+            const uint4 k4 = fetch(i, w);
+            const uint32_t kw[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const float2 fk = widen2<BF>(kw[j]), fv = widen2<BF>(vw[j]);
-              top_k = fmaxf(top_k, fmaxf(fabsf(fk.x), fabsf(fk.y)));
-              top_v = fmaxf(top_v, fmaxf(fabsf(fv.x), fabsf(fv.y)));
+              const float2 f = widen2<BF>(kw[j]);
+              top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
             }
           }
-        }
-        if constexpr (BF) {
-#pragma unroll
-          for (int o_ = 1; o_ < 4; o_ <<= 1) {
-            top_k = fmaxf(top_k, __shfl_xor_sync(0xffffffffu, top_k, o_));
-            top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, o_));
-          }
-          up_k[i] = row_up(top_k);
-          up_v[i] = min(row_up(top_v), 64);  // as for cached rows, so that l's terms stay in range
-          if (c == 0) own_scale[16 * warp + r + 8 * i] = power_of(up_v[i]);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          up_k[i] = row_up(fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)));
         }
       }
 #pragma unroll
@@ -433,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
         uint32_t d[2][4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint4 k4 = fetch(k_base, a.sk_l, i, w);
+          const uint4 k4 = fetch(i, w);
           const uint32_t kw[4] = {k4.x, k4.y, k4.z, k4.w};
           const float by = power_of(up_k[i]);
 #pragma unroll
@@ -455,38 +545,68 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
       }
       kq[0] = power_of(-up_k[0]);
       kq[1] = power_of(-up_k[1]);
-      const float ev[2] = {-(float)up_v[0], -(float)up_v[1]};
-      weigh(s, kq, ev, true, [&](int, int j) { return key0 + r + 8 * (j >> 1) >= own; }, [] {});
+      auto masked = [&](int, int j) { return key0 + r + 8 * (j >> 1) >= own; };
+      if (__syncthreads_or(exponents(true, masked) > kRoom)) {
+        offer(true, masked);
+        __syncthreads();
+        settle();
+        exponents(true, masked);
+      }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint2 wf[NT];
+      for (int n = 0; n < NT; ++n) {
+        float w[4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) wf[n] = ws[(i * NT + n) * 32 + lane];
-        uint32_t h[4][kRun / 2];  // channels of keys 2c, 2c + 1, 2c + 8, 2c + 9, as fp16
+        for (int j = 0; j < 4; ++j) w[j] = ex2(x[n][j]);
+        l[n][0] += w[0] + w[2];
+        l[n][1] += w[1] + w[3];
+        if constexpr (BF) {
+          uint32_t high[4], low[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int in_tile = 16 * i + 2 * c + (x & 1) + 8 * (x >> 1), key = 64 * (p - cached) + in_tile;
-          const uint32_t* src = reinterpret_cast<const uint32_t*>(v_base + key * a.sv_l + warp * (D / 4) + r * kRun);
-#pragma unroll
-          for (int j = 0; j < kRun / 2; ++j) {
-            const uint32_t w = key < own ? __ldg(src + j) : 0u;
-            if constexpr (BF) {
-              const float2 f = widen2<BF>(w);
-              h[x][j] = pack_half2(f.x * own_scale[in_tile], f.y * own_scale[in_tile]);
-            } else {
-              h[x][j] = w;
-            }
+          for (int j = 0; j < 4; ++j) {
+            const float small = w[j] * power_of(-kSmall);
+            high[j] = __float_as_uint(small * 0.99609375f) >> 16;
+            low[j] = narrow<true>(small - __uint_as_float(high[j] << 16));
           }
-        }
-#pragma unroll
-        for (int x = 0; x < kTiles; ++x) {
-          const uint32_t a0 = __byte_perm(h[0][x], h[1][x], 0x5410), a1 = __byte_perm(h[0][x], h[1][x], 0x7632);
-          const uint32_t a2 = __byte_perm(h[2][x], h[3][x], 0x5410), a3 = __byte_perm(h[2][x], h[3][x], 0x7632);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816(o[n][x], a0, a1, a2, a3, wf[n].x, wf[n].y);
+          const int at = (warp * NT + n) * 32 + lane;
+          ws[at] = make_uint2(transpose8x8(high[0] | high[1] << 16), transpose8x8(high[2] | high[3] << 16));
+          ws_low[at] = make_uint2(transpose8x8(low[0] | low[1] << 16), transpose8x8(low[2] | low[3] << 16));
+        } else {
+          ws[(warp * NT + n) * 32 + lane] =
+              make_uint2(transpose8x8(pack_half2(w[0], w[1])), transpose8x8(pack_half2(w[2], w[3])));
         }
       }
-      __syncthreads();  // own_scale and the weights are free again
+      __syncthreads();
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        uint32_t h[4][kRun / 2];  // channels of keys 2c, 2c + 1, 2c + 8, 2c + 9
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int key = 64 * (p - cached) + 16 * i + 2 * c + (y & 1) + 8 * (y >> 1);
+          const uint32_t* src = reinterpret_cast<const uint32_t*>(v_base + key * a.sv_l + warp * (D / 4) + r * kRun);
+#pragma unroll
+          for (int j = 0; j < kRun / 2; ++j) h[y][j] = key < own ? __ldg(src + j) : 0u;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint2 w = ws[(i * NT + n) * 32 + lane];
+          const uint2 w_low = BF ? ws_low[(i * NT + n) * 32 + lane] : w;
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) {
+            const uint32_t a0 = __byte_perm(h[0][t], h[1][t], 0x5410), a1 = __byte_perm(h[0][t], h[1][t], 0x7632);
+            const uint32_t a2 = __byte_perm(h[2][t], h[3][t], 0x5410), a3 = __byte_perm(h[2][t], h[3][t], 0x7632);
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (BF) {
+              mma16816_bf16(part, a0, a1, a2, a3, w.x, w.y);
+              mma16816_bf16(part, a0, a1, a2, a3, w_low.x, w_low.y);
+            } else {
+              mma16816(part, a0, a1, a2, a3, w.x, w.y);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[n][t][j] = fmaf(part[j], power_of(kSmall + 127 - kMostPower), o[n][t][j]);
+          }
+        }
+      }
+      __syncthreads();  // the weights are free again
     }
 
     // the rows' sums over the warps; O goes out from where it is
@@ -524,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
         if (whole) {
           const int li = (first_row + row) / a.group, h = u.kvh * a.group + (first_row + row) % a.group;
           const bool real = sum != 0.f && li < u.tokens;
-          const float f = real ? 1.f / sum : 0.f;
+          const float f = real ? power_of(E - 127) / sum : 0.f;
           uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + u.b * a.so_b + h * a.so_h + li * a.so_l + d);
 #pragma unroll
           for (int x = 0; x < kTiles; ++x)
@@ -532,7 +652,8 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
         } else {
           float2* dst = reinterpret_cast<float2*>(a.part_o + (part * P::kRows + row) * D + d);
 #pragma unroll
-          for (int x = 0; x < kTiles; ++x) dst[x] = make_float2(o[n][x][j], o[n][x][j + 2]);
+          for (int x = 0; x < kTiles; ++x)
+            dst[x] = make_float2(o[n][x][j] * power_of(E - kMostPower), o[n][x][j + 2] * power_of(E - kMostPower));
           if (warp == 0 && r == 0)
             *reinterpret_cast<float2*>(a.part_st + (part * P::kRows + row) * 2) = make_float2(m[n][j], sum);
         }

@@ -481,8 +481,13 @@ D3B_API int d3b_kv4_move_pages(const d3b_kv4_cache* cache, const int32_t* src, c
  *     clamped.
  *   workspace: d3b_kv4_decode_workspace_size() bytes, 16-byte aligned (need not be zeroed;
  *     launches that may overlap need one each)
- * Q, K and V enter the products exactly, in fp16 (queries under a power of two a row); softmax
- * weights are rounded to fp16; sums are fp32. Results do not change from call to call.
+ * Q, K and V enter the products exactly, in fp16 (queries under a power of two a row: what is 2^-29
+ * of a row's largest and less loses bits), whatever the rows' magnitudes are beside each other; a softmax
+ * weight is rounded to fp16's 11 bits, and below 2^-22 of its row's largest to 2^-33 of that; sums are
+ * fp32. V rows whose values are all below 2^-52 may count as zeros. V rows whose largest value lies outside
+ * 2^-10 to 2^7 (or, where a sequence's first rows do, outside 2^-11 to 2^7 of theirs) cost further passes
+ * over their keys.
+ * Results do not change from call to call.
  */
 D3B_API size_t d3b_kv4_decode_workspace_size(const d3b_kv4_cache* cache, int B, int H, int L, int64_t width);
 D3B_API int d3b_kv4_decode(const d3b_kv4_cache* cache, int64_t layer, const void* q, const int64_t* q_strides,
@@ -498,7 +503,8 @@ D3B_API int d3b_kv4_decode(const d3b_kv4_cache* cache, int64_t layer, const void
  *   k_q, v_q [B, kv_heads, L, D], strides {b, h, l}, 16-bit like q; lengths [B] int32 on the
  *     device; an entry outside [0, L] is clamped (device error word 2010). Tokens i >= lengths[b]
  *     get zero rows.
- * Own keys enter as the cached ones do: rows under a power of two, in fp16.
+ * Own K rows enter as cached ones do, under a power of two a row in fp16, own V rows as they are; with bf16
+ * their weights have 15 bits. Own V values below 2^-90 may count as zeros.
  */
 D3B_API size_t d3b_kv4_question_workspace_size(const d3b_kv4_cache* cache, int B, int H, int L, int64_t state_len);
 D3B_API int d3b_kv4_question(const d3b_kv4_cache* cache, int64_t layer, const void* q, const int64_t* q_strides,

@@ -1,5 +1,5 @@
-"""The 4-bit cache's attention where magnitudes lie far apart: query rows of one tile, in place and over a widened
-state. The bounds go by channel."""
+"""The 4-bit cache's attention where magnitudes lie far apart: query rows of one tile, V rows of one step, and a
+block's own rows, in place and over a widened state. The bounds go by channel."""
 
 from __future__ import annotations
 
@@ -100,5 +100,119 @@ def test_padding_queries_of_any_size(monkeypatch, in_place, dim, heads, L):
             if m:
                 check_rows(got[b, :, :m], q[b, :, :m], torch.cat([ks, kq[b, :, :m].double()], 1),
                            torch.cat([vs, vq[b, :, :m].double()], 1), dim**-0.5, True)
+    kv4._plans_of.cache_clear()
+    assert _lib.device_error() == 0
+
+
+# --------------------------------------------------------------------------- V rows of far powers
+def far_values(n, kv_heads, dim, dtype, where, power, seed):
+    """V rows of order 1 in channels 2 and up, and rows of 2^power in channel 0 (or, below 1, in channel 1) alone."""
+    v = rows((n, kv_heads, dim), dtype, seed, 0.2)
+    if dtype == HF:
+        v = (v.double() * 2.0**-9).to(dtype)
+    v[..., :2] = 0
+    at = {"first": [0], "middle": [n // 2], "last": [n - 1], "spread": list(range(3, n, 7)), "half": list(range(0, n, 2)),
+          "tail": list(range(n // 3, n))}[where]
+    v[at] = 0
+    v[at, :, 0 if power > 0 else 1] = 2.0**power
+    return v
+
+
+SHAPES = [(64, 8, 1), (64, 4, 4), (128, 8, 1), (128, 4, 4), (256, 8, 1), (128, 8, 4), (256, 5, 5), (256, 3, 4), (64, 16, 2)]
+
+
+@pytest.mark.parametrize("dim,group,L", SHAPES)
+@pytest.mark.parametrize("dtype,power", [(BF, 16), (BF, 25), (BF, 40), (BF, 90), (BF, 126), (BF, -20), (BF, -40), (HF, 15), (HF, -22)])
+@pytest.mark.parametrize("where", ["first", "middle", "last", "spread", "half", "tail"])
+def test_far_value_rows(dim, group, L, dtype, power, where):
+    n = 200
+    k, v = rows((n, 2, dim), dtype, 1, 0.2), far_values(n, 2, dim, dtype, where, power, 2)
+    cache, table, ks, vs = cache_of(k, v, 16)
+    q = rows((1, 2 * group, L, dim), dtype, 3, 0.2)
+    got = decode(q, cache, table, n, dim**-0.5)
+    check_rows(got[0], q[0], ks, vs, dim**-0.5)
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("dim,group,L", [(64, 8, 1), (128, 16, 1), (256, 8, 1), (128, 8, 4), (256, 6, 5)])
+def test_many_steps_of_mixed_powers(dim, group, L):
+    """Powers that wander over 2^60, rows of zeros and masks; long enough for several CTAs a sequence."""
+    n = 3000
+    k, v = rows((n, 1, dim), BF, 1, 0.2), rows((n, 1, dim), BF, 2, 0.2)
+    g = torch.Generator().manual_seed(4)
+    for d in range(dim):  # each channel has its own keys of its own power
+        keep = torch.rand(n, generator=g) < 0.15
+        v[:, 0, d] = torch.where(keep, v[:, 0, d], 0)
+    power = torch.randint(-30, 31, (n,), generator=g).double() * (torch.rand(n, generator=g) < 0.3)
+    v = (v.double() * 2.0 ** power[:, None, None]).to(BF)
+    v[5::11] = 0
+    v[:40] = 0
+    cache, table, ks, vs = cache_of(k, v, 64)
+    q = rows((1, group, L, dim), BF, 3, 0.2)
+    got = decode(q, cache, table, n, dim**-0.5, causal=True)
+    for i in range(L):
+        m = n - (L - 1 - i)
+        check_rows(got[0, :, i:i + 1], q[0, :, i:i + 1], ks[:, :m], vs[:, :m], dim**-0.5)
+    assert _lib.device_error() == 0
+
+
+def test_all_value_rows_at_one_end():
+    """Nothing but rows of 2^-40, of 2^126, or of zeros and then of 2^100."""
+    dim, n = 128, 100
+    k, q = rows((n, 1, dim), BF, 1, 0.2), rows((1, 4, 1, dim), BF, 3, 0.2)
+    for power in (-40, 120, None):
+        v = rows((n, 1, dim), BF, 2, 0.1)
+        if power is None:
+            v = (v.double() * 2.0**100).to(BF)
+            v[:60] = 0
+        else:
+            v = (v.double() * 2.0**power).to(BF)
+        cache, table, ks, vs = cache_of(k, v, 32)
+        check_rows(decode(q, cache, table, n, dim**-0.5)[0], q[0], ks, vs, dim**-0.5)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("dim,heads,L", [(64, 4, 9), (128, 8, 12), (256, 6, 20)])
+@pytest.mark.parametrize("dtype,power", [(BF, 25), (BF, 60), (BF, -40), (HF, 15)])
+def test_question_far_value_rows(monkeypatch, in_place, dim, heads, L, dtype, power):
+    """Far rows among the state's and among a block's own: the same whichever way the state is read."""
+    monkeypatch.setattr(kv4, "_reads_codes", lambda *a: in_place)
+    kv4._plans_of.cache_clear()
+    state, lengths = 150, [L, L - 3, 1]
+    k = rows((state, 1, dim), dtype, 1, 0.2)
+    q, kq = rows((3, heads, L, dim), dtype, 3, 0.2), rows((3, 1, L, dim), dtype, 4, 0.2)
+    for where, own in (("first", "middle"), ("spread", "spread"), (None, "first"), ("last", None)):
+        v = far_values(state, 1, dim, dtype, where or "last", power if where else 1, 5)
+        vq = torch.stack([far_values(L, 1, dim, dtype, own or "last", power if own else 1, 6 + b).transpose(0, 1) for b in range(3)])
+        cache, table, ks, vs = cache_of(k, v, 32)
+        got = kv4.question_attention(q.cuda(), cache, 0, table, state, kq.cuda(), vq.cuda(), lengths, scale=dim**-0.5)
+        for b, m in enumerate(lengths):
+            check_rows(got[b, :, :m], q[b, :, :m], torch.cat([ks, kq[b, :, :m].double()], 1),
+                       torch.cat([vs, vq[b, :, :m].double()], 1), dim**-0.5, True)
+    kv4._plans_of.cache_clear()
+    assert _lib.device_error() == 0
+
+
+# --------------------------------------------------------------------------- a block's own rows that are not finite
+@pytest.mark.parametrize("dim,heads,L", [(64, 4, 9), (128, 8, 12), (256, 6, 20)])
+@pytest.mark.parametrize("dtype,large", [(BF, 1e6), (BF, 1e30), (HF, 6e4)])
+def test_own_rows_with_an_infinity(monkeypatch, dim, heads, L, dtype, large):
+    """A V row with an infinity in one channel and large numbers in others: the others stay finite."""
+    monkeypatch.setattr(kv4, "_reads_codes", lambda *a: True)
+    kv4._plans_of.cache_clear()
+    state, scale = 70, dim**-0.5
+    k, v = rows((state, 1, dim), dtype, 1, 0.2), rows((state, 1, dim), dtype, 2, 0.2)
+    cache, table, ks, vs = cache_of(k, v, 32)
+    q, kq, vq = rows((2, heads, L, dim), dtype, 3, 0.2), rows((2, 1, L, dim), dtype, 4, 0.2), rows((2, 1, L, dim), dtype, 5, 0.2)
+    vq[:, 0, 2, 0], vq[:, 0, 2, 5] = math.inf, -large
+    got = kv4.question_attention(q.cuda(), cache, 0, table, state, kq.cuda(), vq.cuda(), [L, L], scale=scale)
+    assert bool((got[..., 0] == math.inf).all())
+    tame = vq.clone()
+    tame[:, 0, 2, 0] = 0
+    for b in range(2):
+        out, mass, top = ref.attention(q[b], torch.cat([ks, kq[b].double()], 1), torch.cat([vs, tame[b].double()], 1), scale)
+        spread = torch.cat([vs, tame[b].double()], 1).abs().sum(1, keepdim=True)
+        bound = channel_bound(out, mass, spread, top, state + L, dim, dtype, True)
+        assert bool(((got[b].cpu().double() - out).abs() <= bound)[..., 1:].all())
     kv4._plans_of.cache_clear()
     assert _lib.device_error() == 0
