@@ -236,11 +236,8 @@ struct Span {
   }
 };
 
-// the power of two that brings a row's largest magnitude to [2^14, 2^15), as far as 2^126 goes; rows
-// that are not finite stay
-__device__ __forceinline__ int row_up(float top) {
-  return top < INFINITY ? min(126, 14 - ((int)(__float_as_uint(top) >> 23) - 127)) : 0;
-}
+// the power of two that brings a row's largest finite magnitude to [2^14, 2^15), as far as 2^126 goes
+__device__ __forceinline__ int row_up(float top) { return min(126, 14 - ((int)(__float_as_uint(top) >> 23) - 127)); }
 __device__ __forceinline__ float power_of(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // e in [-126, 127]
 
 // a partial result (O, (m, l)) brought to the reference `base` and added

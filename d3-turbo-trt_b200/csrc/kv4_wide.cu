@@ -511,7 +511,8 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const float2 f = widen2<BF>(kw[j]);
-              top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+              top = fabsf(f.x) < INFINITY ? fmaxf(top, fabsf(f.x)) : top;  // the largest finite one, as for queries
+              top = fabsf(f.y) < INFINITY ? fmaxf(top, fabsf(f.y)) : top;
             }
           }
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));

@@ -216,3 +216,24 @@ def test_own_rows_with_an_infinity(monkeypatch, dim, heads, L, dtype, large):
         assert bool(((got[b].cpu().double() - out).abs() <= bound)[..., 1:].all())
     kv4._plans_of.cache_clear()
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("dim,heads,L", [(64, 4, 9), (128, 8, 12), (256, 6, 20)])
+@pytest.mark.parametrize("dtype,large", [(BF, 1e6), (BF, 1e30), (HF, 6e4)])
+def test_own_key_with_a_score_of_minus_infinity(monkeypatch, in_place, dim, heads, L, dtype, large):
+    """A K row of -infinity where every query is positive, with large numbers where every query is zero: no weight."""
+    monkeypatch.setattr(kv4, "_reads_codes", lambda *a: in_place)
+    kv4._plans_of.cache_clear()
+    state, scale = 70, dim**-0.5
+    k, v = rows((state, 1, dim), dtype, 1, 0.2), rows((state, 1, dim), dtype, 2, 0.2)
+    cache, table, ks, vs = cache_of(k, v, 32)
+    q, kq, vq = rows((2, heads, L, dim), dtype, 3, 0.2), rows((2, 1, L, dim), dtype, 4, 0.2), rows((2, 1, L, dim), dtype, 5, 0.2)
+    q[..., 0], q[..., 5] = q[..., 0].abs() + 1, 0
+    kq[:, 0, 4, 0], kq[:, 0, 4, 5] = -math.inf, large
+    got = kv4.question_attention(q.cuda(), cache, 0, table, state, kq.cuda(), vq.cuda(), [L, L], scale=scale)
+    keep = [i for i in range(L) if i != 4]
+    for b in range(2):
+        check_rows(got[b], q[b], torch.cat([ks, kq[b][:, keep].double()], 1), torch.cat([vs, vq[b][:, keep].double()], 1), scale, True)
+    kv4._plans_of.cache_clear()
+    assert _lib.device_error() == 0
