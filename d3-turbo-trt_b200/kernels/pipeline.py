@@ -184,6 +184,7 @@ class QuestionPipeline:
         slot = self.slots[self.count % len(self.slots)]
         self.count += 1
         lens = block_offsets(lengths, self.device)
+        lens.record_stream(self.compute)  # it may leave the cache before this batch has run
         with torch.cuda.stream(self.copy_in):
             # The slot's input buffers are free once its previous pass has run, its
             # output buffer once that pass's output has left the GPU: the next

@@ -23,6 +23,7 @@ divisible by kv heads (prefix_bidir.py:202-216). There is no fallback.
 
 from __future__ import annotations
 
+import threading
 from collections import OrderedDict
 from typing import Sequence
 
@@ -36,8 +37,12 @@ KERNEL_NAME = "sm100a"
 # outside [0, L] (the entry is clamped; read it with _lib.device_error()).
 SITE_BAD_LENGTH = 2010
 
-_LENGTHS: "OrderedDict[tuple, torch.Tensor]" = OrderedDict()
+# Tables of lengths given on the host, with the stream that each was made on, and those that captured calls read:
+# a graph keeps an address, so the latter stay for good.
+_LENGTHS: "OrderedDict[tuple, tuple[torch.Tensor, int]]" = OrderedDict()
 _LENGTHS_MAX = 16
+_LENGTHS_CAPTURED: dict[tuple, torch.Tensor] = {}
+_LENGTHS_LOCK = threading.Lock()
 
 # Workspaces of d3b_prefix_bidir_ws, one per (device, stream): zero-filled when
 # made; every launch leaves them zeroed again and calls on one stream are
@@ -80,23 +85,48 @@ def triton_available() -> bool:  # name kept for callers of the reference module
     return kernel_available()
 
 
+def _stream_now(device: torch.device) -> tuple[int, bool]:
+    """The device's current stream, and whether it is being captured."""
+    if device.type != "cuda":
+        return 0, False
+    with torch.cuda.device(device):
+        return torch.cuda.current_stream().cuda_stream, torch.cuda.is_current_stream_capturing()
+
+
 def block_offsets(lengths: Sequence[int] | torch.Tensor, device: torch.device) -> torch.Tensor:
     """The block-offset table as a device int32 tensor of lengths, cached like the
-    reference ``_meta`` (prefix_bidir.py:152-163, an LRU of 16 by (lengths, device))."""
+    reference ``_meta`` (prefix_bidir.py:152-163, an LRU of 16 by (lengths, device)).
+
+    The table is for work on the device's current stream. In a captured call lengths on the host need a table
+    that an earlier call made (``RuntimeError`` where there is none); it is kept as long as the process."""
     if isinstance(lengths, torch.Tensor):
         if lengths.is_cuda and lengths.dtype == torch.int32 and lengths.device == device:
             return lengths.contiguous()
         lengths = [int(n) for n in lengths.tolist()]
     key = (tuple(int(n) for n in lengths), str(device))
-    hit = _LENGTHS.get(key)
-    if hit is not None:
-        _LENGTHS.move_to_end(key)
-        return hit
-    if len(_LENGTHS) >= _LENGTHS_MAX:
-        _LENGTHS.popitem(last=False)
-    t = torch.tensor(key[0], dtype=torch.int32).to(device, non_blocking=False)
-    _LENGTHS[key] = t
-    return t
+    stream, capturing = _stream_now(device)
+    with _LENGTHS_LOCK:
+        kept = _LENGTHS_CAPTURED.get(key)
+        if kept is not None:
+            return kept
+        hit = _LENGTHS.get(key)
+        if hit is not None:
+            table, made_on = hit
+            _LENGTHS.move_to_end(key)
+            if capturing:
+                _LENGTHS_CAPTURED[key] = table
+            elif stream != made_on:  # its memory is used again only after this stream's work so far
+                table.record_stream(torch.cuda.current_stream(device))
+            return table
+    if capturing:
+        raise RuntimeError("lengths on the host in a captured call: make the call once before the capture, or give "
+                           "the lengths as an int32 device tensor")
+    table = torch.tensor(key[0], dtype=torch.int32).to(device, non_blocking=False)
+    with _LENGTHS_LOCK:
+        while len(_LENGTHS) >= _LENGTHS_MAX:
+            _LENGTHS.popitem(last=False)
+        _LENGTHS[key] = (table, stream)
+    return table
 
 
 def _check(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
