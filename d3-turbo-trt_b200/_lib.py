@@ -245,7 +245,9 @@ def device_error(device: torch.device | int | None = None, reset: bool = True) -
 
     The word is sticky: once a device-side wait has given up, later launches
     stop early and their outputs are undefined until it is read with
-    ``reset``; check it after a pass (or a batch of passes)."""
+    ``reset``; check it after a pass (or a batch of passes). Codes of inputs on the
+    device that were out of range (lengths, slots, pages) are kept apart: they stop
+    nothing, and are returned where no wait gave up."""
     if device is None:
         dev = torch.device("cuda", torch.cuda.current_device())
     else:

@@ -5,8 +5,9 @@
 
 #include "common.cuh"
 
-// One error word per device; kernels receive its device address as an argument.
-__device__ int g_d3b_device_error = 0;
+// A device's error words; kernels receive their device address as an argument. [0]: a wait gave up, which every
+// later wait heeds; [1]: an input on the device was out of range and left out or clamped, which stops nothing.
+__device__ int g_d3b_device_error[2] = {0, 0};
 
 namespace d3b_host {
 
@@ -130,13 +131,13 @@ const char* d3b_error_string(int status) {
 int d3b_device_error(d3b_stream_t stream, int reset) {
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (cudaStreamSynchronize(s) != cudaSuccess) return D3B_ECUDA;
-  int v = 0;
-  if (cudaMemcpyFromSymbol(&v, g_d3b_device_error, sizeof(int)) != cudaSuccess) return D3B_ECUDA;
-  if (reset && v) {
-    int zero = 0;
-    if (cudaMemcpyToSymbol(g_d3b_device_error, &zero, sizeof(int)) != cudaSuccess) return D3B_ECUDA;
+  int v[2] = {0, 0};
+  if (cudaMemcpyFromSymbol(v, g_d3b_device_error, sizeof(v)) != cudaSuccess) return D3B_ECUDA;
+  if (reset && (v[0] || v[1])) {
+    const int zero[2] = {0, 0};
+    if (cudaMemcpyToSymbol(g_d3b_device_error, zero, sizeof(zero)) != cudaSuccess) return D3B_ECUDA;
   }
-  return v;
+  return v[0] ? v[0] : v[1];
 }
 
 int d3b_selftest_wait_timeout(int limit_ms, d3b_stream_t stream) {

@@ -42,6 +42,11 @@ __device__ __forceinline__ void record_device_error(int* err, int site) {
   if (err) atomicCAS(err, 0, site);
 }
 
+// An input on the device that was out of range, and was left out or clamped: no wait heeds this word.
+__device__ __forceinline__ void record_input_error(int* err, int site) {
+  if (err) atomicCAS(err + 1, 0, site);
+}
+
 // ---------------------------------------------------------------------------
 // mbarrier
 // ---------------------------------------------------------------------------

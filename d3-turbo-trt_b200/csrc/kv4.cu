@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(uint8_t* __restrict__ 
   const int64_t page = slot >> page_shift;
   live = live && slot >= 0;
   if (live && page >= pages) {
-    if (sub == 0) d3b::record_device_error(err, kSiteBadSlot);
+    if (sub == 0) d3b::record_input_error(err, kSiteBadSlot);
     live = false;
   }
   const Coded ck = quantise<D, BF>(k_raw), cv = quantise<D, BF>(v_raw);
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const uint8_t* __restric
   const int64_t page = __ldg(table + (tok >> page_shift));
   uint4 o[4] = {};
   if (page < 0 || page >= pages) {
-    if (sub == 0) d3b::record_device_error(err, kSiteBadPage);
+    if (sub == 0) d3b::record_input_error(err, kSiteBadPage);
   } else {
     const int in_page = (int)tok & ((1 << page_shift) - 1);
     const int t = in_page & 15, group = sub >> 1;
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kThreads) move_kernel(uint8_t* __restrict__ po
     }
     for (int64_t i = (cta - copy_ctas) * kThreads + threadIdx.x; i < n; i += step) {
       const bool order = i + 1 < n && __ldg(src + i) >= __ldg(src + i + 1);
-      if (order || find(src, n, __ldg(dst + i)) >= 0) d3b::record_device_error(err, kSiteBadMove);
+      if (order || find(src, n, __ldg(dst + i)) >= 0) d3b::record_input_error(err, kSiteBadMove);
     }
     return;
   }
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kThreads) move_kernel(uint8_t* __restrict__ po
   const int64_t i = pl % n, layer = pl / n;
   const int64_t from = __ldg(src + i), to = __ldg(dst + i);
   if (from < 0 || from >= pages || to < 0 || to >= pages) {
-    if (threadIdx.x == 0) d3b::record_device_error(err, kSiteBadPage);
+    if (threadIdx.x == 0) d3b::record_input_error(err, kSiteBadPage);
     return;
   }
   const uint4* s = reinterpret_cast<const uint4*>(pool + (layer * pages + from) * page_bytes);

@@ -291,7 +291,7 @@ __device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b, bool repo
   if (a.lengths) {
     s.len = __ldg(a.lengths + b);
     if (s.len < 0 || s.len > a.most) {
-      if (report) d3b::record_device_error(a.err, kSiteBadLength);
+      if (report) d3b::record_input_error(a.err, kSiteBadLength);
       s.len = s.len < 0 ? 0 : a.most;
     }
   }
@@ -300,7 +300,7 @@ __device__ __forceinline__ Sequence sequence(const AttnArgs& a, int b, bool repo
   if (a.own_lengths) {
     s.own = __ldg(a.own_lengths + b);
     if (s.own < 0 || s.own > a.L) {
-      if (report) d3b::record_device_error(a.err, kSiteOwnLength);
+      if (report) d3b::record_input_error(a.err, kSiteOwnLength);
       s.own = s.own < 0 ? 0 : a.L;
     }
     s.tokens = s.own;

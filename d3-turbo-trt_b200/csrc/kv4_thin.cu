@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
 #pragma unroll 1
       for (int i = 0; i < P::GP; ++i) {
         if ((bad >> i) & 1) {
-          if (lane == 0) d3b::record_device_error(a.err, kSiteBadPage);
+          if (lane == 0) d3b::record_input_error(a.err, kSiteBadPage);
           continue;
         }
         src = head_pool + (i ? ids[P::GP - 1] : ids[0]) * a.page_bytes + ((g + i) & in_page) * granule_bytes(D);

@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
     // copy the warp's granule of tile p to ring half HALF: K (how many of its tokens are keys), V
     auto load_k = [&](int p, int id, uint32_t half) -> int {
       if (!in_pool(id)) {
-        if (lane == 0 && p < last_cached && 4 * p + warp < grains) d3b::record_device_error(a.err, kSiteBadPage);
+        if (lane == 0 && p < last_cached && 4 * p + warp < grains) d3b::record_input_error(a.err, kSiteBadPage);
         return 0;
       }
       const uint8_t* src = source(p, id);

@@ -133,12 +133,12 @@ struct Params {
 
 // Real tokens of question block b. The table lives in device memory, so the
 // host cannot check it: a value outside [0, L] is clamped (every access stays
-// inside the caller's [B, *, L, D] tensors) and reported through the device
-// error word (site kSiteBadLength), which voids the launch's results.
+// inside the caller's [B, *, L, D] tensors) and recorded as an input error
+// (site kSiteBadLength).
 __device__ __forceinline__ int block_length(const Params& p, int b) {
   const int n = p.lengths[b];
   if (n < 0 || n > p.L) {
-    d3b::record_device_error(p.err, kSiteBadLength);
+    d3b::record_input_error(p.err, kSiteBadLength);
     return n < 0 ? 0 : p.L;
   }
   return n;

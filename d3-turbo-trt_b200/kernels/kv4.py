@@ -16,7 +16,7 @@ its largest magnitude, in fp16.
   ``prefix_bidir_attention`` over a state that lies in the cache.
 
 Page numbers, slots and lengths given as device tensors are not read on the host: the kernels leave
-out what does not fit the pool or the table and set the device error word (``SITE_BAD_SLOT``,
+out what does not fit the pool or the table and record an input error (``SITE_BAD_SLOT``,
 ``SITE_BAD_PAGE``, ``SITE_BAD_LENGTH``, ``SITE_BAD_MOVE``; ``_lib.device_error()`` reads it).
 A row that held a NaN or an infinity reads back as NaN.
 """
@@ -190,7 +190,7 @@ class Kv4Cache:
                    tables: torch.Tensor) -> None:
         """``copy_pages``, and every entry of ``tables`` (int32, contiguous) that is some ``src[i]``
         becomes ``dst[i]``, in one launch. ``src`` must be ascending (the kernel records a list that
-        is not, or a destination among the sources, in the device error word)."""
+        is not, or a destination among the sources, as an input error)."""
         _index(tables, torch.int32, self.device, "tables")
         if not tables.is_contiguous():
             raise RuntimeError("tables must be contiguous")
@@ -314,8 +314,8 @@ def question_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torc
 
     q [B, H, L, D], k_q/v_q [B, H_kv, L, D], ``lengths`` as there. Returns [B, H, L, D], zero rows
     for padding. Small batches read the codes in place, larger ones widen the state first. A page outside
-    the pool or a device length outside [0, L] sets the device error word (2102, 2010) either way; in
-    place its tokens are left out or it is clamped, but a widened launch's results are void then.
+    the pool (2102) or a device length outside [0, L] (2010) is recorded as an input error: the length is
+    clamped, the page's tokens are left out in place and keys and values of zero where the state is widened.
     """
     cache._check_layer(layer)
     if not 0 < scale < math.inf:

@@ -33,7 +33,7 @@ from .. import _lib
 
 HEAD_DIMS = (32, 64, 128, 256)
 KERNEL_NAME = "sm100a"
-# Device error word set by the kernel when a device-resident lengths entry lies
+# Input error recorded by the kernel when a device-resident lengths entry lies
 # outside [0, L] (the entry is clamped; read it with _lib.device_error()).
 SITE_BAD_LENGTH = 2010
 
@@ -63,7 +63,9 @@ def _workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:
 
 
 def _rezero_workspaces(index: int) -> None:
-    # a launch that gave up may have left a unit's count behind
+    # a launch that gave up may have left a unit's count behind; launches of other streams count in theirs until they end
+    if any(dev == index for dev, _ in _WORKSPACES):
+        torch.cuda.synchronize(index)
     for (dev, _), buf in _WORKSPACES.items():
         if dev == index:
             buf.zero_()
@@ -201,8 +203,8 @@ def prefix_bidir_attention(
 
     ``lengths`` given as Python ints are checked here (``RuntimeError`` outside
     [0, L]). A CUDA int32 tensor is passed to the kernel as it is, without a
-    device sync; the kernel clamps entries outside [0, L] and sets the device
-    error word to ``SITE_BAD_LENGTH``, which ``_lib.device_error()`` returns.
+    device sync; the kernel clamps entries outside [0, L] and records
+    ``SITE_BAD_LENGTH``, which ``_lib.device_error()`` returns.
     """
     _check(q, k_q, v_q)
     if k_state.dtype != q.dtype or v_state.dtype != q.dtype:

@@ -14,6 +14,9 @@
  * still return D3B_OK, since the launch itself was valid). Callers check
  * d3b_device_error() after a pass (or a batch of passes) and discard the
  * results it covers when it is non-zero; reading it with reset != 0 clears it.
+ * Inputs in device memory that are out of range (lengths, slots, page numbers) are left out or
+ * clamped and recorded in a word of their own, which stops nothing: results are those of the
+ * inputs as clamped. d3b_device_error() returns that word's code where no wait gave up.
  *
  * Dtype codes (x_dtype, dtype, h_dtype, out_kind):
  *   D3B_F32 = 0, D3B_F16 = 1, D3B_BF16 = 2, D3B_I32 = 3
@@ -60,7 +63,7 @@ D3B_API const char* d3b_error_string(int status);
 
 /* Returns the device error word of the current device (0 = none) after
  * synchronising `stream`; clears it when `reset` is non-zero. A non-zero
- * value is the site code of the wait that gave up. */
+ * value is the site code of the wait that gave up, or, where none did, of an input out of range. */
 D3B_API int d3b_device_error(d3b_stream_t stream, int reset);
 
 /*
@@ -146,7 +149,7 @@ D3B_API int d3b_w8a8_gemm(const void* qa, const void* qw, const float* sa, const
  * dtype: D3B_F16 or D3B_BF16 for all of q/k/v/out. D in {32, 64, 128, 256};
  * H % Hkv == 0 and H/Hkv <= 128. Strides must be multiples of 8 elements.
  * The kernel reads `lengths` itself: an entry outside [0, L] is clamped and
- * sets the device error word (site 2010, see d3b_device_error).
+ * recorded as an input error (site 2010, see d3b_device_error).
  * Work unit: one (block, head group, 128-row Q tile), one CTA per SM at a
  * time. A head group is the kv head's whole GQA group, or, when the group does
  * not divide 128 rows and fewer tiles result, a divisor of it (G = 6 at 64
@@ -425,8 +428,8 @@ D3B_API void d3b_arena_destroy(void* arena);
  * head_dim in {64, 128, 256}; page_tokens in {16, 32, 64, 128, 256} (else D3B_EUNSUPPORTED).
  * Page p of a table holds tokens p * page_tokens ... of its sequence; slot s of a pool is token
  * s % page_tokens of page s / page_tokens. Page numbers, slots and lengths live on the device:
- * the kernels check each against the pool and the table, leave a bad one out and set the
- * device error word (2101 slot, 2102 page, 2103 length, 2104 page list).
+ * the kernels check each against the pool and the table, leave a bad one out and
+ * record an input error (2101 slot, 2102 page, 2103 length, 2104 page list; d3b_device_error).
  */
 typedef struct d3b_kv4_cache {
   void* pool;
@@ -501,7 +504,7 @@ D3B_API int d3b_kv4_decode(const d3b_kv4_cache* cache, int64_t layer, const void
  * pay for widening the state; larger ones read it with d3b_kv4_read and call d3b_prefix_bidir).
  *   table [width] int32 on the device, width * page_tokens >= state_len
  *   k_q, v_q [B, kv_heads, L, D], strides {b, h, l}, 16-bit like q; lengths [B] int32 on the
- *     device; an entry outside [0, L] is clamped (device error word 2010). Tokens i >= lengths[b]
+ *     device; an entry outside [0, L] is clamped (input error 2010). Tokens i >= lengths[b]
  *     get zero rows.
  * Own K rows enter as cached ones do, under a power of two a row in fp16, own V rows as they are; with bf16
  * their weights have 15 bits. Own V values below 2^-90 may count as zeros.
