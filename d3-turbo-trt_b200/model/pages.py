@@ -10,9 +10,9 @@ page tables. ``store(snapshot)`` quantises the K/V of a state pass's snapshot in
 ``D3Backbone.questions`` reads and ``StateCache`` keeps (``tensor_bytes`` counts its pages).
 ``fork``, ``extend`` and ``compact`` copy and move pages on the device.
 
-Lifetime: a snapshot's pages go back to the pool when the last reference to its list is dropped.
-Work queued before then on the current stream may still read them; what is queued later on that
-stream comes after it. Readers on other streams must be ordered by the caller, as for any tensor.
+Lifetime: a state's pages go back to the pool when the last snapshot, copy of its list or entry of it
+is dropped. Work queued before then on the current stream may still read them; what is queued later on
+that stream comes after it. Readers on other streams must be ordered by the caller, as for any tensor.
 ``compact`` rewrites the tables in place: a captured graph that reads them stays right.
 """
 
@@ -22,7 +22,7 @@ import collections
 import dataclasses
 import heapq
 import threading
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Any, Sequence
 
 import torch
@@ -117,6 +117,21 @@ class PagePool:
             return src, dst
 
 
+class Kv4Pages:
+    """A state's pages and its row of the tables; given back when nothing refers to them any more."""
+
+    __slots__ = ("states", "row", "pages", "tokens")
+
+    def __init__(self, states: "Kv4States", row: int, pages: list[int], tokens: int):
+        self.states, self.row, self.pages, self.tokens = states, row, pages, tokens
+
+    def __del__(self):
+        try:
+            self.states._drop(self.row)
+        except Exception:  # interpreter shutdown, or a constructor that failed
+            pass
+
+
 @dataclass(slots=True, eq=False)
 class Kv4Entry:
     """A full-attention layer's state keys and values in pages (``AttentionEntry`` in 4 bits)."""
@@ -125,6 +140,7 @@ class Kv4Entry:
     layer: int  # of the cache
     table: torch.Tensor  # [pages] int32, a row of the states' tables
     tokens: int
+    held: Kv4Pages | None = field(default=None, repr=False)  # keeps the pages
 
     @property
     def held_bytes(self) -> int:
@@ -132,19 +148,25 @@ class Kv4Entry:
 
 
 class Kv4Snapshot(list):
-    """A snapshot with ``Kv4Entry`` entries; its pages live as long as this list."""
+    """A snapshot with ``Kv4Entry`` entries; its pages live as long as this list or an entry of it."""
 
     packable = False  # not tensors: a state cache keeps it as it is
 
-    def __init__(self, entries: Sequence[Any], states: "Kv4States", row: int, pages: list[int], tokens: int):
+    def __init__(self, entries: Sequence[Any], held: Kv4Pages):
         super().__init__(entries)
-        self.states, self.row, self.pages, self.tokens = states, row, pages, tokens
+        self.held, self.tokens = held, held.tokens
 
-    def __del__(self):
-        try:
-            self.states._drop(self.row)
-        except Exception:  # interpreter shutdown, or a constructor that failed
-            pass
+    @property
+    def states(self) -> "Kv4States":
+        return self.held.states
+
+    @property
+    def row(self) -> int:
+        return self.held.row
+
+    @property
+    def pages(self) -> list[int]:
+        return self.held.pages
 
 
 class Kv4States:
@@ -187,12 +209,12 @@ class Kv4States:
         """A snapshot over ``pages`` (already counted for it); tables from page ``write`` on are set."""
         row = heapq.heappop(self._rows)
         self._held[row] = pages
-        snap = Kv4Snapshot([], self, row, pages, tokens)
+        snap = Kv4Snapshot([], Kv4Pages(self, row, pages, tokens))
         self._fill(snap, write)
         layer = 0
         for e in entries:
             if isinstance(e, (AttentionEntry, Kv4Entry)):
-                e = Kv4Entry(self.cache, layer, self.tables[row, :len(pages)], tokens)
+                e = Kv4Entry(self.cache, layer, self.tables[row, :len(pages)], tokens, snap.held)
                 layer += 1
             snap.append(e)
         return snap
@@ -247,6 +269,8 @@ class Kv4States:
         ``compact``."""
         with self._lock:
             page = self.cache.page_tokens
+            if snap.tokens != snap.held.tokens:
+                raise RuntimeError("a copy of this snapshot was extended already: extend a fork")
             need = self.pages_for(snap.tokens + count, page)
             if count < 0 or need > self.tables.shape[1]:
                 raise RuntimeError(f"{snap.tokens} + {count} tokens, tables hold {self.tables.shape[1] * page}")
@@ -259,7 +283,7 @@ class Kv4States:
             snap.pages.extend(more)
             self._fill(snap, first)
             slots = self.cache.slots(snap_table(snap), snap.tokens, count)
-            snap.tokens += count
+            snap.tokens = snap.held.tokens = snap.tokens + count
             for i, e in enumerate(snap):
                 if isinstance(e, Kv4Entry):
                     snap[i] = dataclasses.replace(e, table=snap_table(snap), tokens=snap.tokens)
