@@ -23,7 +23,7 @@ import dataclasses
 import heapq
 import threading
 from dataclasses import dataclass, field
-from typing import Any, Sequence
+from typing import Any, Callable, Sequence
 
 import torch
 
@@ -104,13 +104,16 @@ class PagePool:
             self.share(pages[:full])
             return list(pages[:full]) + own, list(pages[full:full + 1]) if rest else [], own
 
-    def compact(self) -> tuple[list[int], list[int]]:
+    def compact(self, move: Callable[[list[int], list[int]], None] | None = None) -> tuple[list[int], list[int]]:
         """(src ascending, dst): the moves after which the used pages are 0 .. used. The counts move with
-        them; whoever holds page numbers has to replace src[i] by dst[i]."""
+        them; whoever holds page numbers has to replace src[i] by dst[i]. ``move(src, dst)`` is called first
+        where there is something to move: what it raises leaves the pool as it was."""
         with self._lock:
             used = self.used
             src = [p for p in range(used, self.pages) if self._count[p]]
             dst = [p for p in range(used) if not self._count[p]]
+            if src and move is not None:
+                move(src, dst)
             for a, b in zip(src, dst):
                 self._count[b], self._count[a] = self._count[a], 0
             self._free = list(range(used, self.pages))
@@ -295,12 +298,10 @@ class Kv4States:
         with self._lock:
             self._moving = True
             try:
-                src, dst = self.pool.compact()
-                if src:
-                    self.cache.move_pages(src, dst, self.tables)
-                    to = dict(zip(src, dst))
-                    for pages in self._held.values():
-                        pages[:] = [to.get(p, p) for p in pages]
+                src, dst = self.pool.compact(lambda src, dst: self.cache.move_pages(src, dst, self.tables))
+                to = dict(zip(src, dst))
+                for pages in self._held.values():
+                    pages[:] = [to.get(p, p) for p in pages]
             finally:
                 self._moving = False
                 while self._dropped:

@@ -86,3 +86,30 @@ def test_only_one_copy_is_extended(states):
     assert states.extend(snap, 3) is not None
     fork = states.fork(twin)  # of the 20 tokens that it knows
     assert fork.tokens == 20 and len(fork.pages) == 2 and states.extend(fork, 1) is not None
+
+
+def test_a_compaction_whose_move_fails(states, monkeypatch):
+    """An error of the launch leaves counts, free pages, tables and states as they were; the next one moves them."""
+    hole = states.store(snapshot(33))
+    base = states.store(snapshot(40))
+    fork = states.fork(base)
+    del hole
+    gc.collect()
+    before = ([states.pool.references(p) for p in range(12)], states.pool.free, states.tables.tolist(), list(base.pages), list(fork.pages))
+
+    def fails(src, dst, tables):
+        raise RuntimeError("no launch")
+
+    monkeypatch.setattr(states.cache, "move_pages", fails, raising=False)
+    with pytest.raises(RuntimeError, match="no launch"):
+        states.compact()
+    assert before == ([states.pool.references(p) for p in range(12)], states.pool.free, states.tables.tolist(), base.pages, fork.pages)
+    got = states.pool.allocate(states.pool.free)
+    assert not set(got) & (set(base.pages) | set(fork.pages))
+    states.pool.release(got)
+    monkeypatch.undo()
+    assert states.compact() == 3
+    assert sorted(set(base.pages) | set(fork.pages)) == [0, 1, 2, 3] and base[0].table.tolist() == base.pages
+    del base, fork
+    gc.collect()
+    assert states.pool.used == 0
