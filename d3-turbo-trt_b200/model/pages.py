@@ -251,9 +251,14 @@ class Kv4States:
                     self.cache.append(layer, e.keys[0].transpose(0, 1), e.values[0].transpose(0, 1), slots)
             return snap
 
+    def _own(self, snap: Kv4Snapshot) -> None:
+        if not isinstance(snap, Kv4Snapshot) or snap.states is not self:
+            raise RuntimeError("not a snapshot that these states hold")
+
     def fork(self, snap: Kv4Snapshot) -> Kv4Snapshot | None:
         """A snapshot of the same state that can be extended by itself: its full pages are shared, a partly
         filled last one is copied in every layer. None where no page or row is free."""
+        self._own(snap)
         with self._lock:
             if not self._rows:
                 return None
@@ -269,7 +274,8 @@ class Kv4States:
         """int64 slots of ``count`` new tokens of ``snap``, to append K/V to in every layer; its entries then
         have them. Only for a snapshot whose last page is its own (a stored one that was not forked since,
         or a fork). None where no pages are free. The slots are places in the pool: append before the next
-        ``compact``."""
+        ``compact``. A ``StateCache`` counts the pages that a snapshot had when it was put: put it again."""
+        self._own(snap)
         with self._lock:
             page = self.cache.page_tokens
             if snap.tokens != snap.held.tokens:

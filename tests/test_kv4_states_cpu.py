@@ -12,6 +12,7 @@ from conftest import ROOT  # noqa: F401  (puts the repository on sys.path)
 
 from d3_turbo_trt_b200.kernels import kv4
 from d3_turbo_trt_b200.model import pages
+from d3_turbo_trt_b200.model.cache import StateCache
 from d3_turbo_trt_b200.model.snapshot import AttentionEntry
 
 
@@ -111,5 +112,33 @@ def test_a_compaction_whose_move_fails(states, monkeypatch):
     assert states.compact() == 3
     assert sorted(set(base.pages) | set(fork.pages)) == [0, 1, 2, 3] and base[0].table.tolist() == base.pages
     del base, fork
+    gc.collect()
+    assert states.pool.used == 0
+
+
+def test_snapshots_of_others_are_refused(states, monkeypatch):
+    """Another pool's page numbers mean nothing here."""
+    mine = states.store(snapshot(20))
+    monkeypatch.setattr(pages, "Kv4Cache", NotingCache)
+    other = pages.Kv4States(1, 12, kv_heads=1, head_dim=64, page_tokens=16, max_tokens=96, max_states=5)
+    theirs = other.store(snapshot(20))
+    for bad in (theirs, list(mine), snapshot(20)):
+        with pytest.raises(RuntimeError, match="not a snapshot"):
+            states.fork(bad)
+        with pytest.raises(RuntimeError, match="not a snapshot"):
+            states.extend(bad, 1)
+    assert states.pool.used == other.pool.used == 2 and len(states.cache.calls) == len(other.cache.calls) == 1
+
+
+def test_a_state_cache_counts_a_snapshot_put_again(states):
+    held = StateCache(10**6)
+    snap = states.store(snapshot(20))
+    first = held.put("a", snap, 20).nbytes
+    assert states.extend(snap, 30) is not None
+    assert held.put("a", snap, 50).nbytes == 2 * first == held.bytes and held.count == 1
+    del snap
+    gc.collect()
+    assert states.pool.used == 4
+    held.clear()
     gc.collect()
     assert states.pool.used == 0
