@@ -327,6 +327,8 @@ def question_attention(q: torch.Tensor, cache: Kv4Cache, layer: int, table: torc
         lengths = [int(n) for n in (lengths.tolist() if isinstance(lengths, torch.Tensor) else lengths)]
         if any(not 0 <= n <= width for n in lengths):
             raise RuntimeError(f"lengths must lie in [0, {width}]")
+    elif lengths.dim() != 1:
+        raise RuntimeError(f"lengths must be [{rows}], got {tuple(lengths.shape)}")
     if len(lengths) != rows:
         raise RuntimeError(f"{len(lengths)} lengths for {rows} question blocks")
     q, k_q, v_q = _lib.rows16(q), _lib.rows16(k_q), _lib.rows16(v_q)

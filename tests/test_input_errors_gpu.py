@@ -102,3 +102,13 @@ def test_a_wait_that_gave_up_goes_first():
     assert _lib.lib().d3b_selftest_wait_timeout(200, None) == _lib.OK
     torch.cuda.synchronize()
     assert _lib.device_error() == 9001 and _lib.device_error() == 0
+
+
+def test_lengths_of_another_shape_are_refused():
+    """A table of lengths per block and something else: its first column is not its first elements."""
+    cache, table = kv4.Kv4Cache(1, 4, kv_heads=2, head_dim=64, page_tokens=16), i32([0, 1, 2, 3])
+    q, k = new(2, 4, 3, 64), new(2, 2, 3, 64)
+    for lengths in (i32([[3, 1], [2, 1]]), i32([[3], [2]]), i32([3, 2, 1]), i32(3), torch.tensor([[3, 1], [2, 1]])):
+        with pytest.raises((RuntimeError, TypeError)):
+            kv4.question_attention(q, cache, 0, table, 40, k, k, lengths, scale=0.1)
+    assert _lib.device_error() == 0
