@@ -45,6 +45,7 @@ namespace d3b_kv4 {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr float kHead = 8.f, kRoom = 15.f;
+constexpr float kNone = -3e38f;  // m before any key: finite, so that a score of -infinity has no weight then either
 // Powers of V rows are kept as their bytes (biased by 127).
 constexpr int kLeastPower = kExpMin + 127;  // of rows of zeros
 constexpr int kFirst = 119, kAbove = 3;

@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int row = n * 8 + 2 * c + j;
-        m[n][j] = -INFINITY;
+        m[n][j] = kNone;
         l[n][j] = 0.f;
         qf[n][j] = factors[row];
         limit[n][j] = a.causal ? len - (a.L - 1 - (row0 + row) / a.group) : len;
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
         }
       };
       uint32_t wf[P::GP][NT][2];
-      // m = -infinity (no key yet) makes every exponent +infinity
+      // before any key m makes every finite score pass kRoom
       if (__any_sync(0xffffffffu, exponents() > kRoom || odd)) {
         int band0 = 0, band1 = 0;  // the step's bands; the common products below are those of band 0
         if (__any_sync(0xffffffffu, odd)) {
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
                 if (in) top = fmaxf(top, fmaf(s[i][n][j + 2 * h], kq[i][h] * qf[n][j], -kHead));
               }
             const float now = fmaxf(old, max_over_rows(top));
-            const float keep = ex2(old - finite_or_zero(now));
+            const float keep = ex2(old - now);
             m[n][j] = now;
             l[n][j] *= keep;
 #pragma unroll

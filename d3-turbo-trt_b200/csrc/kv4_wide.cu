@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int row = n * 8 + 2 * c + j;
-        m[n][j] = -INFINITY;
+        m[n][j] = kNone;
         l[n][j] = 0.f;
         qf[n][j] = factors[row];
         limit[n][j] = a.causal ? len - (a.L - 1 - (row0 + row) / a.group) : len;
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float now = j ? top.y : top.x, keep = ex2(m[n][j] - finite_or_zero(now));
+          const float now = j ? top.y : top.x, keep = ex2(m[n][j] - now);
           m[n][j] = now;
           l[n][j] *= keep;
 #pragma unroll
@@ -318,8 +318,8 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
       // rows 2 (lane % 8) and the one behind it
       const uint32_t rel = relative(two_bytes(lds_u16(mine + 2 * (lane & 7))), E);
       const bool odd = !in_band(rel);
-      // Behind this barrier every warp's copies have landed and its work on the other half is done. m = -infinity (no key
-      // yet) makes every exponent +infinity.
+      // Behind this barrier every warp's copies have landed and its work on the other half is done. Before any key m
+      // makes every finite score pass kRoom.
       const bool move = __syncthreads_or(exponents(edge, masked) > kRoom || odd);
       if (lane < 8) vfs[8 * warp + lane] = band_factors(rel);
       load_v(p + 1, id_v, kHalfRing - half);

@@ -237,3 +237,22 @@ def test_own_key_with_a_score_of_minus_infinity(monkeypatch, in_place, dim, head
         check_rows(got[b], q[b], torch.cat([ks, kq[b][:, keep].double()], 1), torch.cat([vs, vq[b][:, keep].double()], 1), scale, True)
     kv4._plans_of.cache_clear()
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("dim,heads", [(64, 4), (128, 8), (256, 6)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_a_share_of_nothing_but_minus_infinity(monkeypatch, in_place, dim, heads, dtype):
+    """The only own key has a score of -infinity, and its tile is a CTA's whole share: no weight, not NaN."""
+    monkeypatch.setattr(kv4, "_reads_codes", lambda *a: in_place)
+    kv4._plans_of.cache_clear()
+    for state in (640, 5000):
+        k, v = rows((state, 1, dim), dtype, 1, 0.2), rows((state, 1, dim), dtype, 2, 0.2)
+        cache, table, ks, vs = cache_of(k, v, 32)
+        q, kq, vq = (rows((1, n, 1, dim), dtype, s, 0.2) for n, s in ((heads, 3), (1, 4), (1, 5)))
+        q[..., 0] = q[..., 0].abs() + 1
+        kq[..., 0] = -math.inf
+        got = kv4.question_attention(q.cuda(), cache, 0, table, state, kq.cuda(), vq.cuda(), [1], scale=dim**-0.5)
+        check_rows(got[0], q[0], ks, vs, dim**-0.5, True)
+    kv4._plans_of.cache_clear()
+    assert _lib.device_error() == 0
