@@ -169,7 +169,7 @@ def check(status: int, what: str) -> None:
 
 
 def stream_of(t: torch.Tensor) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+    return ctypes.c_void_p(raw_stream(t.device.index))
 
 
 def ptr(t: torch.Tensor | None) -> ctypes.c_void_p:

@@ -37,9 +37,10 @@ KERNEL_NAME = "sm100a"
 # outside [0, L] (the entry is clamped; read it with _lib.device_error()).
 SITE_BAD_LENGTH = 2010
 
-# Tables of lengths given on the host, with the stream that each was made on, and those that captured calls read:
-# a graph keeps an address, so the latter stay for good.
-_LENGTHS: "OrderedDict[tuple, tuple[torch.Tensor, int]]" = OrderedDict()
+# Tables of lengths given on the host, with the streams that each is known to (its own, and those whose work its
+# memory waits for before it is used again), and those that captured calls read: a graph keeps an address, so
+# the latter stay for good.
+_LENGTHS: "OrderedDict[tuple, tuple[torch.Tensor, set[int]]]" = OrderedDict()
 _LENGTHS_MAX = 16
 _LENGTHS_CAPTURED: dict[tuple, torch.Tensor] = {}
 _LENGTHS_LOCK = threading.Lock()
@@ -54,7 +55,7 @@ def _workspace(device: torch.device, nbytes: int) -> torch.Tensor | None:
     if nbytes == 0:
         return None
     index = device.index if device.index is not None else torch.cuda.current_device()
-    key = (index, torch.cuda.current_stream(index).cuda_stream)
+    key = (index, _lib.raw_stream(index))
     buf = _WORKSPACES.get(key)
     if buf is None or buf.numel() < nbytes:
         buf = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
@@ -91,8 +92,11 @@ def _stream_now(device: torch.device) -> tuple[int, bool]:
     """The device's current stream, and whether it is being captured."""
     if device.type != "cuda":
         return 0, False
+    now = torch.cuda.current_device()
+    if device.index == now:  # without a context: this is in every call's way
+        return _lib.raw_stream(now), torch.cuda.is_current_stream_capturing()
     with torch.cuda.device(device):
-        return torch.cuda.current_stream().cuda_stream, torch.cuda.is_current_stream_capturing()
+        return _lib.raw_stream(torch.cuda.current_device()), torch.cuda.is_current_stream_capturing()
 
 
 def block_offsets(lengths: Sequence[int] | torch.Tensor, device: torch.device) -> torch.Tensor:
@@ -104,8 +108,8 @@ def block_offsets(lengths: Sequence[int] | torch.Tensor, device: torch.device) -
     if isinstance(lengths, torch.Tensor):
         if lengths.is_cuda and lengths.dtype == torch.int32 and lengths.device == device:
             return lengths.contiguous()
-        lengths = [int(n) for n in lengths.tolist()]
-    key = (tuple(int(n) for n in lengths), str(device))
+        lengths = lengths.tolist()
+    key = (tuple(lengths), str(device))
     stream, capturing = _stream_now(device)
     with _LENGTHS_LOCK:
         kept = _LENGTHS_CAPTURED.get(key)
@@ -113,21 +117,22 @@ def block_offsets(lengths: Sequence[int] | torch.Tensor, device: torch.device) -
             return kept
         hit = _LENGTHS.get(key)
         if hit is not None:
-            table, made_on = hit
+            table, streams = hit
             _LENGTHS.move_to_end(key)
             if capturing:
                 _LENGTHS_CAPTURED[key] = table
-            elif stream != made_on:  # its memory is used again only after this stream's work so far
+            elif stream not in streams:
                 table.record_stream(torch.cuda.current_stream(device))
+                streams.add(stream)
             return table
     if capturing:
         raise RuntimeError("lengths on the host in a captured call: make the call once before the capture, or give "
                            "the lengths as an int32 device tensor")
-    table = torch.tensor(key[0], dtype=torch.int32).to(device, non_blocking=False)
+    table = torch.tensor([int(n) for n in key[0]], dtype=torch.int32).to(device, non_blocking=False)
     with _LENGTHS_LOCK:
         while len(_LENGTHS) >= _LENGTHS_MAX:
             _LENGTHS.popitem(last=False)
-        _LENGTHS[key] = (table, stream)
+        _LENGTHS[key] = (table, {stream})
     return table
 
 
