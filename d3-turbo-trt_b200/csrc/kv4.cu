@@ -10,7 +10,7 @@
 //
 // Measured (B200, launched back to back): append 16384 tokens x 4 heads x 128 12.5 us (43 MB: 3.4 TB/s; it is
 // the instructions of the quantisation that bound it, issue slots three quarters busy), x 256 22.7 us; read of
-// the same 10.4 and 18.6 us (4.1 and 4.6 TB/s, bytes); 700 pages of 16 layers, 64 tokens x 4 heads x 128, moved in
+// the same 10.4 and 18.6 us (4.1 and 4.6 TB/s; widening the codes keeps the ALU 71 % busy, waits for loads follow); 700 pages of 16 layers, 64 tokens x 4 heads x 128, moved in
 // 131 us (6.4 TB/s read and written, as a plain copy).
 #include "kv4.cuh"
 

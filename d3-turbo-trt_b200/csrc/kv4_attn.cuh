@@ -20,7 +20,7 @@
 // through the products once for every band of 19 powers that has rows, each with weights under their own
 // maxima, and the fp32 sums go to O under the band's power. So a row keeps its weight whatever the others'
 // magnitudes are; what it costs is another pass over the step's codes a band, with sums of its own (64 sequences of
-// 16000 tokens, 8 rows x 128, with every 37th V row 2^30 times the others: 510 us instead of 129). Rows at the
+// 16000 tokens, 8 rows x 128, with every 37th V row 2^30 times the others: 520 us instead of 129). Rows at the
 // least power (all values under 2^-52; rows of zeros) count as zeros where E is more than 14 above it, as it is
 // at first.
 //

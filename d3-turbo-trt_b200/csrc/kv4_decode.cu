@@ -114,7 +114,7 @@ struct Plan {
 
 // Up to 8 rows a kv head (16 where O for 16 rows still fits a warp's registers) go to the thin kernel,
 // whose warps work alone; more rows to the wide one, which decodes each code once for up to 32 rows.
-// 64 sequences of 16000 tokens, 4 heads: 8 rows x 256 221 us thin and 354 wide, 8 x 128 128 and 240, 16 x 128 181
+// 64 sequences of 16000 tokens, 4 heads: 8 rows x 256 225 us thin and 354 wide, 8 x 128 129 and 240, 16 x 128 178
 // and 242; below 16 sequences of 4000 the two are within 2 us of each other.
 bool make_plan(const d3b_kv4_cache* c, int B, int H, int L, int64_t keys, bool own, Plan* p) {
   const int D = c->head_dim;

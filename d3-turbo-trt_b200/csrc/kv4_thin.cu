@@ -6,10 +6,10 @@
 //
 // Bound: the cache's bytes, 18 D + 32 for 16 tokens and kv head, with the ALU close behind: a code
 // pair costs a conversion (64 lanes a clock and SM) and a product with its scale. Measured (B200, 4 kv heads,
-// up to 8 rows): 64 sequences of 16000 tokens D = 128 128 us (4.7 TB/s, 0.71 of a plain copy's rate), D = 256
-// 221 us (5.4 TB/s, 0.82); D = 64, 2 heads, 49 us (3.1 TB/s: the instructions for a key do not halve with D). At 64
-// ragged sequences up to 16384 the loads alone took 91 us, the arithmetic alone 99, both 104 to 109. One token
-// of one sequence of 1000 10 us.
+// up to 8 rows): 64 sequences of 16000 tokens D = 128 129 us (4.7 TB/s, 0.71 of a plain copy's rate), D = 256
+// 225 us (5.3 TB/s, 0.81); D = 64, 2 heads, 48 us (3.1 TB/s: the instructions for a key do not halve with D). At 64
+// ragged sequences up to 16384 the loads alone took 91 us, loads and arithmetic together take 104. One token of
+// one sequence of 1000 8.3 us at D = 128.
 #include "kv4_attn.cuh"
 
 namespace d3b_kv4 {
@@ -29,7 +29,8 @@ struct Thin {
   static constexpr int kStage = (granule_bytes(D) + 127) / 128 * 128;  // V rows start on 128-byte lines
   static constexpr int kRows = 8 * NT;
   // CTAs an SM. 8 rows x 64 with 4 of them, 64 x 16000 keys, 49 us, with 5 (registers spilled) and 3 51; 16 x 64 with 3
-  // 64 us, with 2 70; 16 x 128 with 3 175 against 181, but one sequence of 16000 19 against 17 us
+  // 64 us, with 2 70; 16 x 128 with 3 175 against 181, but one sequence of 16000 19 against 17 us. (Measured before V's
+  // powers went into the scales; at these choices 48, 64 and 178 us now.)
   static constexpr int kResident = NT == 1 ? (D == 64 ? 4 : 3) : (D == 64 ? 3 : 2);
   static constexpr int kWarpRing = kDepth * GP * kStage;
   static constexpr int kRing = kWarps * kWarpRing;

@@ -13,8 +13,8 @@
 // Bound: products. 32 rows x 64 keys are 2 D m16n8k16, 8 clocks each on one of four tensor pipes; at D = 256 they
 // take 1.3 times as long as the cache's bytes, and the chain conversion, product with the scale, matrix
 // instruction leaves the pipes idle half the time with two warps a scheduler. Measured (B200): three sequences of
-// up to 98765 tokens, 5 x 6 rows, 4 heads x 256: 130 us with the merge (210 TFLOP/s, 2.0 TB/s of codes); one block of
-// 11 tokens x 8 heads over 4096 tokens of 4 x 128 18 us. Tried and slower: 8 warps a CTA (162 us), 3 CTAs an SM (157
+// 98765 tokens, 5 x 6 rows, 4 heads x 256: 155 us with the merge (235 TFLOP/s, 2.2 TB/s of codes); one block of
+// 11 tokens x 8 heads over 4096 tokens of 4 x 128 16 us. Tried and slower: 8 warps a CTA (162 us), 3 CTAs an SM (157
 // us: spills); no faster: 128 keys a tile with two granules a warp (137 against 136 us then).
 #include "kv4_attn.cuh"
 

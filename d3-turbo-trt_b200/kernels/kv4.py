@@ -3,8 +3,8 @@
 ``Kv4Cache`` is a pool of pages for every layer; a page holds ``page_tokens`` tokens' keys and
 values of all kv heads. A row is kept as e2m1 codes with one e4m3 scale for 16 channels and one
 power of two: 4.56 bits a value at head_dim 128, against 16 in a snapshot (the layout is written
-down in ``include/d3b200.h``). What a row reads back as is exactly representable in bf16 and, up to
-its largest magnitude, in fp16.
+down in ``include/d3b200.h``). What a row reads back as is exact in bf16 and, between fp16's
+subnormals and its largest magnitude, in fp16.
 
 * ``cache.append(layer, k, v, slots)`` quantises rows into slots (page * page_tokens + place);
 * ``cache.read(layer, table, tokens)`` gives a sequence's rows back in 16 bits;

@@ -14,7 +14,7 @@ cfg4 (readout 255 x 5120 x 255; snapshot: the 64-layer state snapshot at a
 255 blocks x 48 tokens x 48 value heads; gdn_state: one GDN layer's state pass,
 4096 tokens x 48 value heads with a final state; gated_norm_fp8, causal_conv,
 qk_norm_rope: the backbone's glue kernels at the question pass's 255 x 48 tokens).
-Kernels over the 4-bit cache have shapes of their own: kv4_append (16384 tokens), kv4_decode
+Kernels over the 4-bit cache have shapes of their own: kv4_append and kv4_read (16384 tokens), kv4_decode
 (64 sequences of 16384 tokens, 32/4 heads x 128), kv4_verify (3 sequences of 98765, five new
 tokens each, 24/4 heads x 256), kv4_question (one block of 11 tokens over 4096); qk_norm_mrope
 is 255 x 48 tokens of 32/4 heads x 128.
@@ -206,7 +206,8 @@ def _glue(kernel: str, dev: torch.device, rows: int = 255, T: int = 48):
 def _kv4(kernel: str, dev: torch.device):
     from .kernels import kv4
 
-    B, n, L, H, Hkv, D = {"kv4_append": (1, 16384, 1, 4, 4, 128), "kv4_decode": (64, 16384, 1, 32, 4, 128),
+    B, n, L, H, Hkv, D = {"kv4_append": (1, 16384, 1, 4, 4, 128), "kv4_read": (1, 16384, 1, 4, 4, 128),
+                          "kv4_decode": (64, 16384, 1, 32, 4, 128),
                           "kv4_verify": (3, 98765, 5, 24, 4, 256), "kv4_question": (1, 4096, 11, 32, 4, 128)}[kernel]
     g = torch.Generator(device=dev).manual_seed(7)
     page = 64
@@ -221,6 +222,8 @@ def _kv4(kernel: str, dev: torch.device):
     codes = (18 * D + 32) / 16
     if kernel == "kv4_append":
         return (lambda: cache.append(0, k, v, slots)), {"bytes": n * Hkv * (row + codes)}
+    if kernel == "kv4_read":
+        return (lambda: cache.read(0, table[0], n)), {"bytes": n * Hkv * (row + codes)}
     q = torch.randn(B, H, L, D, generator=g, device=dev).to(torch.bfloat16)
     work = {"bytes": B * n * Hkv * codes, "flops": 4.0 * B * H * L * n * D}
     if kernel == "kv4_question":
@@ -278,7 +281,7 @@ def main() -> None:
     ap.add_argument("--kernel", required=True,
                     choices=["attention", "gemm_fp8", "gemm_int8", "act_quant_fp8", "act_quant_int8", "readout",
                              "snapshot", "gdn", "gdn_recurrent", "gdn_state", "gated_norm_fp8", "causal_conv",
-                             "qk_norm_rope", "qk_norm_mrope", "kv4_append", "kv4_decode", "kv4_verify", "kv4_question"])
+                             "qk_norm_rope", "qk_norm_mrope", "kv4_append", "kv4_read", "kv4_decode", "kv4_verify", "kv4_question"])
     ap.add_argument("--config", default="cfg3a", choices=[*ATTN, "state4k", "cfg2", "cfg4"])
     ap.add_argument("--launches", type=int, default=3)
     ap.add_argument("--warmup", type=int, default=1)

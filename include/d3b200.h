@@ -455,7 +455,7 @@ D3B_API int d3b_kv4_append(const d3b_kv4_cache* cache, int64_t layer, const void
 
 /*
  * The first `tokens` rows of a sequence: k, v [kv_heads, tokens, head_dim] contiguous, dtype f16
- * or bf16 (exact; a magnitude above the type's largest becomes the largest).
+ * or bf16 (exact but among f16's subnormals; a magnitude above the type's largest becomes the largest).
  *   table [n_pages] int32 on the device, n_pages * page_tokens >= tokens. Rows of a page number
  *   outside the pool read as zeros.
  */
