@@ -15,12 +15,12 @@
 //
 // e_j, a V row's power, goes into its scale: code * scale * 2^d is exact in fp16 for d from -14 to 4
 // (a multiple of 2^-24, at most 43008). E is one power for all of a unit's rows that a warp (thin) or a CTA
-// (wide) sees: kFirst, for rows whose largest value is 2^-10 to 2^7, or, where the first rows that are not zeros go
-// beyond that, kAbove over their largest. A step with powers outside E - 14 .. E + 4 is banded: its V rows go
+// (wide) sees: kFirst, for rows whose largest value is 2^-10 to 2^7, or, where none of the first rows that are not
+// zeros is such a one, kAbove over their largest. A step with powers outside E - 14 .. E + 4 is banded: its V rows go
 // through the products once for every band of 19 powers that has rows, each with weights under their own
 // maxima, and the fp32 sums go to O under the band's power. So a row keeps its weight whatever the others'
 // magnitudes are; what it costs is another pass over the step's codes a band, with sums of its own (64 sequences of
-// 16000 tokens, 8 rows x 128, with every 37th V row 2^30 times the others: 520 us instead of 129). Rows at the
+// 16000 tokens, 8 rows x 128, with every 37th V row 2^30 times the others: 446 us instead of 130). Rows at the
 // least power (all values under 2^-52; rows of zeros) count as zeros where E is more than 14 above it, as it is
 // at first.
 //
@@ -217,25 +217,32 @@ __device__ __forceinline__ uint32_t band_factors(uint32_t two, int E, int k) {
 }
 __device__ __forceinline__ int band_of(int e, int E) { return (e - E + kDown + kBand * 16) / kBand - 16; }
 
-// E after rows of power `top` at most; first: no row but those of zeros came before
-__device__ __forceinline__ int next_power(int E, int top, bool first) {
-  return top > kLeastPower && (first || top > E + kFar) ? min(top + kAbove, kMostPower) : E;
-}
-
-// What a step's rows span, marked rows and those at the least power apart: the largest power (0: no row) and the
-// smallest (255).
+// What a step's rows span, marked rows and those at the least power apart: the largest power (0: no row), the
+// smallest (255), and whether there is one in E's band.
 struct Span {
-  int most, least;
-  __device__ __forceinline__ void add(uint32_t two) {
+  int most, least, near;
+  // two rows' powers, of which the first `live` are of keys
+  __device__ __forceinline__ void add(uint32_t two, int live, int E) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int e = (two >> (16 * h)) & 0xFF;
-      if (e == 255 || e == kLeastPower) continue;
+      if (h >= live || e == 255 || e == kLeastPower) continue;
       most = max(most, e);
       least = min(least, e);
+      near |= (uint32_t)(e - E + kDown) < (uint32_t)kBand;
     }
   }
+  __device__ __forceinline__ void over_warp() {
+    most = (int)__reduce_max_sync(0xffffffffu, (uint32_t)most);
+    least = (int)__reduce_min_sync(0xffffffffu, (uint32_t)least);
+    near = (int)__reduce_or_sync(0xffffffffu, (uint32_t)near);
+  }
 };
+
+// E after a step; first: no row but those of zeros came before
+__device__ __forceinline__ int next_power(int E, const Span& s, bool first) {
+  return s.most > 0 && ((first && !s.near) || s.most > E + kFar) ? min(s.most + kAbove, kMostPower) : E;
+}
 
 // the power of two that brings a row's largest finite magnitude to [2^14, 2^15), as far as 2^126 goes
 __device__ __forceinline__ int row_up(float top) { return min(126, 14 - ((int)(__float_as_uint(top) >> 23) - 127)); }

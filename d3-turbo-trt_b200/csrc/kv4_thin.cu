@@ -328,17 +328,16 @@ __global__ void __launch_bounds__(kThreads, Thin<D, NT>::kResident) thin_kernel(
       if (__any_sync(0xffffffffu, exponents() > kRoom || odd)) {
         int band0 = 0, band1 = 0;  // the step's bands; the common products below are those of band 0
         if (__any_sync(0xffffffffu, odd)) {
-          Span span = {0, 255};
+          Span span = {0, 255, 0};
 #pragma unroll
           for (int i = 0; i < P::GP; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               if (lds_u8(e_at + kAt + i * P::kStage + P::kVe - P::kKe + 8 * h) == 255u) kq[i][h] = __int_as_float(0x7FC00000);
-              span.add(powers(i, h));
+              span.add(powers(i, h), live[i] - 2 * c - 8 * h, E);
             }
-          span.most = (int)__reduce_max_sync(0xffffffffu, (uint32_t)span.most);
-          span.least = (int)__reduce_min_sync(0xffffffffu, (uint32_t)span.least);
-          const int zeros = zero_steps[warp], to = next_power(E, span.most, zeros == now);
+          span.over_warp();
+          const int zeros = zero_steps[warp], to = next_power(E, span, zeros == now);
           __syncwarp();
           if (lane == 0 && span.most == 0) zero_steps[warp] = zeros + 1;
           __syncwarp();

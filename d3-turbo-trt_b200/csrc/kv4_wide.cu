@@ -362,10 +362,9 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
         }
       };
       if (move) {
-        Span span = {0, 255};
-        span.add(two_bytes(lds_u16(mine + 2 * (lane & 7))));
-        span.most = (int)__reduce_max_sync(0xffffffffu, (uint32_t)span.most);
-        span.least = (int)__reduce_min_sync(0xffffffffu, (uint32_t)span.least);
+        Span span = {0, 255, 0};
+        span.add(two_bytes(lds_u16(mine + 2 * (lane & 7))), live_now - 2 * (lane & 7), E);
+        span.over_warp();
         if (lane == 0) spans[warp] = span;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -377,8 +376,9 @@ __global__ void __launch_bounds__(kThreads, Wide<D, NT>::kResident) wide_kernel(
         for (int w = 0; w < kWarps; ++w) {
           span.most = max(span.most, spans[w].most);
           span.least = min(span.least, spans[w].least);
+          span.near |= spans[w].near;
         }
-        const int to = next_power(E, span.most, zero_tiles == p - piece0);
+        const int to = next_power(E, span, zero_tiles == p - piece0);
         zero_tiles += span.most == 0;
         if (to != E) rescale(power_of(E - to));
         E = to;

@@ -488,8 +488,8 @@ D3B_API int d3b_kv4_move_pages(const d3b_kv4_cache* cache, const int32_t* src, c
  * of a row's largest and less loses bits), whatever the rows' magnitudes are beside each other; a softmax
  * weight is rounded to fp16's 11 bits, and below 2^-22 of its row's largest to 2^-33 of that; sums are
  * fp32. V rows whose values are all below 2^-52 may count as zeros. V rows whose largest value lies outside
- * 2^-10 to 2^7 (or, where a sequence's first rows do, outside 2^-11 to 2^7 of theirs) cost further passes
- * over their keys.
+ * 2^-10 to 2^7 (or, where all of a sequence's first rows do, outside 2^-11 to 2^7 of theirs) cost further
+ * passes over their keys.
  * Results do not change from call to call.
  */
 D3B_API size_t d3b_kv4_decode_workspace_size(const d3b_kv4_cache* cache, int B, int H, int L, int64_t width);
