@@ -147,6 +147,7 @@ class Kv4Entry:
 
     @property
     def held_bytes(self) -> int:
+        """Bytes of the layer's pages; those that a fork shares count for each state that does."""
         return self.table.numel() * self.cache.pool.shape[2]
 
 
